@@ -448,6 +448,125 @@ int sdc_abft_correct_fp8_block(const uint8_t* a, const uint8_t* b_rows,
                                uint16_t* d_rowmajor, uint8_t* corrected,
                                sdc_stream_t stream);
 
+/* ---- layer operators beside the protected GEMMs (extension) --------------
+ * None of these has a counterpart in the reference. Element types: 0 fp32,
+ * 1 bf16, 2 fp16; arithmetic is fp32 with one rounding at the store.
+ *
+ * Norm of each query and key head and rotation by position, one pass.
+ * q [batch, sequence, heads_q, dim], k [batch, sequence, heads_k, dim] with
+ * element strides {batch, sequence, head} and a unit last stride; dim even,
+ * <= 512. With weights [dim] (type of the heads, or fp32 when weight_f32):
+ * u = x * rsqrt(mean(x^2) + eps) * weight per head; null weights: u = x.
+ * Then pair p < rotary/2 -- elements (p, p + rotary/2), or (2p, 2p+1) when
+ * interleaved -- turns by the angle whose cosine and sine are
+ * table[position][p] and table[position][rotary/2 + p] (fp32
+ * [table_rows, rotary]); elements from `rotary` on pass. positions: int32 or
+ * int64 with strides {batch, sequence}; one outside the table gives NaN.
+ * Outputs are contiguous. heads_k may be 0. */
+int sdc_head_norm_rotary(int dtype, const void* q, const int64_t* q_strides,
+                         const void* k, const int64_t* k_strides,
+                         int64_t batch, int64_t sequence, int heads_q,
+                         int heads_k, int dim, const float* table,
+                         int64_t table_rows, int rotary, int interleaved,
+                         const void* positions, int positions_64,
+                         const int64_t* position_strides, const void* q_weight,
+                         const void* k_weight, int weight_f32, float eps,
+                         void* q_out, void* k_out, sdc_stream_t stream);
+/* Gradients of the above: dq, dk contiguous, and, with weights, dq_weight,
+ * dk_weight [dim] (type of the weights; summed in a fixed order through the
+ * workspace). The forward's inputs are read again; nothing else is saved. */
+size_t sdc_head_norm_rotary_workspace_bytes(int64_t batch, int64_t sequence,
+                                            int heads_q, int heads_k, int dim);
+int sdc_head_norm_rotary_backward(
+    int dtype, const void* dq_out, const int64_t* dq_strides,
+    const void* dk_out, const int64_t* dk_strides, const void* q,
+    const int64_t* q_strides, const void* k, const int64_t* k_strides,
+    int64_t batch, int64_t sequence, int heads_q, int heads_k, int dim,
+    const float* table, int64_t table_rows, int rotary, int interleaved,
+    const void* positions, int positions_64, const int64_t* position_strides,
+    const void* q_weight, const void* k_weight, int weight_f32, float eps,
+    void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+    size_t workspace_bytes, sdc_stream_t stream);
+
+/* Low-rank adapters of many requests. `rows` int32 [slots...] lists tokens
+ * grouped by adapter, tokens without one last; `tiles` int32 [tile_count][3]
+ * are runs of it: {first slot, slots (<= tile_rows, 16 or 64), adapter or -1}.
+ * Types: bf16 or fp16. Rank <= 256.
+ *
+ * shrink: low[slot, :] = scale[adapter] * x[rows[slot], :] . weight^T, weight
+ * [adapters, rank, width], or [adapters, width, rank] when weight_rank_minor.
+ * low: two planes [2][slots][rank padded to 16] of the element type (the
+ * value rounded, and what the rounding left), sdc_adapter_low_bytes. */
+size_t sdc_adapter_low_bytes(int64_t slots, int rank);
+int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride,
+                       int64_t tokens, const int32_t* rows,
+                       const int32_t* tiles, int64_t tile_count, int tile_rows,
+                       const void* weight, int adapters, int rank,
+                       int64_t width, int weight_rank_minor,
+                       const float* scale, void* low, int64_t slots,
+                       sdc_stream_t stream);
+/* expand: out[token, :] = base[token, :] (null: 0) + low . weight over the
+ * rank; tiles with adapter -1 copy base. out may be base. after_shrink: the
+ * call directly follows the sdc_adapter_shrink that writes low on the same
+ * stream, so its loads of weights and base may overlap it. */
+int sdc_adapter_expand(int dtype, const void* base, int64_t base_stride,
+                       int64_t tokens, const int32_t* rows,
+                       const int32_t* tiles, int64_t tile_count, int tile_rows,
+                       const void* weight, int adapters, int rank,
+                       int64_t width, int weight_rank_minor, const void* low,
+                       int64_t slots, int after_shrink, void* out,
+                       int64_t out_stride, sdc_stream_t stream);
+/* outer: out[adapter] = sum over its slots (group_offsets int32
+ * [adapters + 1]) of x[rows[slot], :] outer low[slot, :], as
+ * [adapters, width, rank] when out_rank_minor, else [adapters, rank, width].
+ * Adapters without slots get zeros. */
+int sdc_adapter_outer(int dtype, const void* x, int64_t x_stride,
+                      int64_t tokens, const int32_t* rows,
+                      const int32_t* group_offsets, int adapters,
+                      const void* low, int64_t slots, int rank, int64_t width,
+                      int out_rank_minor, void* out, sdc_stream_t stream);
+
+/* Distillation loss of student logits [rows, vocab] (row_stride elements
+ * apart) against the teacher's list of `top` (<= 1024) indices (int32 or
+ * int64; negative: no entry) and logits a row:
+ *   p = softmax(teacher / temperature) over the list's entries,
+ *   loss = temperature^2 * sum p (ln p - ln softmax(student / temperature)).
+ * A row without entries has loss 0 and gradient 0; an index >= vocab makes
+ * the row NaN. stats: fp32 [rows, 4], 16-byte aligned, for the backward pass.
+ * grad_loss: null (1), or fp32 with stride 0 (one value) or 1 (one a row).
+ * loss_and_grad reads the logits once when a row fits the shared memory of a
+ * cluster (about 880000 16-bit or 440000 fp32 logits); grad may be the
+ * logits themselves. */
+int sdc_distill_loss(int dtype, const void* logits, int64_t rows,
+                     int64_t vocab, int64_t row_stride, const void* indices,
+                     int indices_64, int64_t index_stride, const void* teacher,
+                     int teacher_dtype, int64_t teacher_stride, int top,
+                     float temperature, float* loss, float* stats,
+                     sdc_stream_t stream);
+/* out fp32 [2]: the sum (or mean over the rows that have entries) of the
+ * losses, and the factor each row's loss had in it. */
+int sdc_distill_reduce(const float* loss, const float* stats, int64_t rows,
+                       int mean, float* out, sdc_stream_t stream);
+/* grad_scale: nullable fp32 [1], a further factor (out[1] of the reduction). */
+int sdc_distill_backward(int dtype, const void* logits, int64_t rows,
+                         int64_t vocab, int64_t row_stride,
+                         const void* indices, int indices_64,
+                         int64_t index_stride, const void* teacher,
+                         int teacher_dtype, int64_t teacher_stride, int top,
+                         float temperature, const float* stats,
+                         const float* grad_loss, int64_t grad_loss_stride,
+                         const float* grad_scale, void* grad,
+                         int64_t grad_stride, sdc_stream_t stream);
+int sdc_distill_loss_and_grad(int dtype, const void* logits, int64_t rows,
+                              int64_t vocab, int64_t row_stride,
+                              const void* indices, int indices_64,
+                              int64_t index_stride, const void* teacher,
+                              int teacher_dtype, int64_t teacher_stride,
+                              int top, float temperature,
+                              const float* grad_loss, int64_t grad_loss_stride,
+                              float* loss, float* stats, void* grad,
+                              int64_t grad_stride, sdc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

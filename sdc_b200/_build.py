@@ -7,7 +7,8 @@ Two shared objects are produced next to this file:
   CUDA runtime statically and reaches the driver's tensor-map encoder through
   ``cudaGetDriverEntryPoint``, so it has no torch or libcuda link dependency.
 * ``_sdc_ops.so`` — the thin torch extension registering the reference's
-  ``sdc_cutlass::*`` operator schemas on top of that ABI (loaded with
+  ``sdc_cutlass::*`` operator schemas, and the layer operators beside them, on
+  top of that ABI (loaded with
   ``torch.ops.load_library``; it has no Python module of its own).
 
 Builds are incremental on source modification times, so importing the package
@@ -38,7 +39,11 @@ CUDA_SOURCES = [
     "augmented.cu",
     "kslice.cu",
     "rowsum.cu",
+    "rotary.cu",
+    "adapters.cu",
+    "distill.cu",
 ]
+OPS_SOURCES = ["torch_ops.cpp", "torch_layers.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -101,8 +106,8 @@ def build_ops(verbose: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "torch_ops.cpp"
-    if not _stale(OPS, [src, INCLUDE / "sdc_b200.h", LIB]):
+    sources = [CSRC / s for s in OPS_SOURCES]
+    if not _stale(OPS, [*sources, INCLUDE / "sdc_b200.h", LIB]):
         return OPS
     includes = []
     for path in cpp_extension.include_paths("cuda"):
@@ -111,7 +116,7 @@ def build_ops(verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_sdc_ops",
-           *includes, "-I", str(INCLUDE), str(src), "-o", str(OPS), *libdirs,
+           *includes, "-I", str(INCLUDE), *map(str, sources), "-o", str(OPS), *libdirs,
            f"-L{HERE}", "-lsdc_b200", "-Wl,-rpath,$ORIGIN",
            "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda"]
     _run(cmd, verbose)

@@ -72,6 +72,25 @@ PROTOTYPES = {
     "sdc_abft_locate": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     "sdc_abft_correct_fp8": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "sdc_abft_correct_nvfp4": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sdc_head_norm_rotary": (_int, [_int, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _vp, _i64, _int, _int,
+                                    _vp, _int, _vp, _vp, _vp, _int, _float, _vp, _vp, _vp]),
+    "sdc_head_norm_rotary_workspace_bytes": (_size, [_i64, _i64, _int, _int, _int]),
+    "sdc_head_norm_rotary_backward": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int,
+                                             _int, _vp, _i64, _int, _int, _vp, _int, _vp, _vp, _vp, _int, _float,
+                                             _vp, _vp, _vp, _vp, _vp, _size, _vp]),
+    "sdc_adapter_low_bytes": (_size, [_i64, _int]),
+    "sdc_adapter_shrink": (_int, [_int, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp, _int, _int, _i64, _int, _vp, _vp,
+                                  _i64, _vp]),
+    "sdc_adapter_expand": (_int, [_int, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp, _int, _int, _i64, _int, _vp,
+                                  _i64, _int, _vp, _i64, _vp]),
+    "sdc_adapter_outer": (_int, [_int, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64, _int, _i64, _int, _vp, _vp]),
+    "sdc_distill_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _i64, _int, _float, _vp,
+                                _vp, _vp]),
+    "sdc_distill_reduce": (_int, [_vp, _vp, _i64, _int, _vp, _vp]),
+    "sdc_distill_backward": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _i64, _int, _float, _vp,
+                                    _vp, _i64, _vp, _vp, _i64, _vp]),
+    "sdc_distill_loss_and_grad": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _i64, _int, _float,
+                                         _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
 }
 
 

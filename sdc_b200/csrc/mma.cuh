@@ -1,0 +1,75 @@
+// Warp-level matrix instructions for the skinny products of the low-rank
+// adapters: 16-bit operands from shared memory, fp32 accumulators in
+// registers. Those products are bound by the streamed operand's bytes (a rank
+// of at most a few dozen against rows of thousands), so they need neither
+// tensor memory nor descriptors, and the fragments can be formed from any
+// row stride.
+#pragma once
+
+#include "layers.cuh"
+
+namespace sdc {
+
+// Four 8x8 matrices of 16-bit elements; lane l gives the address of row l % 8
+// of matrix l / 8.
+__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const void* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(row)));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, const void* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(row)));
+}
+
+// d[16 x 8] += a[16 x 16] b[16 x 8].
+template <typename T>
+__device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, const uint32_t* b);
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+__device__ __forceinline__ void cp_async16(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Eight elements from global to shared memory: asynchronously where the
+// source is 16-byte aligned and whole, else one by one with zeros beyond
+// `valid`. Either way visible after cp_async_wait and a barrier.
+template <typename T>
+__device__ __forceinline__ void copy8(T* shared, const T* global, int64_t valid, bool vector) {
+  if (vector && valid >= 8) {
+    cp_async16(shared, global);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) shared[i] = i < valid ? global[i] : from_float<T>(0.f);
+}
+
+// A float of another block's shared memory (cluster address from mapa_shared).
+__device__ __forceinline__ float load_cluster_f32(uint32_t address) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+  return v;
+}
+
+}  // namespace sdc

@@ -1,0 +1,96 @@
+"""Low-rank adapters of many requests beside a shared projection."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from .. import ops
+
+_OP, _OP_IN_PLACE = ops.low_rank_adapters.default, ops.low_rank_adapters_.default
+
+# Rows of a tile. With at least this many tokens an adapter on average, tiles
+# of 64 rows share one read of the adapter's weights; below, most of their rows
+# would be empty and tiles of 16 do less for the same traffic.
+_WIDE_TILE, _NARROW_TILE, _WIDE_FROM = 64, 16, 32
+
+
+def _tiles(offsets, tokens, rows):
+    """``[n, 3]`` runs {first slot, slots, adapter} of at most ``rows`` slots, the adapters' first, then those of
+    the tokens without one (adapter -1), and how many have an adapter."""
+    starts = np.append(offsets[:-1], offsets[-1])
+    counts = np.append(np.diff(offsets), tokens - offsets[-1])
+    per = -(-counts // rows)
+    group = np.repeat(np.arange(len(counts)), per)
+    within = np.arange(per.sum()) - np.repeat(np.cumsum(per) - per, per)
+    first = starts[group] + within * rows
+    slots = np.minimum(rows, starts[group] + counts[group] - first)
+    adapter = np.where(group == len(counts) - 1, -1, group)
+    return np.stack((first, slots, adapter), 1).astype(np.int32), int(per[:-1].sum())
+
+
+class AdapterBatch:
+    """Which adapter each token of a batch takes, laid out for the kernels.
+
+    ``lengths``: tokens of each request, in the order of the batch's rows;
+    ``adapters``: each request's adapter, or -1 for none (host sequences);
+    ``count``: number of adapters whose weights the calls will pass. Requests
+    that share an adapter share its tiles wherever they are in the batch.
+    Built once for a batch on the host (one copy to ``device``, which it waits
+    for) and used for every projection of every layer; it must stay alive
+    until the work that uses it is done."""
+
+    def __init__(self, lengths, adapters, count, device="cuda"):
+        lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+        adapters = np.asarray(adapters, dtype=np.int64).reshape(-1)
+        if lengths.shape != adapters.shape:
+            raise ValueError("AdapterBatch needs one adapter a request")
+        if count < 1 or count > 65535:
+            raise ValueError("AdapterBatch takes 1 to 65535 adapters")
+        if lengths.size and (lengths.min() < 0 or adapters.min() < -1 or adapters.max() >= count):
+            raise ValueError("AdapterBatch lengths must not be negative and adapters must be -1 or below count")
+        tokens = int(lengths.sum())
+        if tokens >= 2 ** 31 - 128:
+            raise ValueError("AdapterBatch takes fewer than 2^31 - 128 tokens")
+        of_token = np.repeat(np.where(adapters < 0, count, adapters), lengths)
+        offsets = np.concatenate(([0], np.cumsum(np.bincount(of_token, minlength=count + 1))))[:count + 1]
+        slots = int(offsets[-1])
+        used = int((np.diff(offsets) > 0).sum())
+        self.tokens, self.count, self.slots = tokens, int(count), slots
+        self.tile_rows = _WIDE_TILE if used and slots >= _WIDE_FROM * used else _NARROW_TILE
+        tiles, self.active = _tiles(offsets, tokens, self.tile_rows)
+        rows = np.argsort(of_token, kind="stable").astype(np.int32)
+        packed = torch.from_numpy(np.concatenate((rows, offsets.astype(np.int32), tiles.reshape(-1)))).to(device)
+        self.rows, self.groups, tiles = packed.split((tokens, count + 1, tiles.size))
+        self.tiles = tiles.view(-1, 3)
+        self.arguments = (self.rows, self.groups, self.tiles, self.slots, self.active, self.tile_rows)
+
+
+def _check(x, batch):
+    if not x.is_cuda:
+        raise ValueError("low_rank_adapters requires CUDA tensors")
+    if not isinstance(batch, AdapterBatch):
+        raise ValueError("low_rank_adapters needs an AdapterBatch")
+
+
+def low_rank_adapters(base, x, a, b, batch, scale=None):
+    """``base + scale[g] * (x a[g]^T) b[g]^T`` with each token's adapter ``g``.
+
+    ``base`` ``[tokens, out]``: the shared projection's output; ``x``
+    ``[tokens, in]``: its input (bf16 or fp16, contiguous rows); ``a``
+    ``[count, rank, in]`` and ``b`` ``[count, out, rank]``: contiguous weights
+    of the same dtype, rank up to 256 (adapters of lower rank are padded with
+    zeros); ``scale`` fp32 ``[count]``, 1 when None; ``batch``: an
+    ``AdapterBatch`` of the same tokens and count. Tokens without an adapter
+    keep ``base``. Returns a new tensor; differentiable in ``base``, ``x``,
+    ``a`` and ``b``. Adapters without tokens get zero gradients. The low-rank
+    rows are kept in 32 bits up to the second product, which takes them as two
+    16-bit terms; in fp16 they overflow beyond 65504 like the type does."""
+    _check(x, batch)
+    return _OP(base, x, a, b, scale, *batch.arguments)[0]
+
+
+def low_rank_adapters_(base, x, a, b, batch, scale=None):
+    """``low_rank_adapters`` into ``base``: rows without an adapter are not touched."""
+    _check(x, batch)
+    _OP_IN_PLACE(base, x, a, b, scale, *batch.arguments)
+    return base
