@@ -33,14 +33,15 @@
 namespace sdc {
 namespace {
 
-constexpr int kRowThreads = 512;               // threads that stream the slice
+constexpr int kRowThreads = 256;               // threads that stream the slice
 constexpr int kRowBlock = kRowThreads + 32;    // and one warp for the teacher's list
 constexpr int kUnroll = 4;
+constexpr int kChunks = 4;                     // pieces of a slice copied under one barrier each
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
 constexpr size_t kSharedLimit = 227 * 1024;
-// Two blocks per SM: one loads while the other computes or writes.
-constexpr size_t kSliceTarget = 100 * 1024;
+// Four blocks per SM: some load while others compute, exchange or write.
+constexpr size_t kSliceTarget = 50 * 1024;
 constexpr int kBackThreads = 256;
 constexpr int kBackGranules = 8;               // 16-byte words per thread
 
@@ -66,6 +67,7 @@ struct DistillParams {
   const float* upstream_scale;  // nullable: 1
   int slice;                // 16-byte words of a row per block
   int chunks;               // backward: blocks per row
+  int32_t* watchdog;
 };
 
 // 1 / sum of a row without teacher entries.
@@ -91,47 +93,46 @@ __device__ __forceinline__ float teacher_at(const DistillParams& p, int64_t row,
 
 __device__ __forceinline__ bool is_entry(int64_t index, float t) { return index >= 0 && t != -INFINITY; }
 
-// A row as 16-byte words: the row starts `phase` elements into word 0.
+// A row as 16-byte words: the row starts `phase` elements into word 0. Words
+// of a block are counted from `first`; those of [lo, hi) lie in the row.
 template <typename T>
 struct RowWords {
   static constexpr int kPer = 16 / sizeof(T);
-  T* row;
-  int phase;
-  int64_t vocab;
-  __device__ __forceinline__ RowWords(T* r, int64_t v)
-      : row(r), phase(static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))), vocab(v) {}
-  __device__ __forceinline__ int64_t words() const { return (phase + vocab + kPer - 1) / kPer; }
-  __device__ __forceinline__ bool whole(int64_t word) const {
-    const int64_t e = word * kPer - phase;
-    return e >= 0 && e + kPer <= vocab;
+  const T* row;
+  const uint4* words;  // word `first`, if it were whole
+  int phase, vocab, first, count, lo, hi;
+
+  __device__ __forceinline__ RowWords(const T* r, int v, int first_word, int at_most)
+      : row(r), phase(static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))), vocab(v), first(first_word) {
+    words = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r) & ~uintptr_t{15}) + first;
+    const int all = (phase + vocab + kPer - 1) / kPer;
+    count = max(0, min(at_most, all - first));
+    lo = first == 0 && phase > 0;
+    hi = max(lo, count - (first + count == all && (phase + vocab) % kPer != 0));
   }
-  __device__ __forceinline__ T* at(int64_t word) const { return row + (word * kPer - phase); }
-  // Elements outside the row read as -inf.
-  __device__ __forceinline__ uint4 load(int64_t word) const {
-    if (whole(word)) return *reinterpret_cast<const uint4*>(at(word));
-    using Value = std::remove_const_t<T>;
+  __device__ __forceinline__ int element(int word) const { return (first + word) * kPer - phase; }
+  // Word with elements outside the row; they read as -inf.
+  __device__ __forceinline__ uint4 load_partial(int word) const {
     uint4 r;
-    Value* v = reinterpret_cast<Value*>(&r);
+    T* v = reinterpret_cast<T*>(&r);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t e = word * kPer - phase + i;
-      v[i] = e >= 0 && e < vocab ? row[e] : from_float<Value>(-INFINITY);
+      const int e = element(word) + i;
+      v[i] = e >= 0 && e < vocab ? row[e] : from_float<T>(-INFINITY);
     }
     return r;
   }
-  __device__ __forceinline__ void store(int64_t word, const uint4& r) const {
-    if (whole(word)) {
-      *reinterpret_cast<uint4*>(at(word)) = r;
+  // The same word of another row (a gradient's), which may start elsewhere in its words.
+  __device__ __forceinline__ void store(T* to, bool same_phase, int word, const uint4& r) const {
+    if (same_phase && word >= lo && word < hi) {
+      *reinterpret_cast<uint4*>(to + element(word)) = r;
       return;
     }
-    store_elements(word, r);
-  }
-  __device__ __forceinline__ void store_elements(int64_t word, const uint4& r) const {
     const T* v = reinterpret_cast<const T*>(&r);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t e = word * kPer - phase + i;
-      if (e >= 0 && e < vocab) row[e] = v[i];
+      const int e = element(word) + i;
+      if (e >= 0 && e < vocab) to[e] = v[i];
     }
   }
 };
@@ -161,28 +162,80 @@ __device__ __forceinline__ uint4 pack_word(const float* v) {
   }
 }
 
-// Whether (s - m) c cannot be formed as s c - m c: a finite m with m c near
-// the end of fp32's range.
-__device__ __forceinline__ bool is_wild(float m, float c) { return fabsf(m) * c > 1e38f && fabsf(m) < INFINITY; }
+// Two fp32 lanes in one register pair.
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ explicit Pair(float x) : Pair(x, x) {}
+  __device__ __forceinline__ Pair(float lo, float hi) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  }
+  __device__ __forceinline__ void split(float& lo, float& hi) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+  }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair exp2_fast(Pair a) {
+  float lo, hi;
+  a.split(lo, hi);
+  return Pair(exp2_fast(lo), exp2_fast(hi));
+}
 
-// 2^((s - m) c) for a row or thread maximum m.
+// Largest element of a word (NaN only if all are).
+template <typename T>
+__device__ __forceinline__ float word_max(const uint4& r) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(&r);
+    const T2 top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&top));
+    return fmaxf(f.x, f.y);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& r, Pair* v) {
+  float f[16 / sizeof(T)];
+  unpack_word<T>(r, f);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(8 / sizeof(T)); ++i) v[i] = Pair(f[2 * i], f[2 * i + 1]);
+}
+
+// 2^((s - m) c) for a maximum m. It is formed as 2^(s c - m c), one fma a
+// value, unless m is finite with m c near the end of fp32's range.
 struct Exponent {
   float m, mc;
   bool wild;
   __device__ __forceinline__ Exponent(float top, float c)
-      : m(top), mc(top == -INFINITY ? 0.f : top * c), wild(is_wild(top, c)) {}
+      : m(top), mc(top == -INFINITY ? 0.f : top * c), wild(fabsf(top) * c > 1e38f && fabsf(top) < INFINITY) {}
   __device__ __forceinline__ float operator()(float s, float c) const {
     return exp2_fast(wild ? (s - m) * c : fmaf(s, c, -mc));
   }
-  // v[i] = 2^((v[i] - m) c) * scale, the choice made once.
   template <int N>
-  __device__ __forceinline__ void apply(float* v, float c, float scale) const {
+  __device__ __forceinline__ void apply(Pair* v, float c) const {
     if (!wild) {
+      const Pair c2(c), shift(-mc);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = exp2_fast(fmaf(v[i], c, -mc)) * scale;
+      for (int i = 0; i < N; ++i) v[i] = exp2_fast(fma2(v[i], c2, shift));
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = exp2_fast((v[i] - m) * c) * scale;
+      for (int i = 0; i < N; ++i) v[i] = exp2_fast(mul2(add2(v[i], Pair(-m)), Pair(c)));
     }
   }
 };
@@ -190,35 +243,36 @@ struct Exponent {
 // Running maximum m and sum of 2^((s - m) c). While nothing above -inf was
 // seen m c counts as 0, so that -inf terms add 0.
 struct Softmax {
-  float m = -INFINITY, mc = 0.f, sum = 0.f;
-  bool wild = false;
+  Exponent power{-INFINITY, 1.f};
+  Pair sums{0.f};
 
   __device__ __forceinline__ void raise(float to, float c) {
     const Exponent next(to, c);
-    sum = m == -INFINITY ? sum : sum * next(m, c);
-    m = to;
-    mc = next.mc;
-    wild = next.wild;
+    if (power.m != -INFINITY) sums = mul2(sums, Pair(next(power.m, c)));
+    power = next;
   }
-  template <int N>
-  __device__ __forceinline__ void add(const float* v, float c) {
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    if (top > m) raise(top, c);
-    float part = 0.f;
-    if (!wild) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) part += exp2_fast(fmaf(v[i], c, -mc));
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& word, float c) {
+    constexpr int kPairs = 8 / sizeof(T);
+    const float top = word_max<T>(word);
+    if (top > power.m) raise(top, c);
+    Pair v[kPairs];
+    unpack_pairs<T>(word, v);
+    power.apply<kPairs>(v, c);
+    if constexpr (kPairs == 4) {
+      sums = add2(sums, add2(add2(v[0], v[1]), add2(v[2], v[3])));
     } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) part += exp2_fast((v[i] - m) * c);
+      sums = add2(sums, add2(v[0], v[1]));
     }
-    sum += part;
   }
-  __device__ __forceinline__ void join(float m2, float sum2, float c) {
-    if (m2 > m) raise(m2, c);
-    sum += m2 == -INFINITY ? sum2 : sum2 * Exponent(m, c)(m2, c);
+  __device__ __forceinline__ float total() const {
+    float lo, hi;
+    sums.split(lo, hi);
+    return lo + hi;
+  }
+  __device__ __forceinline__ void join(float m, float sum, float c) {
+    if (m > power.m) raise(m, c);
+    sums = add2(sums, Pair(m == -INFINITY ? sum : sum * power(m, c), 0.f));
   }
 };
 
@@ -241,216 +295,307 @@ struct Entry {
   int at;      // index, -1: no entry
 };
 
-// A cluster of blocks per row; GRAD stages the slice and writes the gradient.
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kRowBlock) distill_rows(DistillParams p) {
-  extern __shared__ uint4 shared[];
-  __shared__ float warp_m[kRowThreads / 32], warp_s[kRowThreads / 32];
-  __shared__ float2 parts[kMaxCluster];
-  constexpr int kPer = 16 / sizeof(T);
-  Entry* list = reinterpret_cast<Entry*>(shared);
-  uint4* stage = shared + p.top;  // an Entry is 16 bytes
-
-  const uint32_t rank = cluster_ctarank();
-  uint32_t ranks;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  // The other blocks' shared memory may be written once they have started;
-  // the wait comes just before.
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const int64_t row = blockIdx.x / ranks;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool lists = threadIdx.x >= kRowThreads;
-
-  const RowWords<const T> in(static_cast<const T*>(p.logits) + row * p.row_stride, p.vocab);
-  const int64_t first = static_cast<int64_t>(rank) * p.slice;
-  const int count = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.slice), in.words() - first)));
-
-  // The first words are on their way while the list is looked at.
-  uint4 ahead[kUnroll];
-  if (!lists) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int w = threadIdx.x + u * kRowThreads;
-      if (w < count) ahead[u] = in.load(first + w);
-    }
-  }
+// Whether the row's list has an entry (one warp).
+__device__ __forceinline__ bool any_entry(const DistillParams& p, int64_t row, int lane) {
   bool some = false;
   for (int k = 0; k < p.top && !some; k += 32) {
     bool entry = false;
     if (k + lane < p.top) entry = is_entry(index_at(p, row, k + lane), teacher_at(p, row, k + lane));
     some = __any_sync(0xffffffffu, entry);
   }
-  if (!some) {  // the same for every thread of the cluster
-    if (GRAD && !lists) {
-      const RowWords<T> out(static_cast<T*>(p.grad) + row * p.grad_stride, p.vocab);
-      const int64_t words = out.words();
-      for (int64_t w = static_cast<int64_t>(rank) * kRowThreads + threadIdx.x; w < words;
-           w += static_cast<int64_t>(ranks) * kRowThreads) {
-        out.store(w, make_uint4(0, 0, 0, 0));
-      }
-    }
-    if (rank == 0 && threadIdx.x == 0) {
-      if (p.loss != nullptr) p.loss[row] = 0.f;
-      if (p.stats != nullptr) p.stats[row] = make_float4(0.f, kEmptyRow, 0.f, 0.f);
-    }
-    __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    return;
-  }
+  return some;
+}
 
-  Softmax mine;
-  float teacher_max = 0.f, teacher_inv = 0.f;
-  bool stray = false;
-  if (lists) {
-    float m = -INFINITY;
-    for (int k = lane; k < p.top; k += 32) {
-      const int64_t index = index_at(p, row, k);
-      const float t = teacher_at(p, row, k);
-      Entry e{t, 0.f, 0.f, -1};
-      if (index >= p.vocab) stray = true;
-      else if (is_entry(index, t)) {
-        e.at = static_cast<int>(index);
-        e.s = to_float(in.row[index]);
-        m = fmaxf(m, t);
-      }
-      list[k] = e;
+struct TeacherSoftmax {
+  float max, inv;
+  bool stray;  // an index beyond the vocabulary
+};
+
+// Fills `list` (one warp): the teacher's softmax and the student's logits at its indices.
+template <typename T>
+__device__ __forceinline__ TeacherSoftmax read_list(const DistillParams& p, int64_t row, const T* logits, int lane,
+                                                    Entry* list) {
+  TeacherSoftmax t{-INFINITY, 0.f, false};
+  for (int k = lane; k < p.top; k += 32) {
+    const int64_t index = index_at(p, row, k);
+    Entry e{teacher_at(p, row, k), 0.f, 0.f, -1};
+    if (index >= p.vocab) {
+      t.stray = true;
+    } else if (is_entry(index, e.p)) {
+      e.at = static_cast<int>(index);
+      e.s = to_float(logits[index]);
+      t.max = fmaxf(t.max, e.p);
     }
-    m = warp_max(m);
-    stray = __any_sync(0xffffffffu, stray);
-    teacher_max = m;
-    float sum = 0.f;
-    for (int k = lane; k < p.top; k += 32) {
-      if (list[k].at >= 0) sum += exp2_fast((list[k].p - m) * p.c);
-    }
-    sum = warp_sum(sum);
-    teacher_inv = 1.f / sum;
-    const float log_sum = logf(sum);
-    for (int k = lane; k < p.top; k += 32) {
-      const float x = list[k].p - m;
-      list[k].log_p = x * p.inv_tau - log_sum;
-      list[k].p = exp2_fast(x * p.c) * teacher_inv;
-    }
-    __syncwarp();
-  } else {
-    for (int base = 0; base < count; base += kUnroll * kRowThreads) {
-      uint4 next[kUnroll];
-      const int after = base + kUnroll * kRowThreads + threadIdx.x;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (after + u * kRowThreads < count) next[u] = in.load(first + after + u * kRowThreads);
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int w = base + threadIdx.x + u * kRowThreads;
-        if (w < count) {
-          if constexpr (GRAD) stage[w] = ahead[u];
-          float v[kPer];
-          unpack_word<T>(ahead[u], v);
-          mine.add<kPer>(v, p.c);
-        }
-        ahead[u] = next[u];
-      }
-    }
+    list[k] = e;
+  }
+  t.max = warp_max(t.max);
+  t.stray = __any_sync(0xffffffffu, t.stray);
+  float sum = 0.f;
+  for (int k = lane; k < p.top; k += 32) {
+    if (list[k].at >= 0) sum += exp2_fast((list[k].p - t.max) * p.c);
+  }
+  sum = warp_sum(sum);
+  t.inv = 1.f / sum;
+  const float log_sum = logf(sum);
+  for (int k = lane; k < p.top; k += 32) {
+    const float x = list[k].p - t.max;
+    list[k].log_p = x * p.inv_tau - log_sum;
+    list[k].p = exp2_fast(x * p.c) * t.inv;
+  }
+  __syncwarp();
+  return t;
+}
+
+// Row maximum and sum over the threads of a cluster's blocks: every thread of
+// every block calls it, `mine` counts for the streaming ones. The cluster
+// barrier's first phase was arrived at when the kernel started: the other
+// blocks' shared memory may be written once they have started as well.
+__device__ __forceinline__ Softmax join_row(Softmax mine, float c, uint32_t rank, uint32_t ranks) {
+  __shared__ float2 warps[kRowThreads / 32];
+  __shared__ float2 blocks[kMaxCluster];
+  if (threadIdx.x < kRowThreads) {
+    float m = mine.power.m, sum = mine.total();
 #pragma unroll
     for (int step = 16; step > 0; step /= 2) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, mine.m, step);
-      const float s2 = __shfl_xor_sync(0xffffffffu, mine.sum, step);
-      mine.join(m2, s2, p.c);
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, step);
+      const float s2 = __shfl_xor_sync(0xffffffffu, sum, step);
+      const float top = fmaxf(m, m2);
+      const Exponent power(top, c);
+      sum = (m == -INFINITY ? sum : sum * power(m, c)) + (m2 == -INFINITY ? s2 : s2 * power(m2, c));
+      m = top;
     }
-    if (lane == 0) warp_m[warp] = mine.m, warp_s[warp] = mine.sum;
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x / 32] = make_float2(m, sum);
   }
   __syncthreads();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (threadIdx.x < ranks) {  // one thread per block of the cluster
     Softmax block;
-    for (int i = 0; i < kRowThreads / 32; ++i) block.join(warp_m[i], warp_s[i], p.c);
-    const uint32_t to = mapa_shared(&parts[rank], threadIdx.x);
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(block.m), "f"(block.sum) : "memory");
+    for (int i = 0; i < kRowThreads / 32; ++i) block.join(warps[i].x, warps[i].y, c);
+    const uint32_t to = mapa_shared(&blocks[rank], threadIdx.x);
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(block.power.m), "f"(block.total())
+                 : "memory");
   }
   cluster_sync();
   Softmax all;
-  for (uint32_t i = 0; i < ranks; ++i) all.join(parts[i].x, parts[i].y, p.c);
-  float inv = 1.f / all.sum;
+  for (uint32_t i = 0; i < ranks; ++i) all.join(blocks[i].x, blocks[i].y, c);
+  return all;
+}
 
+// The row's loss and statistics (the list warp of block 0).
+__device__ __forceinline__ void write_loss(const DistillParams& p, int64_t row, const Entry* list, int lane,
+                                           const Softmax& all, float inv, const TeacherSoftmax& teacher) {
+  const float log_sum = logf(all.total());
+  float total = 0.f;
+  for (int k = lane; k < p.top; k += 32) {
+    const Entry e = list[k];
+    if (e.at >= 0 && e.p != 0.f) total += e.p * (e.log_p - ((e.s - all.power.m) * p.inv_tau - log_sum));
+  }
+  total = warp_sum(total);
+  if (lane == 0) {
+    p.loss[row] = teacher.stray ? __int_as_float(0x7fffffff) : total * p.tau * p.tau;
+    p.stats[row] = make_float4(all.power.m, inv, teacher.max, teacher.inv);
+  }
+}
+
+__device__ __forceinline__ void write_empty(const DistillParams& p, int64_t row) {
+  p.loss[row] = 0.f;
+  p.stats[row] = make_float4(0.f, kEmptyRow, 0.f, 0.f);
+}
+
+// The losses alone: a cluster of blocks per row streams it through registers.
+template <typename T>
+__global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams p) {
+  extern __shared__ uint4 shared[];
+  __shared__ volatile int empty_row;
+  Entry* list = reinterpret_cast<Entry*>(shared);
+  const uint32_t rank = cluster_ctarank();
+  uint32_t ranks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int64_t row = blockIdx.x / ranks;
+  const int lane = threadIdx.x & 31;
+  const bool lists = threadIdx.x >= kRowThreads;
+  if (threadIdx.x == 0) empty_row = 0;
+  __syncthreads();
+
+  const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
+  const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(rank) * p.slice, p.slice);
+  Softmax mine;
+  TeacherSoftmax teacher{0.f, 0.f, false};
   if (lists) {
-    if (stray) inv = __int_as_float(0x7fffffff);
-    if (rank == 0) {
-      const float log_sum = logf(all.sum);
-      float total = 0.f;
-      for (int k = lane; k < p.top; k += 32) {
-        const Entry e = list[k];
-        if (e.at >= 0 && e.p != 0.f) total += e.p * (e.log_p - ((e.s - all.m) * p.inv_tau - log_sum));
-      }
-      total = warp_sum(total);
-      if (lane == 0) {
-        const float nan = __int_as_float(0x7fffffff);
-        if (p.loss != nullptr) p.loss[row] = stray ? nan : total * p.tau * p.tau;
-        if (p.stats != nullptr) p.stats[row] = make_float4(all.m, inv, teacher_max, teacher_inv);
+    if (any_entry(p, row, lane)) teacher = read_list(p, row, logits, lane, list);
+    else empty_row = 1;
+  } else {
+    // Whole words, the next ones on their way while these are added.
+    uint4 ahead[kUnroll];
+    const int start = in.lo + static_cast<int>(threadIdx.x);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (start + u * kRowThreads < in.hi) ahead[u] = in.words[start + u * kRowThreads];
+    }
+    for (int w = start; w < in.hi; w += kUnroll * kRowThreads) {
+      if (empty_row) break;  // nothing of the row counts
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint4 word = ahead[u];
+        const int next = w + (kUnroll + u) * kRowThreads;
+        if (next < in.hi) ahead[u] = in.words[next];
+        if (w + u * kRowThreads < in.hi) mine.add<T>(word, p.c);
       }
     }
+    if (threadIdx.x == 0 && in.lo > 0 && in.count > 0) mine.add<T>(in.load_partial(0), p.c);
+    if (threadIdx.x == 1 && in.hi < in.count) mine.add<T>(in.load_partial(in.count - 1), p.c);
+    __syncwarp();
   }
-  if constexpr (GRAD) {
-    __shared__ float row_inv;
-    if (threadIdx.x == kRowThreads) row_inv = inv;
-    __syncthreads();
-    inv = row_inv;
-    float a = p.tau;
-    if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
-    const float scaled = a * inv;
-    const RowWords<T> out(static_cast<T*>(p.grad) + row * p.grad_stride, p.vocab);
-    const bool same_phase = out.phase == in.phase;
-    const Exponent power(all.m, p.c);
-    if (!lists) {
-      for (int w = threadIdx.x; w < count; w += kRowThreads) {
-        float v[kPer];
-        unpack_word<T>(stage[w], v);
-        power.template apply<kPer>(v, p.c, scaled);
-        const uint4 r = pack_word<T>(v);
-        if (same_phase) {
-          out.store(first + w, r);
+  const Softmax all = join_row(mine, p.c, rank, ranks);
+  if (!lists || rank != 0) return;
+  if (empty_row) {
+    if (lane == 0) write_empty(p, row);
+    return;
+  }
+  const float inv = teacher.stray ? __int_as_float(0x7fffffff) : 1.f / all.total();
+  write_loss(p, row, list, lane, all, inv, teacher);
+}
+
+// Loss and gradient in one pass: each block of the row's cluster copies its
+// slice to shared memory (bulk copies, the first chunk added while the last
+// is on its way), and after the exchange turns it into the gradient.
+template <typename T>
+__global__ void __launch_bounds__(kRowBlock, 4) distill_grad_rows(DistillParams p) {
+  extern __shared__ uint4 shared[];
+  __shared__ __align__(8) uint64_t arrived[kChunks];
+  __shared__ int state;  // 1: the row has no entries; 2: a copy did not arrive
+  __shared__ int32_t abort;
+  __shared__ float row_inv;
+  constexpr int kPer = 16 / sizeof(T);
+  Entry* list = reinterpret_cast<Entry*>(shared);
+  uint4* stage = shared + p.top;  // an Entry is 16 bytes
+  const uint32_t rank = cluster_ctarank();
+  uint32_t ranks;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int64_t row = blockIdx.x / ranks;
+  const int lane = threadIdx.x & 31;
+  const bool lists = threadIdx.x >= kRowThreads;
+  if (threadIdx.x == kRowThreads) {
+    for (int i = 0; i < kChunks; ++i) mbar_init(&arrived[i], 1);
+    fence_barrier_init();
+    state = 0;
+    abort = 0;
+  }
+  __syncthreads();
+
+  const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
+  T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
+  const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(rank) * p.slice, p.slice);
+  const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
+  const int chunk = (in.count + kChunks * kRowThreads - 1) / (kChunks * kRowThreads) * kRowThreads;
+  Softmax mine;
+  TeacherSoftmax teacher{0.f, 0.f, false};
+  if (lists) {
+    const bool some = any_entry(p, row, lane);
+    if (some) {
+      if (lane == 0 && in.lo > 0 && in.count > 0) stage[0] = in.load_partial(0);
+      if (lane == 0 && in.hi < in.count) stage[in.count - 1] = in.load_partial(in.count - 1);
+    } else if (lane == 0) {
+      state = 1;
+    }
+    if (lane == 0) {
+      for (int i = 0; i < kChunks; ++i) {
+        const int from = max(in.lo, i * chunk), to = min(in.hi, (i + 1) * chunk);
+        if (some && from < to) {
+          const uint32_t bytes = static_cast<uint32_t>(to - from) * 16;
+          mbar_arrive_expect_tx(&arrived[i], bytes);
+          asm volatile(
+              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                  smem_u32(stage + from)),
+              "l"(in.words + from), "r"(bytes), "r"(smem_u32(&arrived[i]))
+              : "memory");
         } else {
-          const RowWords<T> shifted = [&] { RowWords<T> s = out; s.phase = in.phase; return s; }();
-          shifted.store_elements(first + w, r);
+          mbar_arrive(&arrived[i]);
         }
       }
-    }
-    __syncthreads();
-    if (!lists) return;
-    // The list's columns again, with the teacher's part. Each entry leaves
-    // its number in its (no longer needed) staged logit: one that finds
-    // another number there shares its column.
-    T* slot = reinterpret_cast<T*>(stage);
-    auto local = [&](int k) -> int64_t {
-      if (list[k].at < 0) return -1;
-      const int64_t e = list[k].at + in.phase - first * kPer;
-      return e >= 0 && e < static_cast<int64_t>(count) * kPer ? e : -1;
-    };
-    using Mark = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
-    Mark* mark = reinterpret_cast<Mark*>(slot);
-    for (int k = lane; k < p.top; k += 32) {
-      const int64_t e = local(k);
-      if (e >= 0) mark[e] = static_cast<Mark>(k);
     }
     __syncwarp();
-    bool shared_column = false;
-    for (int k = lane; k < p.top; k += 32) {
-      const int64_t e = local(k);
-      if (e >= 0 && mark[e] != static_cast<Mark>(k)) shared_column = true;
+    if (some) teacher = read_list(p, row, logits, lane, list);
+  } else {
+    for (int i = 0; i < kChunks; ++i) {
+      mbar_wait(&arrived[i], 0, kWaitOther, &abort, p.watchdog);
+      if (state == 1) break;
+      const int to = min(in.count, (i + 1) * chunk);
+#pragma unroll 2
+      for (int w = i * chunk + static_cast<int>(threadIdx.x); w < to; w += kRowThreads) mine.add<T>(stage[w], p.c);
     }
-    shared_column = __any_sync(0xffffffffu, shared_column);
-    for (int k = lane; k < p.top; k += 32) {
-      if (local(k) < 0) continue;
-      const Entry e = list[k];
-      float prob = e.p;
-      if (shared_column) {  // every entry of the column writes the same sum
-        prob = 0.f;
-        for (int j = 0; j < p.top; ++j) {
-          if (list[j].at == e.at) prob += list[j].p;
-        }
+    __syncwarp();
+  }
+  const Softmax all = join_row(mine, p.c, rank, ranks);
+  if (abort != 0 && threadIdx.x == 0) {  // never leave a copy behind in flight
+    for (int i = 0; i < kChunks; ++i) mbar_drain(&arrived[i], 0);
+  }
+  if (state == 1) {
+    if (!lists) {
+      for (int w = threadIdx.x; w < in.count; w += kRowThreads) in.store(grad, same_phase, w, make_uint4(0, 0, 0, 0));
+    } else if (rank == 0 && lane == 0) {
+      write_empty(p, row);
+    }
+    return;
+  }
+  const float nan = __int_as_float(0x7fffffff);
+  if (lists) {
+    const float inv = teacher.stray || abort != 0 ? nan : 1.f / all.total();
+    if (lane == 0) row_inv = inv;
+    if (rank == 0) write_loss(p, row, list, lane, all, inv, teacher);
+  }
+  __syncthreads();
+  const float inv = row_inv;
+  float a = p.tau;
+  if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
+  if (!lists) {
+    const Pair scaled(a * inv);
+#pragma unroll 2
+    for (int w = threadIdx.x; w < in.count; w += kRowThreads) {
+      Pair v[kPer / 2];
+      unpack_pairs<T>(stage[w], v);
+      all.power.apply<kPer / 2>(v, p.c);
+      float f[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i) mul2(v[i], scaled).split(f[2 * i], f[2 * i + 1]);
+      in.store(grad, same_phase, w, pack_word<T>(f));
+    }
+  }
+  __syncthreads();
+  if (!lists) return;
+  // The list's columns again, with the teacher's part. Each entry leaves its
+  // number in its (no longer needed) staged logit: one that finds another
+  // number there shares its column.
+  using Mark = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+  Mark* mark = reinterpret_cast<Mark*>(stage);
+  auto local = [&](int k) {
+    const int e = list[k].at + in.phase - in.first * kPer;
+    return list[k].at >= 0 && e >= 0 && e < in.count * kPer ? e : -1;
+  };
+  for (int k = lane; k < p.top; k += 32) {
+    const int e = local(k);
+    if (e >= 0) mark[e] = static_cast<Mark>(k);
+  }
+  __syncwarp();
+  bool shared_column = false;
+  for (int k = lane; k < p.top; k += 32) {
+    const int e = local(k);
+    if (e >= 0 && mark[e] != static_cast<Mark>(k)) shared_column = true;
+  }
+  shared_column = __any_sync(0xffffffffu, shared_column);
+  for (int k = lane; k < p.top; k += 32) {
+    if (local(k) < 0) continue;
+    const Entry e = list[k];
+    float prob = e.p;
+    if (shared_column) {  // every entry of the column writes the same sum
+      prob = 0.f;
+      for (int j = 0; j < p.top; ++j) {
+        if (list[j].at == e.at) prob += list[j].p;
       }
-      const float q = power(e.s, p.c) * inv;
-      out.row[e.at] = from_float<T>(a * (q - prob));
     }
+    grad[e.at] = from_float<T>(a * (all.power(e.s, p.c) * inv - prob));
   }
 }
 
@@ -464,28 +609,28 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
   __shared__ uint32_t seen[(kWords * kPer + 31) / 32];
   __shared__ int shared_column;
   const int64_t row = blockIdx.x / p.chunks;
-  const int64_t first = static_cast<int64_t>(blockIdx.x % p.chunks) * kWords;
-  const RowWords<const T> in(static_cast<const T*>(p.logits) + row * p.row_stride, p.vocab);
-  const RowWords<T> out(static_cast<T*>(p.grad) + row * p.grad_stride, p.vocab);
-  const int64_t words = in.words();
+  const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
+  T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
+  const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(blockIdx.x % p.chunks) * kWords, kWords);
+  const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
 
+  const float4 stats = p.stats[row];
+  const bool empty = stats.y == kEmptyRow;
   uint4 raw[kBackGranules];
 #pragma unroll
   for (int u = 0; u < kBackGranules; ++u) {
-    const int64_t w = first + threadIdx.x + u * kBackThreads;
-    if (w < words) raw[u] = in.load(w);
+    const int w = static_cast<int>(threadIdx.x) + u * kBackThreads;
+    if (w >= in.lo && w < in.hi) raw[u] = in.words[w];
+    else if (w < in.count) raw[u] = in.load_partial(w);
   }
-  const float4 stats = p.stats[row];
   float a = p.tau;
   if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
   if (p.upstream_scale != nullptr) a *= *p.upstream_scale;
-  const bool empty = stats.y == kEmptyRow;
-  const float scaled = a * stats.y;
   const Exponent power(stats.x, p.c);
 
   // This block's entries of the list; their logits before they are
   // overwritten (the gradient may replace the logits).
-  int64_t at[kEntries];
+  int at[kEntries];
   float s[kEntries];
 #pragma unroll
   for (int i = 0; i < kEntries; ++i) {
@@ -493,11 +638,11 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
     const int k = threadIdx.x + i * kBackThreads;
     if (empty || k >= p.top) continue;
     const int64_t index = index_at(p, row, k);
-    const int64_t word = (index + in.phase) / kPer;
-    if (index < 0 || index >= p.vocab || word < first || word >= first + kWords) continue;
-    if (!is_entry(index, teacher_at(p, row, k))) continue;
-    at[i] = index;
-    s[i] = to_float(in.row[index]);
+    if (index < 0 || index >= p.vocab) continue;
+    const int e = static_cast<int>(index) + in.phase - in.first * kPer;
+    if (e < 0 || e >= in.count * kPer || !is_entry(index, teacher_at(p, row, k))) continue;
+    at[i] = static_cast<int>(index);
+    s[i] = to_float(logits[index]);
   }
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(seen) / 4); i += kBackThreads) seen[i] = 0;
   if (threadIdx.x == 0) shared_column = 0;
@@ -505,23 +650,21 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
 #pragma unroll
   for (int i = 0; i < kEntries; ++i) {
     if (at[i] < 0) continue;
-    const uint32_t e = static_cast<uint32_t>(at[i] + in.phase - first * kPer);
+    const uint32_t e = static_cast<uint32_t>(at[i] + in.phase - in.first * kPer);
     if (atomicOr(&seen[e / 32], 1u << (e % 32)) >> (e % 32) & 1u) shared_column = 1;
   }
+  const Pair scaled(a * stats.y);
 #pragma unroll
   for (int u = 0; u < kBackGranules; ++u) {
-    const int64_t w = first + threadIdx.x + u * kBackThreads;
-    if (w >= words) continue;
-    float v[kPer];
-    unpack_word<T>(raw[u], v);
-    power.apply<kPer>(v, p.c, scaled);
-    const uint4 r = empty ? make_uint4(0, 0, 0, 0) : pack_word<T>(v);
-    if (out.phase == in.phase) {
-      out.store(w, r);
-    } else {
-      const RowWords<T> shifted = [&] { RowWords<T> o = out; o.phase = in.phase; return o; }();
-      shifted.store_elements(w, r);
-    }
+    const int w = static_cast<int>(threadIdx.x) + u * kBackThreads;
+    if (w >= in.count) continue;
+    Pair v[kPer / 2];
+    unpack_pairs<T>(raw[u], v);
+    power.apply<kPer / 2>(v, p.c);
+    float f[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) mul2(v[i], scaled).split(f[2 * i], f[2 * i + 1]);
+    in.store(grad, same_phase, w, empty ? make_uint4(0, 0, 0, 0) : pack_word<T>(f));
   }
   __syncthreads();
 #pragma unroll
@@ -537,8 +680,7 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
         if (t != -INFINITY) prob += exp2_fast((t - stats.z) * p.c) * stats.w;
       }
     }
-    const float q = power(s[i], p.c) * stats.y;
-    out.row[at[i]] = from_float<T>(a * (q - prob));
+    grad[at[i]] = from_float<T>(a * (power(s[i], p.c) * stats.y - prob));
   }
 }
 
@@ -613,14 +755,14 @@ size_t shared_bytes(int64_t vocab, int dtype, int top, int cluster, bool grad) {
          (grad ? static_cast<size_t>(ceil_div(max_words(vocab, dtype), cluster)) * 16 : 0);
 }
 
-// Blocks per row: the gradient's slice should let two blocks share an SM
+// Blocks per row: the gradient's slice should let four blocks share an SM
 // (and must fit one); beyond that, few rows are split until the blocks fill
 // the SMs. 0: a row does not fit a cluster.
 int cluster_size(int64_t rows, int64_t vocab, int dtype, int top, bool grad) {
   int cluster = 1;
-  while (cluster < kMaxCluster && shared_bytes(vocab, dtype, top, cluster, grad) > kSliceTarget) cluster *= 2;
+  while (cluster < kMaxCluster && grad && shared_bytes(vocab, dtype, top, cluster, grad) > kSliceTarget) cluster *= 2;
   if (shared_bytes(vocab, dtype, top, cluster, grad) > kSharedLimit - 2048) return 0;
-  while (cluster < kMaxCluster && rows * cluster < 2 * sm_count() && max_words(vocab, dtype) / cluster > 2 * kRowThreads) {
+  while (cluster < kMaxCluster && rows * cluster < 4 * sm_count() && max_words(vocab, dtype) / cluster > 2 * kRowThreads) {
     cluster *= 2;
   }
   return cluster;
@@ -628,14 +770,17 @@ int cluster_size(int64_t rows, int64_t vocab, int dtype, int top, bool grad) {
 
 template <typename T, bool GRAD>
 int launch_rows(DistillParams p, int64_t rows, int cluster, size_t shared, cudaStream_t stream) {
-  static std::atomic<uint64_t> prepared{0};
-  int device = 0;
-  SDC_CUDA_CHECK(cudaGetDevice(&device));
-  const uint64_t bit = 1ull << (device & 63);
-  if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
-    SDC_CUDA_CHECK(cudaFuncSetAttribute(distill_rows<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(kSharedLimit - 2048)));
-    prepared.fetch_or(bit, std::memory_order_relaxed);
+  void (*kernel)(DistillParams) = GRAD ? distill_grad_rows<T> : distill_loss_rows<T>;
+  if (GRAD) {
+    static std::atomic<uint64_t> prepared{0};
+    int device = 0;
+    SDC_CUDA_CHECK(cudaGetDevice(&device));
+    const uint64_t bit = 1ull << (device & 63);
+    if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
+      SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          static_cast<int>(kSharedLimit - 2048)));
+      prepared.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(rows * cluster));
@@ -649,7 +794,7 @@ int launch_rows(DistillParams p, int64_t rows, int cluster, size_t shared, cudaS
   attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  SDC_CUDA_CHECK(cudaLaunchKernelEx(&config, distill_rows<T, GRAD>, p));
+  SDC_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, p));
   return SDC_OK;
 }
 
@@ -657,6 +802,8 @@ template <bool GRAD>
 int run_rows(DistillParams p, int dtype, int64_t rows, int cluster, cudaStream_t stream) {
   SDC_REQUIRE(rows <= INT_MAX / cluster, "distillation has too many rows for one launch");
   p.slice = static_cast<int>(ceil_div(max_words(p.vocab, dtype), cluster));
+  p.watchdog = watchdog_ptr();
+  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "distillation has no watchdog word on this device");
   const size_t shared = shared_bytes(p.vocab, dtype, p.top, cluster, GRAD);
   if (dtype == kF32) return launch_rows<float, GRAD>(p, rows, cluster, shared, stream);
   if (dtype == kBF16) return launch_rows<__nv_bfloat16, GRAD>(p, rows, cluster, shared, stream);
