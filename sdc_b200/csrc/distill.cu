@@ -18,10 +18,7 @@
 // also one read and one write: a cluster of blocks shares a row, each block
 // keeps its slice in shared memory, the (max, sum) pairs cross the cluster
 // through distributed shared memory, and the second pass over the slice
-// writes the gradient. Softmax statistics are fp32; the exponents are formed
-// as fma(s, c, -max c) with the same rounded max c in the sum and in the
-// gradient, so its rounding cancels; where max c could overflow (rows masked
-// with the type's lowest value throughout) as (s - max) c instead.
+// writes the gradient. Softmax statistics are fp32.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -35,10 +32,12 @@ namespace {
 
 constexpr int kRowThreads = 256;               // threads that stream the slice
 constexpr int kRowBlock = kRowThreads + 32;    // and one warp for the teacher's list
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;                      // words at once from global memory
+constexpr int kAtOnce = 4;                      // and from shared memory
 constexpr int kChunks = 4;                     // pieces of a slice copied under one barrier each
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kGradBlocks = 4;                 // of loss with gradient on an SM
 constexpr size_t kSharedLimit = 227 * 1024;
 // Four blocks per SM: some load while others compute, exchange or write.
 constexpr size_t kSliceTarget = 50 * 1024;
@@ -68,6 +67,8 @@ struct DistillParams {
   int slice;                // 16-byte words of a row per block
   int chunks;               // backward: blocks per row
   int32_t* watchdog;
+  int64_t rows;             // loss with gradient: rows and log2 of the hash table's size
+  int hash_bits;
 };
 
 // 1 / sum of a row without teacher entries.
@@ -217,64 +218,77 @@ __device__ __forceinline__ void unpack_pairs(const uint4& r, Pair* v) {
   for (int i = 0; i < static_cast<int>(8 / sizeof(T)); ++i) v[i] = Pair(f[2 * i], f[2 * i + 1]);
 }
 
-// 2^((s - m) c) for a maximum m. It is formed as 2^(s c - m c), one fma a
-// value, unless m is finite with m c near the end of fp32's range.
+// 2^((s - m) c) for a maximum m. The difference is formed first: s c - m c
+// would be one instruction less, but overflows where a row is masked with the
+// type's lowest value throughout. While nothing above -inf was seen m counts
+// as 0, so that -inf terms give 0.
 struct Exponent {
-  float m, mc;
-  bool wild;
-  __device__ __forceinline__ Exponent(float top, float c)
-      : m(top), mc(top == -INFINITY ? 0.f : top * c), wild(fabsf(top) * c > 1e38f && fabsf(top) < INFINITY) {}
-  __device__ __forceinline__ float operator()(float s, float c) const {
-    return exp2_fast(wild ? (s - m) * c : fmaf(s, c, -mc));
-  }
-  template <int N>
-  __device__ __forceinline__ void apply(Pair* v, float c) const {
-    if (!wild) {
-      const Pair c2(c), shift(-mc);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = exp2_fast(fma2(v[i], c2, shift));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = exp2_fast(mul2(add2(v[i], Pair(-m)), Pair(c)));
-    }
+  float shift;
+  __device__ __forceinline__ explicit Exponent(float m) : shift(m == -INFINITY ? 0.f : -m) {}
+  __device__ __forceinline__ float operator()(float s, float c) const { return exp2_fast((s + shift) * c); }
+  __device__ __forceinline__ Pair operator()(Pair s, float c) const {
+    return exp2_fast(mul2(add2(s, Pair(shift)), Pair(c)));
   }
 };
 
-// Running maximum m and sum of 2^((s - m) c). While nothing above -inf was
-// seen m c counts as 0, so that -inf terms add 0.
+// Running maximum m and sum of 2^((s - m) c) of one thread.
 struct Softmax {
-  Exponent power{-INFINITY, 1.f};
+  float m = -INFINITY;
+  Exponent power{-INFINITY};
   Pair sums{0.f};
 
-  __device__ __forceinline__ void raise(float to, float c) {
-    const Exponent next(to, c);
-    if (power.m != -INFINITY) sums = mul2(sums, Pair(next(power.m, c)));
-    power = next;
+  // N words at once: one look at the maximum, and their exponents do not wait for one another.
+  template <typename T, int N>
+  __device__ __forceinline__ void add(const uint4* words, float c) {
+    constexpr int kPairs = 8 / sizeof(T);
+    float top = word_max<T>(words[0]);
+#pragma unroll
+    for (int n = 1; n < N; ++n) top = fmaxf(top, word_max<T>(words[n]));
+    if (top > m) {
+      const Exponent next(top);
+      if (m != -INFINITY) sums = mul2(sums, Pair(next(m, c)));
+      m = top;
+      power = next;
+    }
+    Pair part[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      Pair v[kPairs];
+      unpack_pairs<T>(words[n], v);
+      part[n] = power(v[0], c);
+#pragma unroll
+      for (int i = 1; i < kPairs; ++i) part[n] = add2(part[n], power(v[i], c));
+    }
+#pragma unroll
+    for (int n = 1; n < N; ++n) part[0] = add2(part[0], part[n]);
+    sums = add2(sums, part[0]);
   }
   template <typename T>
   __device__ __forceinline__ void add(const uint4& word, float c) {
-    constexpr int kPairs = 8 / sizeof(T);
-    const float top = word_max<T>(word);
-    if (top > power.m) raise(top, c);
-    Pair v[kPairs];
-    unpack_pairs<T>(word, v);
-    power.apply<kPairs>(v, c);
-    if constexpr (kPairs == 4) {
-      sums = add2(sums, add2(add2(v[0], v[1]), add2(v[2], v[3])));
-    } else {
-      sums = add2(sums, add2(v[0], v[1]));
-    }
+    add<T, 1>(&word, c);
   }
-  __device__ __forceinline__ float total() const {
+  __device__ __forceinline__ float2 pair() const {
     float lo, hi;
     sums.split(lo, hi);
-    return lo + hi;
-  }
-  __device__ __forceinline__ void join(float m, float sum, float c) {
-    if (m > power.m) raise(m, c);
-    sums = add2(sums, Pair(m == -INFINITY ? sum : sum * power(m, c), 0.f));
+    return make_float2(m, lo + hi);
   }
 };
+
+// Joins the lanes' (max, sum) over groups of WIDTH lanes; every lane gets it.
+template <int WIDTH>
+__device__ __forceinline__ float2 join_lanes(float2 mine, float c) {
+  float m = mine.x;
+#pragma unroll
+  for (int step = WIDTH / 2; step > 0; step /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
+  float sum = mine.x == -INFINITY ? mine.y : mine.y * Exponent(m)(mine.x, c);
+#pragma unroll
+  for (int step = WIDTH / 2; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+  return make_float2(m, sum);
+}
+// Joins pairs[0 .. count), count <= 32, read one a lane.
+__device__ __forceinline__ float2 join_parts(const float2* pairs, int count, int lane, float c) {
+  return join_lanes<32>(lane < count ? pairs[lane] : make_float2(-INFINITY, 0.f), c);
+}
 
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
@@ -350,50 +364,41 @@ __device__ __forceinline__ TeacherSoftmax read_list(const DistillParams& p, int6
 // every block calls it, `mine` counts for the streaming ones. The cluster
 // barrier's first phase was arrived at when the kernel started: the other
 // blocks' shared memory may be written once they have started as well.
-__device__ __forceinline__ Softmax join_row(Softmax mine, float c, uint32_t rank, uint32_t ranks) {
+__device__ __forceinline__ float2 join_row(const Softmax& mine, float c, uint32_t rank, uint32_t ranks) {
   __shared__ float2 warps[kRowThreads / 32];
   __shared__ float2 blocks[kMaxCluster];
+  const int lane = threadIdx.x & 31;
   if (threadIdx.x < kRowThreads) {
-    float m = mine.power.m, sum = mine.total();
-#pragma unroll
-    for (int step = 16; step > 0; step /= 2) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, step);
-      const float s2 = __shfl_xor_sync(0xffffffffu, sum, step);
-      const float top = fmaxf(m, m2);
-      const Exponent power(top, c);
-      sum = (m == -INFINITY ? sum : sum * power(m, c)) + (m2 == -INFINITY ? s2 : s2 * power(m2, c));
-      m = top;
-    }
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x / 32] = make_float2(m, sum);
+    const float2 part = join_lanes<32>(mine.pair(), c);
+    if (lane == 0) warps[threadIdx.x / 32] = part;
   }
   __syncthreads();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (threadIdx.x < ranks) {  // one thread per block of the cluster
-    Softmax block;
-    for (int i = 0; i < kRowThreads / 32; ++i) block.join(warps[i].x, warps[i].y, c);
-    const uint32_t to = mapa_shared(&blocks[rank], threadIdx.x);
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(block.power.m), "f"(block.total())
-                 : "memory");
+  if (threadIdx.x < 32) {
+    const float2 block = join_parts(warps, kRowThreads / 32, lane, c);
+    if (lane < static_cast<int>(ranks)) {
+      const uint32_t to = mapa_shared(&blocks[rank], static_cast<uint32_t>(lane));
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(block.x), "f"(block.y) : "memory");
+    }
+    __syncwarp();
   }
   cluster_sync();
-  Softmax all;
-  for (uint32_t i = 0; i < ranks; ++i) all.join(blocks[i].x, blocks[i].y, c);
-  return all;
+  return join_parts(blocks, static_cast<int>(ranks), lane, c);
 }
 
 // The row's loss and statistics (the list warp of block 0).
 __device__ __forceinline__ void write_loss(const DistillParams& p, int64_t row, const Entry* list, int lane,
-                                           const Softmax& all, float inv, const TeacherSoftmax& teacher) {
-  const float log_sum = logf(all.total());
+                                           float2 all, float inv, const TeacherSoftmax& teacher) {
+  const float log_sum = logf(all.y);
   float total = 0.f;
   for (int k = lane; k < p.top; k += 32) {
     const Entry e = list[k];
-    if (e.at >= 0 && e.p != 0.f) total += e.p * (e.log_p - ((e.s - all.power.m) * p.inv_tau - log_sum));
+    if (e.at >= 0 && e.p != 0.f) total += e.p * (e.log_p - ((e.s - all.x) * p.inv_tau - log_sum));
   }
   total = warp_sum(total);
   if (lane == 0) {
     p.loss[row] = teacher.stray ? __int_as_float(0x7fffffff) : total * p.tau * p.tau;
-    p.stats[row] = make_float4(all.power.m, inv, teacher.max, teacher.inv);
+    p.stats[row] = make_float4(all.x, inv, teacher.max, teacher.inv);
   }
 }
 
@@ -426,177 +431,341 @@ __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams 
     if (any_entry(p, row, lane)) teacher = read_list(p, row, logits, lane, list);
     else empty_row = 1;
   } else {
-    // Whole words, the next ones on their way while these are added.
+    // Whole words, kUnroll at once while the next ones are on their way.
+    constexpr int kStep = kUnroll * kRowThreads;
+    const uint4* from = in.words + in.lo + threadIdx.x;
+    const int words = in.hi - in.lo, rounds = words / kStep;
     uint4 ahead[kUnroll];
-    const int start = in.lo + static_cast<int>(threadIdx.x);
+    if (rounds > 0) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (start + u * kRowThreads < in.hi) ahead[u] = in.words[start + u * kRowThreads];
+      for (int u = 0; u < kUnroll; ++u) ahead[u] = from[u * kRowThreads];
     }
-    for (int w = start; w < in.hi; w += kUnroll * kRowThreads) {
-      if (empty_row) break;  // nothing of the row counts
+    for (int round = 1; round <= rounds; ++round) {
+      uint4 now[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const uint4 word = ahead[u];
-        const int next = w + (kUnroll + u) * kRowThreads;
-        if (next < in.hi) ahead[u] = in.words[next];
-        if (w + u * kRowThreads < in.hi) mine.add<T>(word, p.c);
+      for (int u = 0; u < kUnroll; ++u) now[u] = ahead[u];
+      if (round < rounds) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) ahead[u] = from[round * kStep + u * kRowThreads];
       }
+      if (empty_row) break;  // nothing of the row counts
+      mine.add<T, kUnroll>(now, p.c);
+    }
+    for (int w = rounds * kStep + static_cast<int>(threadIdx.x); w < words; w += kRowThreads) {
+      mine.add<T>(in.words[in.lo + w], p.c);
     }
     if (threadIdx.x == 0 && in.lo > 0 && in.count > 0) mine.add<T>(in.load_partial(0), p.c);
     if (threadIdx.x == 1 && in.hi < in.count) mine.add<T>(in.load_partial(in.count - 1), p.c);
     __syncwarp();
   }
-  const Softmax all = join_row(mine, p.c, rank, ranks);
+  const float2 all = join_row(mine, p.c, rank, ranks);
   if (!lists || rank != 0) return;
   if (empty_row) {
     if (lane == 0) write_empty(p, row);
     return;
   }
-  const float inv = teacher.stray ? __int_as_float(0x7fffffff) : 1.f / all.total();
+  const float inv = teacher.stray ? __int_as_float(0x7fffffff) : 1.f / all.y;
   write_loss(p, row, list, lane, all, inv, teacher);
 }
 
-// Loss and gradient in one pass: each block of the row's cluster copies its
-// slice to shared memory (bulk copies, the first chunk added while the last
-// is on its way), and after the exchange turns it into the gradient.
+// ------------------------------------------------ loss with gradient ----
+
+// Loss and gradient in one pass over the logits. A cluster of blocks walks
+// the rows; a block keeps its slice of a row in shared memory. The streaming
+// warps add the slice chunk by chunk as its bulk copies arrive, exchange
+// (max, sum) with the other blocks, then turn the slice into the gradient
+// chunk by chunk; a chunk they have read for the last time is refilled with
+// the next row's at once. The list warp looks ahead for rows without entries
+// (which are not read at all), issues the copies, and after the streaming
+// warps writes the list's columns again with the teacher's part.
+struct GradBarriers {
+  uint64_t full[kChunks];   // the chunk's copy has arrived
+  uint64_t empty[kChunks];  // every streaming warp has read the chunk for the last time
+  uint64_t joined;          // every streaming warp's pair is there, and the list has been read
+  uint64_t exchanged[2];    // the pairs of all blocks, of alternate rows
+};
+
+enum RowState : int { kEmptyList = 1, kStrayIndex = 2 };
+
+// Whether the row's list is empty or has an index beyond the vocabulary (one warp).
+__device__ __forceinline__ int scan_list(const DistillParams& p, int64_t row, int lane) {
+  bool some = false, stray = false;
+  for (int k = lane; k < p.top; k += 32) {
+    const int64_t index = index_at(p, row, k);
+    if (index >= p.vocab) stray = true;
+    if (index >= 0) some = some || teacher_at(p, row, k) != -INFINITY;
+  }
+  return (__any_sync(0xffffffffu, some) ? 0 : kEmptyList) | (__any_sync(0xffffffffu, stray) ? kStrayIndex : 0);
+}
+
+// Whether two entries of the list name the same column: a hash table of
+// indices, at most half full (one warp).
+__device__ __forceinline__ bool repeats(const DistillParams& p, const Entry* list, int* table, int lane) {
+  const int size = 1 << p.hash_bits;
+  for (int i = lane; i < size; i += 32) table[i] = -1;
+  __syncwarp();
+  bool found = false;
+  for (int k = lane; k < p.top; k += 32) {
+    const int at = list[k].at;
+    if (at < 0) continue;
+    int slot = static_cast<int>((static_cast<uint32_t>(at) * 2654435761u) >> (32 - p.hash_bits));
+    for (;;) {
+      const int old = atomicCAS(&table[slot], -1, at);
+      if (old == at) found = true;
+      if (old == -1 || old == at) break;
+      slot = (slot + 1) & (size - 1);
+    }
+  }
+  return __any_sync(0xffffffffu, found);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kRowBlock, 4) distill_grad_rows(DistillParams p) {
+__global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(DistillParams p) {
   extern __shared__ uint4 shared[];
-  __shared__ __align__(8) uint64_t arrived[kChunks];
-  __shared__ int state;  // 1: the row has no entries; 2: a copy did not arrive
+  __shared__ GradBarriers bars;
+  __shared__ int states[2];
+  __shared__ float upstream[2];
   __shared__ int32_t abort;
-  __shared__ float row_inv;
+  __shared__ float2 warp_parts[kRowThreads / 32];
+  __shared__ float2 parts[2][kMaxCluster];
   constexpr int kPer = 16 / sizeof(T);
   Entry* list = reinterpret_cast<Entry*>(shared);
-  uint4* stage = shared + p.top;  // an Entry is 16 bytes
+  int* table = reinterpret_cast<int*>(shared + p.top);
+  uint4* stage = shared + p.top + (1 << p.hash_bits) / 4;
   const uint32_t rank = cluster_ctarank();
   uint32_t ranks;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const int64_t row = blockIdx.x / ranks;
-  const int lane = threadIdx.x & 31;
-  const bool lists = threadIdx.x >= kRowThreads;
-  if (threadIdx.x == kRowThreads) {
-    for (int i = 0; i < kChunks; ++i) mbar_init(&arrived[i], 1);
+  const int64_t clusters = gridDim.x / ranks;
+  const int64_t first_row = blockIdx.x / ranks;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const bool lists = tid >= kRowThreads;
+  const uint32_t exchange_bytes = ranks * sizeof(float2);
+  if (tid == kRowThreads) {
+    for (int i = 0; i < kChunks; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], kRowThreads / 32);
+    }
+    mbar_init(&bars.joined, kRowThreads / 32 + 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.exchanged[i], 1);
+      mbar_arrive_expect_tx(&bars.exchanged[i], exchange_bytes);
+    }
     fence_barrier_init();
-    state = 0;
     abort = 0;
   }
-  __syncthreads();
+  cluster_sync();
 
-  const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
-  T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
-  const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(rank) * p.slice, p.slice);
-  const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
-  const int chunk = (in.count + kChunks * kRowThreads - 1) / (kChunks * kRowThreads) * kRowThreads;
-  Softmax mine;
-  TeacherSoftmax teacher{0.f, 0.f, false};
+  // False for the whole warp once a wait of the block has run out. Every wait
+  // is of this kind, so the warps then leave their loops one after the other
+  // and meet at the cluster's last barrier.
+  auto wait = [&](uint64_t* bar, uint32_t phase) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, phase, kWaitOther, &abort, p.watchdog)) != 0;
+  };
+  auto words_of = [&](int64_t row) {
+    return RowWords<T>(static_cast<const T*>(p.logits) + row * p.row_stride, static_cast<int>(p.vocab),
+                       static_cast<int>(rank) * p.slice, p.slice);
+  };
+  // All rows use chunks of the same size: a slot is refilled by the next row's.
+  const int chunk = (p.slice + kChunks * kRowThreads - 1) / (kChunks * kRowThreads) * kRowThreads;
+  auto row_softmax = [&](uint32_t exchange) {
+    return join_parts(parts[exchange & 1], static_cast<int>(ranks), lane, p.c);
+  };
+
+  uint32_t exchange = 0;  // rows with entries so far
   if (lists) {
-    const bool some = any_entry(p, row, lane);
-    if (some) {
-      if (lane == 0 && in.lo > 0 && in.count > 0) stage[0] = in.load_partial(0);
-      if (lane == 0 && in.hi < in.count) stage[in.count - 1] = in.load_partial(in.count - 1);
-    } else if (lane == 0) {
-      state = 1;
+    auto prepare = [&](int64_t row, uint32_t turn) {
+      const int state = scan_list(p, row, lane);
+      if (lane == 0) {
+        states[turn & 1] = state;
+        upstream[turn & 1] = p.upstream != nullptr ? p.upstream[row * p.upstream_stride] : 1.f;
+      }
+      return state;
+    };
+    uint32_t issued = 0;  // parity of each chunk's latest copy
+    auto issue = [&](const RowWords<T>& in, int state, int i, uint32_t turn) {
+      issued = (issued & ~(1u << i)) | (turn & 1) << i;
+      if (lane != 0) return;
+      const int from = max(in.lo, i * chunk), to = min(in.hi, (i + 1) * chunk);
+      const bool read = (state & kEmptyList) == 0;
+      if (read && in.count > 0) {
+        if (in.lo > 0 && i == 0) stage[0] = in.load_partial(0);
+        if (in.hi < in.count && (in.count - 1) / chunk == i) stage[in.count - 1] = in.load_partial(in.count - 1);
+      }
+      if (read && from < to) {
+        const uint32_t bytes = static_cast<uint32_t>(to - from) * 16;
+        mbar_arrive_expect_tx(&bars.full[i], bytes);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(stage + from)),
+            "l"(in.words + from), "r"(bytes), "r"(smem_u32(&bars.full[i]))
+            : "memory");
+      } else {
+        mbar_arrive(&bars.full[i]);
+      }
+    };
+    int state = kEmptyList;
+    if (first_row < p.rows) {
+      state = prepare(first_row, 0);
+      __syncwarp();
+      const RowWords<T> in = words_of(first_row);
+      for (int i = 0; i < kChunks; ++i) issue(in, state, i, 0);
+      __syncwarp();
     }
-    if (lane == 0) {
-      for (int i = 0; i < kChunks; ++i) {
-        const int from = max(in.lo, i * chunk), to = min(in.hi, (i + 1) * chunk);
-        if (some && from < to) {
-          const uint32_t bytes = static_cast<uint32_t>(to - from) * 16;
-          mbar_arrive_expect_tx(&arrived[i], bytes);
-          asm volatile(
-              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                  smem_u32(stage + from)),
-              "l"(in.words + from), "r"(bytes), "r"(smem_u32(&arrived[i]))
-              : "memory");
-        } else {
-          mbar_arrive(&arrived[i]);
+    uint32_t turn = 0;
+    for (int64_t row = first_row; row < p.rows; row += clusters, ++turn) {
+      const bool some = (state & kEmptyList) == 0;
+      const RowWords<T> in = words_of(row);
+      T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
+      TeacherSoftmax teacher{0.f, 0.f, false};
+      bool shared_column = false;
+      if (some) {
+        teacher = read_list(p, row, in.row, lane, list);
+        shared_column = repeats(p, list, table, lane);
+        __syncwarp();
+        // Not before the list's logits are here may any block write (the
+        // gradient may replace them).
+        if (lane == 0) mbar_arrive(&bars.joined);
+      }
+      const float a = p.tau * upstream[turn & 1];
+      int next_state = kEmptyList;
+      const bool more = row + clusters < p.rows;
+      if (more) next_state = prepare(row + clusters, turn + 1);
+      float2 all{0.f, 0.f};
+      float inv = 0.f;
+      if (some) {
+        if (!wait(&bars.exchanged[exchange & 1], exchange >> 1 & 1)) break;
+        all = row_softmax(exchange);
+        ++exchange;
+        inv = teacher.stray ? __int_as_float(0x7fffffff) : 1.f / all.y;
+        if (rank == 0) write_loss(p, row, list, lane, all, inv, teacher);
+      } else if (rank == 0 && lane == 0) {
+        write_empty(p, row);
+      }
+      const RowWords<T> next = words_of(more ? row + clusters : row);
+      bool drained = true;
+      for (int i = 0; i < kChunks && drained; ++i) {
+        drained = wait(&bars.empty[i], turn & 1);
+        if (more && drained) issue(next, next_state, i, turn + 1);
+      }
+      __syncwarp();
+      if (!drained) break;
+      if (some) {
+        for (int k = lane; k < p.top; k += 32) {
+          const Entry e = list[k];
+          const int at = e.at + in.phase - in.first * kPer;
+          if (e.at < 0 || at < 0 || at >= in.count * kPer) continue;
+          float prob = e.p;
+          if (shared_column) {  // every entry of the column writes the same sum
+            prob = 0.f;
+            for (int j = 0; j < p.top; ++j) {
+              if (list[j].at == e.at) prob += list[j].p;
+            }
+          }
+          grad[e.at] = from_float<T>(a * (Exponent(all.x)(e.s, p.c) * inv - prob));
         }
+        __syncwarp();
+      }
+      state = next_state;
+    }
+    if (abort != 0 && lane == 0) {  // leave no copy behind in flight
+      for (int i = 0; i < kChunks; ++i) mbar_drain(&bars.full[i], issued >> i & 1);
+    }
+  } else {
+    uint32_t turn = 0;
+    for (int64_t row = first_row; row < p.rows; row += clusters, ++turn) {
+      const RowWords<T> in = words_of(row);
+      T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
+      const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
+      if (!wait(&bars.full[0], turn & 1)) break;
+      const int state = states[turn & 1];
+      const float a = p.tau * upstream[turn & 1];
+      bool arrived = true;
+      if (state & kEmptyList) {
+        for (int i = 1; i < kChunks && arrived; ++i) arrived = wait(&bars.full[i], turn & 1);
+        if (!arrived) break;
+        for (int w = tid; w < in.count; w += kRowThreads) in.store(grad, same_phase, w, make_uint4(0, 0, 0, 0));
+        __syncwarp();
+        if (lane == 0) {
+          for (int i = 0; i < kChunks; ++i) mbar_arrive(&bars.empty[i]);
+        }
+        continue;
+      }
+      Softmax mine;
+      for (int i = 0; i < kChunks && arrived; ++i) {
+        if (i > 0) arrived = wait(&bars.full[i], turn & 1);
+        const int to = min(in.count, (i + 1) * chunk);
+        int w = i * chunk + tid;
+        for (; w + (kAtOnce - 1) * kRowThreads < to; w += kAtOnce * kRowThreads) {
+          uint4 words[kAtOnce];
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u) words[u] = stage[w + u * kRowThreads];
+          mine.add<T, kAtOnce>(words, p.c);
+        }
+        for (; w < to; w += kRowThreads) mine.add<T>(stage[w], p.c);
+      }
+      __syncwarp();
+      if (!arrived) break;
+      const float2 part = join_lanes<32>(mine.pair(), p.c);
+      if (lane == 0) {
+        warp_parts[tid / 32] = part;
+        mbar_arrive(&bars.joined);
+      }
+      if (tid < 32) {
+        if (!wait(&bars.joined, exchange & 1)) break;
+        const float2 block = join_parts(warp_parts, kRowThreads / 32, lane, p.c);
+        if (lane < static_cast<int>(ranks)) {  // one lane per block of the cluster
+          asm volatile(
+              "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+                  mapa_shared(&parts[exchange & 1][rank], static_cast<uint32_t>(lane))),
+              "f"(block.x), "f"(block.y),
+              "r"(mapa_shared(&bars.exchanged[exchange & 1], static_cast<uint32_t>(lane)))
+              : "memory");
+        }
+        __syncwarp();
+      }
+      if (!wait(&bars.exchanged[exchange & 1], exchange >> 1 & 1)) break;
+      // For the row after the next one: no block sends its pair before this
+      // one has sent the next row's.
+      if (tid == 0) mbar_arrive_expect_tx(&bars.exchanged[exchange & 1], exchange_bytes);
+      const float2 all = row_softmax(exchange);
+      ++exchange;
+      const float inv = (state & kStrayIndex) ? __int_as_float(0x7fffffff) : 1.f / all.y;
+      const Exponent power(all.x);
+      const Pair scaled(a * inv);
+      auto gradient = [&](const uint4& word) {
+        Pair v[kPer / 2];
+        unpack_pairs<T>(word, v);
+        float f[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) mul2(power(v[e], p.c), scaled).split(f[2 * e], f[2 * e + 1]);
+        return pack_word<T>(f);
+      };
+      for (int i = 0; i < kChunks; ++i) {
+        const int from = i * chunk, to = min(in.count, (i + 1) * chunk);
+        if (same_phase) {
+          uint4* out = reinterpret_cast<uint4*>(grad + in.element(0));  // only whole words of it are written
+          const int end = min(in.hi, to);
+          int w = max(in.lo, from) + tid;
+          for (; w + (kAtOnce - 1) * kRowThreads < end; w += kAtOnce * kRowThreads) {
+            uint4 words[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) words[u] = gradient(stage[w + u * kRowThreads]);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) out[w + u * kRowThreads] = words[u];
+          }
+          for (; w < end; w += kRowThreads) out[w] = gradient(stage[w]);
+          if (tid == 0 && from < in.lo && from < to) in.store(grad, false, 0, gradient(stage[0]));
+          if (tid == 0 && in.hi >= from && in.hi < to) in.store(grad, false, in.hi, gradient(stage[in.hi]));
+        } else {
+          for (int w = from + tid; w < to; w += kRowThreads) in.store(grad, false, w, gradient(stage[w]));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.empty[i]);
       }
     }
-    __syncwarp();
-    if (some) teacher = read_list(p, row, logits, lane, list);
-  } else {
-    for (int i = 0; i < kChunks; ++i) {
-      mbar_wait(&arrived[i], 0, kWaitOther, &abort, p.watchdog);
-      if (state == 1) break;
-      const int to = min(in.count, (i + 1) * chunk);
-#pragma unroll 2
-      for (int w = i * chunk + static_cast<int>(threadIdx.x); w < to; w += kRowThreads) mine.add<T>(stage[w], p.c);
-    }
-    __syncwarp();
-  }
-  const Softmax all = join_row(mine, p.c, rank, ranks);
-  if (abort != 0 && threadIdx.x == 0) {  // never leave a copy behind in flight
-    for (int i = 0; i < kChunks; ++i) mbar_drain(&arrived[i], 0);
-  }
-  if (state == 1) {
-    if (!lists) {
-      for (int w = threadIdx.x; w < in.count; w += kRowThreads) in.store(grad, same_phase, w, make_uint4(0, 0, 0, 0));
-    } else if (rank == 0 && lane == 0) {
-      write_empty(p, row);
-    }
-    return;
-  }
-  const float nan = __int_as_float(0x7fffffff);
-  if (lists) {
-    const float inv = teacher.stray || abort != 0 ? nan : 1.f / all.total();
-    if (lane == 0) row_inv = inv;
-    if (rank == 0) write_loss(p, row, list, lane, all, inv, teacher);
-  }
-  __syncthreads();
-  const float inv = row_inv;
-  float a = p.tau;
-  if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
-  if (!lists) {
-    const Pair scaled(a * inv);
-#pragma unroll 2
-    for (int w = threadIdx.x; w < in.count; w += kRowThreads) {
-      Pair v[kPer / 2];
-      unpack_pairs<T>(stage[w], v);
-      all.power.apply<kPer / 2>(v, p.c);
-      float f[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer / 2; ++i) mul2(v[i], scaled).split(f[2 * i], f[2 * i + 1]);
-      in.store(grad, same_phase, w, pack_word<T>(f));
-    }
-  }
-  __syncthreads();
-  if (!lists) return;
-  // The list's columns again, with the teacher's part. Each entry leaves its
-  // number in its (no longer needed) staged logit: one that finds another
-  // number there shares its column.
-  using Mark = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
-  Mark* mark = reinterpret_cast<Mark*>(stage);
-  auto local = [&](int k) {
-    const int e = list[k].at + in.phase - in.first * kPer;
-    return list[k].at >= 0 && e >= 0 && e < in.count * kPer ? e : -1;
-  };
-  for (int k = lane; k < p.top; k += 32) {
-    const int e = local(k);
-    if (e >= 0) mark[e] = static_cast<Mark>(k);
   }
   __syncwarp();
-  bool shared_column = false;
-  for (int k = lane; k < p.top; k += 32) {
-    const int e = local(k);
-    if (e >= 0 && mark[e] != static_cast<Mark>(k)) shared_column = true;
-  }
-  shared_column = __any_sync(0xffffffffu, shared_column);
-  for (int k = lane; k < p.top; k += 32) {
-    if (local(k) < 0) continue;
-    const Entry e = list[k];
-    float prob = e.p;
-    if (shared_column) {  // every entry of the column writes the same sum
-      prob = 0.f;
-      for (int j = 0; j < p.top; ++j) {
-        if (list[j].at == e.at) prob += list[j].p;
-      }
-    }
-    grad[e.at] = from_float<T>(a * (all.power(e.s, p.c) * inv - prob));
-  }
+  cluster_sync();  // the other blocks may still be sending their pairs
 }
 
 // The gradient from the row statistics: one read, one write, blocks of a row
@@ -626,7 +795,7 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
   float a = p.tau;
   if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
   if (p.upstream_scale != nullptr) a *= *p.upstream_scale;
-  const Exponent power(stats.x, p.c);
+  const Exponent power(stats.x);
 
   // This block's entries of the list; their logits before they are
   // overwritten (the gradient may replace the logits).
@@ -660,10 +829,9 @@ __global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p
     if (w >= in.count) continue;
     Pair v[kPer / 2];
     unpack_pairs<T>(raw[u], v);
-    power.apply<kPer / 2>(v, p.c);
     float f[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) mul2(v[i], scaled).split(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < kPer / 2; ++i) mul2(power(v[i], p.c), scaled).split(f[2 * i], f[2 * i + 1]);
     in.store(grad, same_phase, w, empty ? make_uint4(0, 0, 0, 0) : pack_word<T>(f));
   }
   __syncthreads();
@@ -750,9 +918,15 @@ int max_words(int64_t vocab, int dtype) {
   return static_cast<int>(ceil_div(vocab + per - 1, per));  // whatever the row's phase
 }
 
+int hash_bits(int top) {
+  int bits = 6;
+  while ((1 << bits) < 2 * top) ++bits;
+  return bits;
+}
+
 size_t shared_bytes(int64_t vocab, int dtype, int top, int cluster, bool grad) {
   return static_cast<size_t>(top) * sizeof(Entry) +
-         (grad ? static_cast<size_t>(ceil_div(max_words(vocab, dtype), cluster)) * 16 : 0);
+         (grad ? (sizeof(int) << hash_bits(top)) + static_cast<size_t>(ceil_div(max_words(vocab, dtype), cluster)) * 16 : 0);
 }
 
 // Blocks per row: the gradient's slice should let four blocks share an SM
@@ -771,19 +945,9 @@ int cluster_size(int64_t rows, int64_t vocab, int dtype, int top, bool grad) {
 template <typename T, bool GRAD>
 int launch_rows(DistillParams p, int64_t rows, int cluster, size_t shared, cudaStream_t stream) {
   void (*kernel)(DistillParams) = GRAD ? distill_grad_rows<T> : distill_loss_rows<T>;
-  if (GRAD) {
-    static std::atomic<uint64_t> prepared{0};
-    int device = 0;
-    SDC_CUDA_CHECK(cudaGetDevice(&device));
-    const uint64_t bit = 1ull << (device & 63);
-    if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
-      SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          static_cast<int>(kSharedLimit - 2048)));
-      prepared.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
+  int64_t clusters = rows;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(rows * cluster));
+  config.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
   config.blockDim = dim3(kRowBlock);
   config.dynamicSmemBytes = shared;
   config.stream = stream;
@@ -794,6 +958,26 @@ int launch_rows(DistillParams p, int64_t rows, int cluster, size_t shared, cudaS
   attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
+  if (GRAD) {
+    // As many clusters as are resident at a time walk the rows. Asked once
+    // for each device, cluster size and amount of shared memory in use.
+    struct Resident {
+      int device = -1, cluster = 0, clusters = 0;
+      size_t shared = 0;
+    };
+    static thread_local Resident last;
+    int device = 0;
+    SDC_CUDA_CHECK(cudaGetDevice(&device));
+    if (last.device != device || last.cluster != cluster || last.shared != shared) {
+      SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          static_cast<int>(kSharedLimit - 2048)));
+      config.gridDim = dim3(static_cast<unsigned>(cluster));
+      SDC_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&last.clusters, kernel, &config));
+      last.device = device, last.cluster = cluster, last.shared = shared;
+    }
+    clusters = std::min<int64_t>(rows, std::max(last.clusters, 1));
+    config.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
+  }
   SDC_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, p));
   return SDC_OK;
 }
@@ -802,6 +986,8 @@ template <bool GRAD>
 int run_rows(DistillParams p, int dtype, int64_t rows, int cluster, cudaStream_t stream) {
   SDC_REQUIRE(rows <= INT_MAX / cluster, "distillation has too many rows for one launch");
   p.slice = static_cast<int>(ceil_div(max_words(p.vocab, dtype), cluster));
+  p.rows = rows;
+  p.hash_bits = hash_bits(p.top);
   p.watchdog = watchdog_ptr();
   if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "distillation has no watchdog word on this device");
   const size_t shared = shared_bytes(p.vocab, dtype, p.top, cluster, GRAD);
