@@ -33,16 +33,19 @@ namespace {
 constexpr int kRowThreads = 256;               // threads that stream the slice
 constexpr int kRowBlock = kRowThreads + 32;    // and one warp for the teacher's list
 constexpr int kUnroll = 4;                      // words at once from global memory
-constexpr int kAtOnce = 4;                      // and from shared memory
-constexpr int kChunks = 4;                     // pieces of a slice copied under one barrier each
+constexpr int kAtOnce = 2;                      // and from shared memory
+constexpr int kChunks = 2;                     // pieces of a slice copied under one barrier each
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kGradBlocks = 4;                 // of loss with gradient on an SM
+constexpr int kGradBlocks = 3;
 constexpr size_t kSharedLimit = 227 * 1024;
-// Four blocks per SM: some load while others compute, exchange or write.
-constexpr size_t kSliceTarget = 50 * 1024;
+// Three blocks of loss with gradient on an SM: some compute while others
+// exchange. At 4096 x 151936 bf16 this took 520 us; two blocks of 80 KB 560,
+// four of 50 KB 550 (the exchange costs each block about a microsecond a row),
+// one of 152 KB 550.
+constexpr size_t kSliceTarget = 74 * 1024;
 constexpr int kBackThreads = 256;
-constexpr int kBackGranules = 8;               // 16-byte words per thread
+constexpr int kBackWords = 4;                  // 16-byte words per thread of the backward pass
 
 struct DistillParams {
   const void* logits;
@@ -112,6 +115,9 @@ struct RowWords {
     hi = max(lo, count - (first + count == all && (phase + vocab) % kPer != 0));
   }
   __device__ __forceinline__ int element(int word) const { return (first + word) * kPer - phase; }
+  __device__ __forceinline__ bool holds(int e) const {
+    return e + phase >= first * kPer && e + phase < (first + count) * kPer;
+  }
   // Word with elements outside the row; they read as -inf.
   __device__ __forceinline__ uint4 load_partial(int word) const {
     uint4 r;
@@ -175,11 +181,6 @@ struct Pair {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
   }
 };
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   Pair d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
@@ -263,10 +264,6 @@ struct Softmax {
     for (int n = 1; n < N; ++n) part[0] = add2(part[0], part[n]);
     sums = add2(sums, part[0]);
   }
-  template <typename T>
-  __device__ __forceinline__ void add(const uint4& word, float c) {
-    add<T, 1>(&word, c);
-  }
   __device__ __forceinline__ float2 pair() const {
     float lo, hi;
     sums.split(lo, hi);
@@ -303,47 +300,56 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // What the list warp keeps of an entry.
 struct Entry {
-  float p;     // teacher probability
-  float log_p; // its natural logarithm
-  float s;     // student logit
-  int at;      // index, -1: no entry
+  float p;      // teacher probability
+  float column; // that of all entries with the same index (loss with gradient)
+  float s;      // student logit
+  int at;       // index, -1: no entry
 };
-
-// Whether the row's list has an entry (one warp).
-__device__ __forceinline__ bool any_entry(const DistillParams& p, int64_t row, int lane) {
-  bool some = false;
-  for (int k = 0; k < p.top && !some; k += 32) {
-    bool entry = false;
-    if (k + lane < p.top) entry = is_entry(index_at(p, row, k + lane), teacher_at(p, row, k + lane));
-    some = __any_sync(0xffffffffu, entry);
-  }
-  return some;
-}
 
 struct TeacherSoftmax {
   float max, inv;
-  bool stray;  // an index beyond the vocabulary
+  float entropy;  // -sum p ln p
+  bool stray;     // an index beyond the vocabulary
+  bool empty;     // no entry
 };
 
-// Fills `list` (one warp): the teacher's softmax and the student's logits at its indices.
+// Fills `list` (one warp): the teacher's softmax, and the student's logits at
+// the indices of this block's slice, or `everywhere`. Four entries a lane are
+// on their way at a time.
 template <typename T>
-__device__ __forceinline__ TeacherSoftmax read_list(const DistillParams& p, int64_t row, const T* logits, int lane,
-                                                    Entry* list) {
-  TeacherSoftmax t{-INFINITY, 0.f, false};
-  for (int k = lane; k < p.top; k += 32) {
-    const int64_t index = index_at(p, row, k);
-    Entry e{teacher_at(p, row, k), 0.f, 0.f, -1};
-    if (index >= p.vocab) {
-      t.stray = true;
-    } else if (is_entry(index, e.p)) {
-      e.at = static_cast<int>(index);
-      e.s = to_float(logits[index]);
-      t.max = fmaxf(t.max, e.p);
+__device__ __forceinline__ TeacherSoftmax read_list(const DistillParams& p, int64_t row, const RowWords<T>& in,
+                                                    bool everywhere, int lane, Entry* list) {
+  TeacherSoftmax t{-INFINITY, 0.f, 0.f, false, true};
+  for (int base = lane; base < p.top; base += 128) {
+    int64_t index[4];
+    Entry e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in_list = base + 32 * i < p.top;
+      index[i] = in_list ? index_at(p, row, base + 32 * i) : -1;
+      e[i] = Entry{in_list ? teacher_at(p, row, base + 32 * i) : 0.f, 0.f, 0.f, -1};
     }
-    list[k] = e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!is_entry(index[i], e[i].p)) continue;
+      t.empty = false;
+      if (index[i] >= p.vocab) {
+        t.stray = true;
+        continue;
+      }
+      e[i].at = static_cast<int>(index[i]);
+      if (everywhere || in.holds(e[i].at)) e[i].s = to_float(in.row[e[i].at]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e[i].at >= 0) t.max = fmaxf(t.max, e[i].p);
+      if (base + 32 * i < p.top) list[base + 32 * i] = e[i];
+    }
   }
   t.max = warp_max(t.max);
   t.stray = __any_sync(0xffffffffu, t.stray);
+  t.empty = __all_sync(0xffffffffu, t.empty);
+  if (t.empty) return t;
   float sum = 0.f;
   for (int k = lane; k < p.top; k += 32) {
     if (list[k].at >= 0) sum += exp2_fast((list[k].p - t.max) * p.c);
@@ -353,9 +359,11 @@ __device__ __forceinline__ TeacherSoftmax read_list(const DistillParams& p, int6
   const float log_sum = logf(sum);
   for (int k = lane; k < p.top; k += 32) {
     const float x = list[k].p - t.max;
-    list[k].log_p = x * p.inv_tau - log_sum;
-    list[k].p = exp2_fast(x * p.c) * t.inv;
+    const float prob = exp2_fast(x * p.c) * t.inv;
+    if (list[k].at >= 0 && prob != 0.f) t.entropy -= prob * (x * p.inv_tau - log_sum);
+    list[k].p = list[k].column = prob;
   }
+  t.entropy = warp_sum(t.entropy);
   __syncwarp();
   return t;
 }
@@ -393,9 +401,9 @@ __device__ __forceinline__ void write_loss(const DistillParams& p, int64_t row, 
   float total = 0.f;
   for (int k = lane; k < p.top; k += 32) {
     const Entry e = list[k];
-    if (e.at >= 0 && e.p != 0.f) total += e.p * (e.log_p - ((e.s - all.x) * p.inv_tau - log_sum));
+    if (e.at >= 0 && e.p != 0.f) total -= e.p * ((e.s - all.x) * p.inv_tau - log_sum);
   }
-  total = warp_sum(total);
+  total = warp_sum(total) - teacher.entropy;
   if (lane == 0) {
     p.loss[row] = teacher.stray ? __int_as_float(0x7fffffff) : total * p.tau * p.tau;
     p.stats[row] = make_float4(all.x, inv, teacher.max, teacher.inv);
@@ -426,10 +434,10 @@ __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams 
   const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
   const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(rank) * p.slice, p.slice);
   Softmax mine;
-  TeacherSoftmax teacher{0.f, 0.f, false};
+  TeacherSoftmax teacher{};
   if (lists) {
-    if (any_entry(p, row, lane)) teacher = read_list(p, row, logits, lane, list);
-    else empty_row = 1;
+    teacher = read_list(p, row, in, rank == 0, lane, list);
+    if (teacher.empty) empty_row = 1;
   } else {
     // Whole words, kUnroll at once while the next ones are on their way.
     constexpr int kStep = kUnroll * kRowThreads;
@@ -452,10 +460,12 @@ __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams 
       mine.add<T, kUnroll>(now, p.c);
     }
     for (int w = rounds * kStep + static_cast<int>(threadIdx.x); w < words; w += kRowThreads) {
-      mine.add<T>(in.words[in.lo + w], p.c);
+      mine.add<T, 1>(in.words + in.lo + w, p.c);
     }
-    if (threadIdx.x == 0 && in.lo > 0 && in.count > 0) mine.add<T>(in.load_partial(0), p.c);
-    if (threadIdx.x == 1 && in.hi < in.count) mine.add<T>(in.load_partial(in.count - 1), p.c);
+    if ((threadIdx.x == 0 && in.lo > 0 && in.count > 0) || (threadIdx.x == 1 && in.hi < in.count)) {
+      const uint4 word = in.load_partial(threadIdx.x == 0 ? 0 : in.count - 1);
+      mine.add<T, 1>(&word, p.c);
+    }
     __syncwarp();
   }
   const float2 all = join_row(mine, p.c, rank, ranks);
@@ -487,36 +497,47 @@ struct GradBarriers {
 
 enum RowState : int { kEmptyList = 1, kStrayIndex = 2 };
 
-// Whether the row's list is empty or has an index beyond the vocabulary (one warp).
-__device__ __forceinline__ int scan_list(const DistillParams& p, int64_t row, int lane) {
-  bool some = false, stray = false;
-  for (int k = lane; k < p.top; k += 32) {
-    const int64_t index = index_at(p, row, k);
-    if (index >= p.vocab) stray = true;
-    if (index >= 0) some = some || teacher_at(p, row, k) != -INFINITY;
-  }
-  return (__any_sync(0xffffffffu, some) ? 0 : kEmptyList) | (__any_sync(0xffffffffu, stray) ? kStrayIndex : 0);
-}
-
-// Whether two entries of the list name the same column: a hash table of
-// indices, at most half full (one warp).
-__device__ __forceinline__ bool repeats(const DistillParams& p, const Entry* list, int* table, int lane) {
+// Sums the probabilities of entries that name the same column of this block's
+// slice: a hash table of indices, at most half full, finds them (one warp).
+template <typename T>
+__device__ __forceinline__ void join_columns(const DistillParams& p, const RowWords<T>& in, Entry* list, int* table,
+                                             int lane) {
+  constexpr int kTwice = static_cast<int>(0x80000000u);
   const int size = 1 << p.hash_bits;
   for (int i = lane; i < size; i += 32) table[i] = -1;
   __syncwarp();
+  auto first_slot = [&](int at) {
+    return static_cast<int>((static_cast<uint32_t>(at) * 2654435761u) >> (32 - p.hash_bits));
+  };
   bool found = false;
   for (int k = lane; k < p.top; k += 32) {
     const int at = list[k].at;
-    if (at < 0) continue;
-    int slot = static_cast<int>((static_cast<uint32_t>(at) * 2654435761u) >> (32 - p.hash_bits));
-    for (;;) {
+    if (at < 0 || !in.holds(at)) continue;
+    for (int slot = first_slot(at);; slot = (slot + 1) & (size - 1)) {
       const int old = atomicCAS(&table[slot], -1, at);
-      if (old == at) found = true;
-      if (old == -1 || old == at) break;
-      slot = (slot + 1) & (size - 1);
+      if (old == -1) break;
+      if ((old & ~kTwice) == at) {
+        atomicOr(&table[slot], kTwice);
+        found = true;
+        break;
+      }
     }
   }
-  return __any_sync(0xffffffffu, found);
+  if (!__any_sync(0xffffffffu, found)) return;
+  __syncwarp();
+  for (int k = lane; k < p.top; k += 32) {
+    const int at = list[k].at;
+    if (at < 0 || !in.holds(at)) continue;
+    int slot = first_slot(at);
+    while ((table[slot] & ~kTwice) != at) slot = (slot + 1) & (size - 1);
+    if ((table[slot] & kTwice) == 0) continue;
+    float column = 0.f;
+    for (int j = 0; j < p.top; ++j) {
+      if (list[j].at == at) column += list[j].p;
+    }
+    list[k].column = column;
+  }
+  __syncwarp();
 }
 
 template <typename T>
@@ -529,9 +550,9 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
   __shared__ float2 warp_parts[kRowThreads / 32];
   __shared__ float2 parts[2][kMaxCluster];
   constexpr int kPer = 16 / sizeof(T);
-  Entry* list = reinterpret_cast<Entry*>(shared);
-  int* table = reinterpret_cast<int*>(shared + p.top);
-  uint4* stage = shared + p.top + (1 << p.hash_bits) / 4;
+  Entry* lists_of[2] = {reinterpret_cast<Entry*>(shared), reinterpret_cast<Entry*>(shared + p.top)};
+  int* table = reinterpret_cast<int*>(shared + 2 * p.top);
+  uint4* stage = shared + 2 * p.top + (1 << p.hash_bits) / 4;
   const uint32_t rank = cluster_ctarank();
   uint32_t ranks;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -573,20 +594,26 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
 
   uint32_t exchange = 0;  // rows with entries so far
   if (lists) {
+    // A row's list is read while the row before it is worked on. (The row's
+    // logits are still there: no block replaces them with the gradient before
+    // this one has sent its pair for the row.)
     auto prepare = [&](int64_t row, uint32_t turn) {
-      const int state = scan_list(p, row, lane);
+      Entry* list = lists_of[turn & 1];
+      const RowWords<T> in = words_of(row);
+      const TeacherSoftmax t = read_list(p, row, in, rank == 0, lane, list);
+      if (!t.empty) join_columns(p, in, list, table, lane);
       if (lane == 0) {
-        states[turn & 1] = state;
+        states[turn & 1] = (t.empty ? kEmptyList : 0) | (t.stray ? kStrayIndex : 0);
         upstream[turn & 1] = p.upstream != nullptr ? p.upstream[row * p.upstream_stride] : 1.f;
       }
-      return state;
+      __syncwarp();
+      return t;
     };
     uint32_t issued = 0;  // parity of each chunk's latest copy
-    auto issue = [&](const RowWords<T>& in, int state, int i, uint32_t turn) {
+    auto issue = [&](const RowWords<T>& in, bool read, int i, uint32_t turn) {
       issued = (issued & ~(1u << i)) | (turn & 1) << i;
       if (lane != 0) return;
       const int from = max(in.lo, i * chunk), to = min(in.hi, (i + 1) * chunk);
-      const bool read = (state & kEmptyList) == 0;
       if (read && in.count > 0) {
         if (in.lo > 0 && i == 0) stage[0] = in.load_partial(0);
         if (in.hi < in.count && (in.count - 1) / chunk == i) stage[in.count - 1] = in.load_partial(in.count - 1);
@@ -603,33 +630,24 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
         mbar_arrive(&bars.full[i]);
       }
     };
-    int state = kEmptyList;
+    TeacherSoftmax teacher{};
     if (first_row < p.rows) {
-      state = prepare(first_row, 0);
-      __syncwarp();
+      teacher = prepare(first_row, 0);
       const RowWords<T> in = words_of(first_row);
-      for (int i = 0; i < kChunks; ++i) issue(in, state, i, 0);
+      for (int i = 0; i < kChunks; ++i) issue(in, !teacher.empty, i, 0);
       __syncwarp();
     }
     uint32_t turn = 0;
     for (int64_t row = first_row; row < p.rows; row += clusters, ++turn) {
-      const bool some = (state & kEmptyList) == 0;
+      const Entry* list = lists_of[turn & 1];
+      const bool some = !teacher.empty;
       const RowWords<T> in = words_of(row);
       T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
-      TeacherSoftmax teacher{0.f, 0.f, false};
-      bool shared_column = false;
-      if (some) {
-        teacher = read_list(p, row, in.row, lane, list);
-        shared_column = repeats(p, list, table, lane);
-        __syncwarp();
-        // Not before the list's logits are here may any block write (the
-        // gradient may replace them).
-        if (lane == 0) mbar_arrive(&bars.joined);
-      }
+      if (some && lane == 0) mbar_arrive(&bars.joined);
       const float a = p.tau * upstream[turn & 1];
-      int next_state = kEmptyList;
+      TeacherSoftmax next_teacher{};
       const bool more = row + clusters < p.rows;
-      if (more) next_state = prepare(row + clusters, turn + 1);
+      if (more) next_teacher = prepare(row + clusters, turn + 1);
       float2 all{0.f, 0.f};
       float inv = 0.f;
       if (some) {
@@ -645,27 +663,19 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
       bool drained = true;
       for (int i = 0; i < kChunks && drained; ++i) {
         drained = wait(&bars.empty[i], turn & 1);
-        if (more && drained) issue(next, next_state, i, turn + 1);
+        if (more && drained) issue(next, !next_teacher.empty, i, turn + 1);
       }
       __syncwarp();
       if (!drained) break;
       if (some) {
         for (int k = lane; k < p.top; k += 32) {
           const Entry e = list[k];
-          const int at = e.at + in.phase - in.first * kPer;
-          if (e.at < 0 || at < 0 || at >= in.count * kPer) continue;
-          float prob = e.p;
-          if (shared_column) {  // every entry of the column writes the same sum
-            prob = 0.f;
-            for (int j = 0; j < p.top; ++j) {
-              if (list[j].at == e.at) prob += list[j].p;
-            }
-          }
-          grad[e.at] = from_float<T>(a * (Exponent(all.x)(e.s, p.c) * inv - prob));
+          if (e.at < 0 || !in.holds(e.at)) continue;
+          grad[e.at] = from_float<T>(a * (Exponent(all.x)(e.s, p.c) * inv - e.column));
         }
         __syncwarp();
       }
-      state = next_state;
+      teacher = next_teacher;
     }
     if (abort != 0 && lane == 0) {  // leave no copy behind in flight
       for (int i = 0; i < kChunks; ++i) mbar_drain(&bars.full[i], issued >> i & 1);
@@ -701,7 +711,7 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
           for (int u = 0; u < kAtOnce; ++u) words[u] = stage[w + u * kRowThreads];
           mine.add<T, kAtOnce>(words, p.c);
         }
-        for (; w < to; w += kRowThreads) mine.add<T>(stage[w], p.c);
+        for (; w < to; w += kRowThreads) mine.add<T, 1>(stage + w, p.c);
       }
       __syncwarp();
       if (!arrived) break;
@@ -769,86 +779,96 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
 }
 
 // The gradient from the row statistics: one read, one write, blocks of a row
-// independent of each other.
+// independent of each other. A warp of its own collects the block's entries of
+// the list meanwhile (their logits before they are overwritten: the gradient
+// may replace them) and writes their columns last.
+struct BackEntry {
+  float s, p;
+  int at;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kBackThreads) distill_backward(DistillParams p) {
+__global__ void __launch_bounds__(kBackThreads + 32, 6) distill_backward(DistillParams p) {
+  extern __shared__ uint4 shared[];
   constexpr int kPer = 16 / sizeof(T);
-  constexpr int kWords = kBackThreads * kBackGranules;
-  constexpr int kEntries = kMaxTop / kBackThreads;
+  constexpr int kWords = kBackThreads * kBackWords;
   __shared__ uint32_t seen[(kWords * kPer + 31) / 32];
-  __shared__ int shared_column;
+  BackEntry* list = reinterpret_cast<BackEntry*>(shared);
   const int64_t row = blockIdx.x / p.chunks;
   const T* logits = static_cast<const T*>(p.logits) + row * p.row_stride;
   T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
   const RowWords<T> in(logits, static_cast<int>(p.vocab), static_cast<int>(blockIdx.x % p.chunks) * kWords, kWords);
-  const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
+  const int tid = threadIdx.x, lane = tid & 31;
 
-  const float4 stats = p.stats[row];
-  const bool empty = stats.y == kEmptyRow;
-  uint4 raw[kBackGranules];
+  if (tid < kBackThreads) {
+    uint4 raw[kBackWords];
 #pragma unroll
-  for (int u = 0; u < kBackGranules; ++u) {
-    const int w = static_cast<int>(threadIdx.x) + u * kBackThreads;
-    if (w >= in.lo && w < in.hi) raw[u] = in.words[w];
-    else if (w < in.count) raw[u] = in.load_partial(w);
+    for (int u = 0; u < kBackWords; ++u) {
+      const int w = tid + u * kBackThreads;
+      if (w >= in.lo && w < in.hi) raw[u] = in.words[w];
+      else if (w < in.count) raw[u] = in.load_partial(w);
+    }
+    const float4 stats = p.stats[row];
+    float a = p.tau;
+    if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
+    if (p.upstream_scale != nullptr) a *= *p.upstream_scale;
+    const Exponent power(stats.x);
+    const Pair scaled(a * stats.y);
+    const bool same_phase = static_cast<int>((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) == in.phase;
+    __syncthreads();  // the list's logits have been read
+#pragma unroll
+    for (int u = 0; u < kBackWords; ++u) {
+      const int w = tid + u * kBackThreads;
+      if (w >= in.count) continue;
+      Pair v[kPer / 2];
+      unpack_pairs<T>(raw[u], v);
+      float f[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i) mul2(power(v[i], p.c), scaled).split(f[2 * i], f[2 * i + 1]);
+      in.store(grad, same_phase, w, stats.y == kEmptyRow ? make_uint4(0, 0, 0, 0) : pack_word<T>(f));
+    }
+    __syncthreads();
+    return;
   }
+
+  for (int i = lane; i < static_cast<int>(sizeof(seen) / 4); i += 32) seen[i] = 0;
+  __syncwarp();
+  const float4 stats = p.stats[row];
+  int count = 0;
+  bool shared_column = false;
+  for (int base = 0; base < p.top && stats.y != kEmptyRow; base += 32) {
+    BackEntry e{0.f, 0.f, -1};
+    if (base + lane < p.top) {
+      const int64_t index = index_at(p, row, base + lane);
+      const float t = teacher_at(p, row, base + lane);
+      if (is_entry(index, t) && index < p.vocab) {
+        const int local = static_cast<int>(index) + in.phase - in.first * kPer;
+        if (in.holds(static_cast<int>(index))) {
+          e = BackEntry{to_float(logits[index]), exp2_fast((t - stats.z) * p.c) * stats.w, static_cast<int>(index)};
+          if (atomicOr(&seen[local / 32], 1u << (local % 32)) >> (local % 32) & 1u) shared_column = true;
+        }
+      }
+    }
+    const uint32_t mask = __ballot_sync(0xffffffffu, e.at >= 0);
+    if (e.at >= 0) list[count + __popc(mask & ((1u << lane) - 1))] = e;
+    count += __popc(mask);
+  }
+  shared_column = __any_sync(0xffffffffu, shared_column);
+  __syncthreads();
   float a = p.tau;
   if (p.upstream != nullptr) a *= p.upstream[row * p.upstream_stride];
   if (p.upstream_scale != nullptr) a *= *p.upstream_scale;
-  const Exponent power(stats.x);
-
-  // This block's entries of the list; their logits before they are
-  // overwritten (the gradient may replace the logits).
-  int at[kEntries];
-  float s[kEntries];
-#pragma unroll
-  for (int i = 0; i < kEntries; ++i) {
-    at[i] = -1;
-    const int k = threadIdx.x + i * kBackThreads;
-    if (empty || k >= p.top) continue;
-    const int64_t index = index_at(p, row, k);
-    if (index < 0 || index >= p.vocab) continue;
-    const int e = static_cast<int>(index) + in.phase - in.first * kPer;
-    if (e < 0 || e >= in.count * kPer || !is_entry(index, teacher_at(p, row, k))) continue;
-    at[i] = static_cast<int>(index);
-    s[i] = to_float(logits[index]);
-  }
-  for (int i = threadIdx.x; i < static_cast<int>(sizeof(seen) / 4); i += kBackThreads) seen[i] = 0;
-  if (threadIdx.x == 0) shared_column = 0;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEntries; ++i) {
-    if (at[i] < 0) continue;
-    const uint32_t e = static_cast<uint32_t>(at[i] + in.phase - in.first * kPer);
-    if (atomicOr(&seen[e / 32], 1u << (e % 32)) >> (e % 32) & 1u) shared_column = 1;
-  }
-  const Pair scaled(a * stats.y);
-#pragma unroll
-  for (int u = 0; u < kBackGranules; ++u) {
-    const int w = static_cast<int>(threadIdx.x) + u * kBackThreads;
-    if (w >= in.count) continue;
-    Pair v[kPer / 2];
-    unpack_pairs<T>(raw[u], v);
-    float f[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) mul2(power(v[i], p.c), scaled).split(f[2 * i], f[2 * i + 1]);
-    in.store(grad, same_phase, w, empty ? make_uint4(0, 0, 0, 0) : pack_word<T>(f));
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEntries; ++i) {
-    if (at[i] < 0) continue;
-    const int k = threadIdx.x + i * kBackThreads;
-    float prob = exp2_fast((teacher_at(p, row, k) - stats.z) * p.c) * stats.w;
-    if (shared_column) {
+  for (int k = lane; k < count; k += 32) {
+    const BackEntry e = list[k];
+    float prob = e.p;
+    if (shared_column) {  // every entry of a column writes the same sum
       prob = 0.f;
-      for (int j = 0; j < p.top; ++j) {
-        if (index_at(p, row, j) != at[i]) continue;
-        const float t = teacher_at(p, row, j);
-        if (t != -INFINITY) prob += exp2_fast((t - stats.z) * p.c) * stats.w;
+      for (int j = 0; j < count; ++j) {
+        if (list[j].at == e.at) prob += list[j].p;
       }
     }
-    grad[at[i]] = from_float<T>(a * (power(s[i], p.c) * stats.y - prob));
+    grad[e.at] = from_float<T>(a * (Exponent(stats.x)(e.s, p.c) * stats.y - prob));
   }
 }
 
@@ -925,19 +945,19 @@ int hash_bits(int top) {
 }
 
 size_t shared_bytes(int64_t vocab, int dtype, int top, int cluster, bool grad) {
-  return static_cast<size_t>(top) * sizeof(Entry) +
+  return static_cast<size_t>(top) * sizeof(Entry) * (grad ? 2 : 1) +
          (grad ? (sizeof(int) << hash_bits(top)) + static_cast<size_t>(ceil_div(max_words(vocab, dtype), cluster)) * 16 : 0);
 }
 
-// Blocks per row: the gradient's slice should let four blocks share an SM
+// Blocks per row: the gradient's slice should let three blocks share an SM
 // (and must fit one); beyond that, few rows are split until the blocks fill
 // the SMs. 0: a row does not fit a cluster.
 int cluster_size(int64_t rows, int64_t vocab, int dtype, int top, bool grad) {
   int cluster = 1;
-  while (cluster < kMaxCluster && grad && shared_bytes(vocab, dtype, top, cluster, grad) > kSliceTarget) cluster *= 2;
+  while (cluster < kMaxCluster && grad && shared_bytes(vocab, dtype, top, cluster, grad) > kSliceTarget) ++cluster;
   if (shared_bytes(vocab, dtype, top, cluster, grad) > kSharedLimit - 2048) return 0;
   while (cluster < kMaxCluster && rows * cluster < 4 * sm_count() && max_words(vocab, dtype) / cluster > 2 * kRowThreads) {
-    cluster *= 2;
+    cluster = std::min(2 * cluster, kMaxCluster);
   }
   return cluster;
 }
@@ -997,12 +1017,13 @@ int run_rows(DistillParams p, int dtype, int64_t rows, int cluster, cudaStream_t
 }
 
 int run_backward(DistillParams p, int dtype, int64_t rows, cudaStream_t stream) {
-  p.chunks = static_cast<int>(ceil_div(max_words(p.vocab, dtype), kBackThreads * kBackGranules));
+  p.chunks = static_cast<int>(ceil_div(max_words(p.vocab, dtype), kBackThreads * kBackWords));
   SDC_REQUIRE(rows <= INT_MAX / p.chunks, "distillation has too many rows for one launch");
   const unsigned grid = static_cast<unsigned>(rows * p.chunks);
-  if (dtype == kF32) distill_backward<float><<<grid, kBackThreads, 0, stream>>>(p);
-  else if (dtype == kBF16) distill_backward<__nv_bfloat16><<<grid, kBackThreads, 0, stream>>>(p);
-  else distill_backward<__half><<<grid, kBackThreads, 0, stream>>>(p);
+  const size_t shared = static_cast<size_t>(p.top) * sizeof(BackEntry);
+  if (dtype == kF32) distill_backward<float><<<grid, kBackThreads + 32, shared, stream>>>(p);
+  else if (dtype == kBF16) distill_backward<__nv_bfloat16><<<grid, kBackThreads + 32, shared, stream>>>(p);
+  else distill_backward<__half><<<grid, kBackThreads + 32, shared, stream>>>(p);
   SDC_CUDA_CHECK(cudaGetLastError());
   return SDC_OK;
 }

@@ -534,6 +534,46 @@ def test_distillation_masks_and_values_that_are_not_finite():
     assert nothing == 0 and not torch.autograd.grad(nothing, empty)[0].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_finds_one_value_that_is_not_finite_anywhere(dtype):
+    """Wherever in a 16-byte word it is: NaN and inf make the row NaN, -inf and the lowest value are left out."""
+    vocab = 1003
+    logits, indices, teacher = _distill_inputs(64, vocab, 4, dtype)
+    indices[:] = torch.tensor([100, 200, 300, 400], device=DEV)
+    for i in range(16):
+        logits[i, 500 + i] = math.nan
+        logits[16 + i, 500 + i] = math.inf
+        logits[32 + i, 500 + i] = -math.inf
+        logits[48 + i, 500 + i] = torch.finfo(dtype).min
+    loss, grad = distillation_loss_and_grad(logits, indices, teacher)
+    leaf = logits.detach().requires_grad_()
+    losses = distillation_loss(leaf, indices, teacher, reduction="none")
+    (again,) = torch.autograd.grad(losses, leaf, torch.ones_like(losses))
+    loss64, size, grad64, q, p = distill64(logits[32:], indices[32:], teacher[32:], 1.0)
+    for one, slope in ((loss, grad), (losses.detach(), again)):
+        assert one[:32].isnan().all() and slope[:32].isnan().all()
+        close(one[32:], loss64, size, 2.0 ** -17)
+        close(slope[32:], grad64, q + p, 2.0 ** -17)
+    for i in range(32):
+        assert grad[32 + i, 500 + i % 16] == 0 and again[32 + i, 500 + i % 16] == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_of_rows_masked_throughout(dtype):
+    """All of the vocabulary at the type's lowest value is a uniform distribution."""
+    vocab = 5001
+    logits, indices, teacher = _distill_inputs(3, vocab, 4, dtype)
+    logits[0] = torch.finfo(dtype).min
+    logits[1] = torch.finfo(dtype).max
+    logits[2, ::2] = torch.finfo(dtype).min
+    loss64, size, grad64, q, p = distill64(logits, indices, teacher, 1.0)
+    loss, grad = distillation_loss_and_grad(logits, indices, teacher)
+    close(loss, loss64, size, 2.0 ** -17)
+    close(grad, grad64, q + p, 2.0 ** -17)
+    losses = distillation_loss(logits, indices, teacher, reduction="none")
+    close(losses, loss64, size, 2.0 ** -17)
+
+
 def test_distillation_shapes_types_and_no_rows():
     logits, indices, teacher = _distill_inputs(6, 500, 8, torch.bfloat16)
     flat = distillation_loss_and_grad(logits, indices, teacher)
