@@ -64,6 +64,8 @@ struct AdapterParams {
   int64_t out_stride;        // expand: row; outer: column
   int64_t out_rank_stride;   // outer
   int chunks_per_split;
+  int tile_count, tiles_per_block;  // expand
+  int piece_bits;            // expand: 2^piece_bits >= rank_pad / 8 threads copy a row
 };
 
 __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot) {
@@ -252,39 +254,51 @@ __host__ __device__ constexpr int expand_group_bytes(int rank_pad) { return 32 *
 __host__ __device__ constexpr int expand_weight_bytes(int columns, int rank_pad, bool trans) {
   return trans ? rank_pad * (columns + 8) * 2 : columns / 32 * expand_group_bytes(rank_pad);
 }
+// Two tiles' low rows, or one where two do not fit.
+__host__ __device__ constexpr int low_buffers(int rank_pad) { return rank_pad <= 128 ? 2 : 1; }
 __host__ __device__ constexpr int expand_bytes(int rows, int columns, int rank_pad, bool trans) {
-  return expand_weight_bytes(columns, rank_pad, trans) + 2 * rows * (rank_pad + 8) * 2;
+  return expand_weight_bytes(columns, rank_pad, trans) + low_buffers(rank_pad) * 2 * rows * (rank_pad + 8) * 2;
 }
 
-template <typename T, int ROWS, bool TRANS>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_expand(AdapterParams p) {
+// A block keeps 256 columns of one adapter's weight in shared memory and walks
+// a run of tiles: the next tile's low rows are copied and its part of base is
+// loaded into registers as soon as the current one's has been used, so loads
+// never stop. FAST: widths, strides and addresses allow 16-byte accesses to
+// base and out throughout.
+template <typename T, int ROWS, bool TRANS, bool FAST>
+__global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterParams p) {
   using S = ExpandShape<ROWS>;
   extern __shared__ __align__(16) uint8_t shared[];
-  const uint32_t column_blocks = static_cast<uint32_t>((p.width + S::kColumns - 1) / S::kColumns);
-  const Tile tile = p.tiles[blockIdx.x / column_blocks];
-  const int64_t column0 = static_cast<int64_t>(blockIdx.x % column_blocks) * S::kColumns;
+  const int width = static_cast<int>(p.width);
+  const int column_blocks = (width + S::kColumns - 1) / S::kColumns;
+  const int run = static_cast<int>(blockIdx.x) / column_blocks;
+  const int column0 = (static_cast<int>(blockIdx.x) - run * column_blocks) * S::kColumns;
+  const int first = run * p.tiles_per_block, last = min(first + p.tiles_per_block, p.tile_count);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool adapted = tile.adapter >= 0 && tile.adapter < p.adapters;
-  const int pitch = p.rank_pad + 8;
+  const int pitch = p.rank_pad + 8, pieces = p.rank_pad / 8;
   uint8_t* weight_shared = shared;
   T* low_shared = reinterpret_cast<T*>(shared + expand_weight_bytes(S::kColumns, p.rank_pad, TRANS));
+  const int low_elements = 2 * ROWS * pitch;  // of one tile
+  const bool two_buffers = low_buffers(p.rank_pad) == 2;
 
-  if (adapted) {
-    const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(tile.adapter) * p.rank * p.width;
+  auto load_weight = [&](int adapter) {
+    const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
     if constexpr (!TRANS) {
-      const int pieces = p.rank_pad / 8;
-      for (int i = tid; i < S::kColumns * pieces; i += kAdapterThreads) {
-        const int c = i / pieces, r = (i - c * pieces) * 8;
-        T* to = reinterpret_cast<T*>(weight_shared + (c >> 5) * expand_group_bytes(p.rank_pad) +
-                                     (c & 31) * pitch * 2 + ((c >> 3) & 3) * 32) + r;
-        copy8(to, weight + (column0 + c) * p.rank + r, column0 + c < p.width ? p.rank - r : 0, p.vector_weight);
+      const int piece = (tid & ((1 << p.piece_bits) - 1)), r = piece * 8;
+      if (piece < pieces) {
+        for (int c = tid >> p.piece_bits; c < S::kColumns; c += kAdapterThreads >> p.piece_bits) {
+          T* to = reinterpret_cast<T*>(weight_shared + (c >> 5) * expand_group_bytes(p.rank_pad) +
+                                       (c & 31) * pitch * 2 + ((c >> 3) & 3) * 32) + r;
+          copy8(to, weight + static_cast<int64_t>(column0 + c) * p.rank + r, column0 + c < width ? p.rank - r : 0,
+                p.vector_weight);
+        }
       }
     } else {
       constexpr int kPieces = S::kColumns / 8;
       for (int i = tid; i < p.rank_pad * kPieces; i += kAdapterThreads) {
         const int r = i / kPieces, c = i % kPieces * 8;
         const T* from = weight + r * p.width + column0 + c;
-        const int64_t left = r < p.rank ? p.width - (column0 + c) : 0;
+        const int left = r < p.rank ? width - (column0 + c) : 0;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (left >= 8 && p.vector_weight) {
           w = *reinterpret_cast<const uint4*>(from);
@@ -300,108 +314,147 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_expand(AdapterParams 
         to[0] = w.x, to[4] = w.y, to[8] = w.z, to[12] = w.w;
       }
     }
-  }
-
-  // This thread's part of base: rows lane / 4 and lane / 4 + 8, 8 columns of
-  // each group. Read before waiting for `low`.
-  const int row0 = (ROWS == 64 ? warp * 16 : 0) + (lane >> 2);
-  const int64_t column = column0 + (ROWS == 64 ? 0 : warp * 32) + (lane & 3) * 8;
-  int64_t token[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) token[h] = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
-  Raw8<T> base[S::kGroups][2];
-#pragma unroll
-  for (int g = 0; g < S::kGroups; ++g) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      base[g][h].w[0] = make_uint4(0, 0, 0, 0);
-      const int64_t left = p.width - (column + g * 32);
-      if (p.base == nullptr || token[h] < 0 || left <= 0) continue;
-      const T* from = static_cast<const T*>(p.base) + token[h] * p.base_stride + column + g * 32;
-      if (p.vector_rows && left >= 8) {
-        base[g][h] = load8(from);
-      } else {
-        T* e = reinterpret_cast<T*>(&base[g][h]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < left) e[j] = from[j];
-        }
-      }
-    }
-  }
-
-  griddep_wait();
-  if (adapted) {
-    const int pieces = p.rank_pad / 8;
-    const T* high = static_cast<const T*>(p.low);
-    for (int i = tid; i < 2 * ROWS * pieces; i += kAdapterThreads) {
-      const int plane = i >= ROWS * pieces;
-      const int row = (i - plane * ROWS * pieces) / pieces, r = i % pieces * 8;
-      T* to = low_shared + (plane * ROWS + row) * pitch + r;
+  };
+  auto load_low = [&](const Tile& tile, int buffer) {
+    T* to_tile = low_shared + buffer * low_elements;
+    const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * p.rank_pad;
+    const int piece = tid & ((1 << p.piece_bits) - 1), r = piece * 8;
+    if (piece >= pieces) return;
+    for (int i = tid >> p.piece_bits; i < 2 * ROWS; i += kAdapterThreads >> p.piece_bits) {
+      const int row = i % ROWS;
+      T* to = to_tile + i * pitch + r;
       if (row < tile.count) {
-        cp_async16(to, high + (plane * p.slots + tile.start + row) * p.rank_pad + r);
+        cp_async16(to, from + (i >= ROWS ? p.slots * p.rank_pad : 0) + row * p.rank_pad + r);
       } else {
         *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
       }
     }
-  }
-  cp_async_commit();
-  cp_async_wait<0>();
-  __syncthreads();
+  };
+  auto adapted = [&](const Tile& tile) { return tile.adapter >= 0 && tile.adapter < p.adapters; };
 
+  // This thread's part of base and out: rows lane / 4 and lane / 4 + 8 of its
+  // 16, 8 columns of each 32.
+  const int row0 = (ROWS == 64 ? warp * 16 : 0) + (lane >> 2);
+  const int column = column0 + (ROWS == 64 ? 0 : warp * 32) + (lane & 3) * 8;
+  auto look = [&](const Tile& tile, int64_t* token) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) token[h] = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
+  };
+  const T* base = static_cast<const T*>(p.base);
+  auto load_base = [&](int64_t token, int g) {
+    Raw8<T> r;
+    r.w[0] = make_uint4(0, 0, 0, 0);
+    const int left = width - (column + g * 32);
+    if (base == nullptr || token < 0 || left <= 0) return r;
+    const T* from = base + token * p.base_stride + column + g * 32;
+    if constexpr (FAST) {
+      r = load8(from);
+    } else {
+      T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < left) e[j] = from[j];
+      }
+    }
+    return r;
+  };
+
+  Tile tile = p.tiles[first];
+  int64_t token[2], next_token[2];
+  look(tile, token);
+  Raw8<T> part[S::kGroups][2];
 #pragma unroll
   for (int g = 0; g < S::kGroups; ++g) {
-    float acc[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    if (adapted) {
-      const int group = ROWS == 64 ? g : warp;
-      const T* rows = low_shared + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 8;
-      for (int k = 0; k < p.rank_pad; k += 16) {
-        uint32_t hi[4], lo[4];
-        ldmatrix_x4(hi, rows + k);
-        ldmatrix_x4(lo, rows + ROWS * pitch + k);
+    for (int h = 0; h < 2; ++h) part[g][h] = load_base(token[h], g);
+  }
+  int adapter = -1;  // whose weight is in shared memory
+  if (adapted(tile)) load_weight(adapter = tile.adapter);
+  griddep_wait();  // `low` from here on
+  if (adapted(tile)) load_low(tile, 0);
+  cp_async_commit();
+  Tile next = first + 1 < last ? p.tiles[first + 1] : Tile{0, 0, -1};
+  for (int t = first; t < last; ++t) {
+    const int buffer = two_buffers ? (t - first) & 1 : 0;
+    const bool more = t + 1 < last;
+    const Tile after = t + 2 < last ? p.tiles[t + 2] : Tile{0, 0, -1};
+    if (more) look(next, next_token);
+    if (two_buffers && more && adapted(next)) load_low(next, buffer ^ 1);
+    cp_async_commit();
+    if (adapted(tile) && tile.adapter != adapter) {
+      __syncthreads();  // the last tile's products are done with the old weight
+      load_weight(adapter = tile.adapter);
+      cp_async_commit();
+      cp_async_wait<0>();
+    } else {
+      cp_async_wait<1>();
+    }
+    __syncthreads();
+    const T* low = low_shared + buffer * low_elements + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 8;
 #pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
-          uint32_t b[4];
-          if constexpr (!TRANS) {
-            const int i = lane & 7, j = 2 * pair + (lane >> 4);
-            const int c = (i >> 1) * 8 + j * 2 + (i & 1);
-            ldmatrix_x4(b, reinterpret_cast<const T*>(weight_shared + group * expand_group_bytes(p.rank_pad) +
-                                                      c * pitch * 2 + (c >> 3) * 32) + k + ((lane >> 3) & 1) * 8);
-          } else {
-            ldmatrix_x4_trans(b, reinterpret_cast<const T*>(weight_shared) +
-                                     (k + ((lane >> 3) & 1) * 8 + (lane & 7)) * (S::kColumns + 8) + group * 32 +
-                                     pair * 16 + (lane >> 4) * 8);
+    for (int g = 0; g < S::kGroups; ++g) {
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      if (adapted(tile)) {
+        const int group = ROWS == 64 ? g : warp;
+        for (int k = 0; k < p.rank_pad; k += 16) {
+          uint32_t hi[4], lo[4];
+          ldmatrix_x4(hi, low + k);
+          ldmatrix_x4(lo, low + ROWS * pitch + k);
+#pragma unroll
+          for (int pair = 0; pair < 2; ++pair) {
+            uint32_t b[4];
+            if constexpr (!TRANS) {
+              const int i = lane & 7, j = 2 * pair + (lane >> 4);
+              const int c = (i >> 1) * 8 + j * 2 + (i & 1);
+              ldmatrix_x4(b, reinterpret_cast<const T*>(weight_shared + group * expand_group_bytes(p.rank_pad) +
+                                                        c * pitch * 2 + (c >> 3) * 32) + k + ((lane >> 3) & 1) * 8);
+            } else {
+              ldmatrix_x4_trans(b, reinterpret_cast<const T*>(weight_shared) +
+                                       (k + ((lane >> 3) & 1) * 8 + (lane & 7)) * (S::kColumns + 8) + group * 32 +
+                                       pair * 16 + (lane >> 4) * 8);
+            }
+            mma_16816<T>(acc[2 * pair], hi, b);
+            mma_16816<T>(acc[2 * pair + 1], hi, b + 2);
+            mma_16816<T>(acc[2 * pair], lo, b);
+            mma_16816<T>(acc[2 * pair + 1], lo, b + 2);
           }
-          mma_16816<T>(acc[2 * pair], hi, b);
-          mma_16816<T>(acc[2 * pair], lo, b);
-          mma_16816<T>(acc[2 * pair + 1], hi, b + 2);
-          mma_16816<T>(acc[2 * pair + 1], lo, b + 2);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        unpack8(part[g][h], v);
+        if (more) part[g][h] = load_base(next_token[h], g);
+        const int left = width - (column + g * 32);
+        if (token[h] < 0 || left <= 0) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] += acc[j][2 * h];
+          v[2 * j + 1] += acc[j][2 * h + 1];
+        }
+        T* to = static_cast<T*>(p.out) + token[h] * p.out_stride + column + g * 32;
+        if constexpr (FAST) {
+          store8(to, pack8<T>(v));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j < left) to[j] = from_float<T>(v[j]);
+          }
         }
       }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t left = p.width - (column + g * 32);
-      if (token[h] < 0 || left <= 0) continue;
-      float v[8];
-      unpack8(base[g][h], v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] += acc[j][2 * h];
-        v[2 * j + 1] += acc[j][2 * h + 1];
-      }
-      T* to = static_cast<T*>(p.out) + token[h] * p.out_stride + column + g * 32;
-      if (p.vector_out && left >= 8) {
-        store8(to, pack8<T>(v));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < left) to[j] = from_float<T>(v[j]);
-        }
-      }
+    if (!two_buffers) {
+      __syncthreads();
+      if (more && adapted(next)) load_low(next, 0);
+      cp_async_commit();
+      cp_async_wait<0>();
     }
+    tile = next;
+    next = after;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) token[h] = next_token[h];
   }
 }
 
@@ -415,6 +468,7 @@ struct OuterShape {
   static constexpr int kColumns = 128;
   static constexpr int kTokens = 32;
   static constexpr int kStages = 4;
+  static constexpr int kLook = 2 * kStages;  // token lists in flight
   static constexpr int kRowPitch = kColumns + 8;
   static constexpr int kLowPitch = RANK + 8;
   static constexpr int kStageElements = kTokens * (kRowPitch + 2 * kLowPitch);
@@ -427,6 +481,7 @@ template <typename T, int RANK>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p) {
   using S = OuterShape<RANK>;
   extern __shared__ __align__(16) uint8_t shared[];
+  __shared__ int32_t tokens[S::kLook][S::kTokens];
   T* stages = reinterpret_cast<T*>(shared);
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
@@ -449,14 +504,12 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
   const int64_t columns_left = p.width - (column0 + piece * 8);
   const T* low = static_cast<const T*>(p.low);
 
-  // Tokens of the next tile to load, read one tile ahead.
-  int32_t tokens[kPasses];
+  // The tokens of a tile are copied kStages - 1 tiles before its rows.
   auto look = [&](int tile) {
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + tid / kPieces + i * kRowStep;
-      tokens[i] = tile < last && slot < end ? static_cast<int32_t>(token_of(p, slot)) : -1;
-    }
+    const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + tid;
+    if (tid >= S::kTokens || tile >= last) return;
+    if (slot < end) cp_async4(&tokens[tile % S::kLook][tid], p.rows + slot);
+    else tokens[tile % S::kLook][tid] = -1;
   };
   auto load = [&](int tile) {
     T* rows = stages + ((tile - first) % S::kStages) * S::kStageElements;
@@ -464,18 +517,18 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int row = tid / kPieces + i * kRowStep;
-      copy8(rows + row * S::kRowPitch + piece * 8, x + static_cast<int64_t>(tokens[i]) * p.row_stride,
-            tokens[i] >= 0 ? columns_left : 0, p.vector_rows);
+      const int64_t token = tokens[tile % S::kLook][row];
+      copy8(rows + row * S::kRowPitch + piece * 8, x + token * p.row_stride,
+            token >= 0 && token < p.tokens ? columns_left : 0, p.vector_rows);
     }
+    const int64_t slot0 = begin + static_cast<int64_t>(tile) * S::kTokens;
     for (int i = tid; i < 2 * S::kTokens * (RANK / 8); i += kAdapterThreads) {
       const int plane = i / (S::kTokens * (RANK / 8));
       const int row = i / (RANK / 8) % S::kTokens, r = i % (RANK / 8) * 8;
-      const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + row;
-      const bool in = slot < end && rank0 + r < p.rank_pad;
+      const bool in = slot0 + row < end && rank0 + r < p.rank_pad;
       copy8(lows + (plane * S::kTokens + row) * S::kLowPitch + r,
-            low + (plane * p.slots + slot) * p.rank_pad + rank0 + r, in ? 8 : 0, true);
+            low + (plane * p.slots + slot0 + row) * p.rank_pad + rank0 + r, in ? 8 : 0, true);
     }
-    look(tile + 1);
   };
 
   float acc[2][RANK / 8][4];
@@ -484,7 +537,11 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
 #pragma unroll
     for (int i = 0; i < RANK / 8; ++i) acc[m][i][0] = acc[m][i][1] = acc[m][i][2] = acc[m][i][3] = 0.f;
   }
-  look(first);
+#pragma unroll
+  for (int i = 0; i < 2 * (S::kStages - 1); ++i) look(first + i);
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
     if (first + i < last) load(first + i);
@@ -494,6 +551,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
     cp_async_wait<S::kStages - 2>();
     __syncthreads();
     if (tile + S::kStages - 1 < last) load(tile + S::kStages - 1);
+    look(tile + 2 * (S::kStages - 1));
     cp_async_commit();
     const T* rows = stages + ((tile - first) % S::kStages) * S::kStageElements;
     const T* lows = rows + S::kTokens * S::kRowPitch;
@@ -634,12 +692,23 @@ int shrink_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tile
 }
 
 template <typename T, int ROWS, bool TRANS>
-int launch_expand(const AdapterParams& p, int64_t tiles, bool dependent, cudaStream_t stream) {
+int launch_expand(AdapterParams p, int64_t tiles, bool dependent, cudaStream_t stream) {
   constexpr int kColumns = ExpandShape<ROWS>::kColumns;
-  const int64_t blocks = ceil_div(p.width, kColumns) * tiles;
+  const int64_t column_blocks = ceil_div(p.width, kColumns);
+  // Runs of tiles that fill the SMs' four blocks each once; tiles of few rows
+  // are bound by the weight, of which each then wants its own.
+  p.tile_count = static_cast<int>(tiles);
+  const int64_t runs = std::max<int64_t>(1, 4 * sm_count() / column_blocks);
+  p.tiles_per_block = ROWS == 64 ? static_cast<int>(ceil_div(tiles, runs)) : 1;
+  const int64_t blocks = column_blocks * ceil_div(tiles, p.tiles_per_block);
   SDC_REQUIRE(blocks <= INT_MAX, "low-rank adapters have too many tiles for one launch");
-  return launch_clustered(adapter_expand<T, ROWS, TRANS>, p, dim3(static_cast<unsigned>(blocks)), 0,
-                          expand_bytes(ROWS, kColumns, p.rank_pad, TRANS), dependent, stream);
+  while ((8 << p.piece_bits) < p.rank_pad) ++p.piece_bits;
+  const int shared = expand_bytes(ROWS, kColumns, p.rank_pad, TRANS);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (p.vector_rows && p.vector_out && p.width % 8 == 0) {
+    return launch_clustered(adapter_expand<T, ROWS, TRANS, true>, p, grid, 0, shared, dependent, stream);
+  }
+  return launch_clustered(adapter_expand<T, ROWS, TRANS, false>, p, grid, 0, shared, dependent, stream);
 }
 
 template <typename T>

@@ -46,6 +46,9 @@ __device__ __forceinline__ void mma_16816<__half>(float* d, const uint32_t* a, c
 __device__ __forceinline__ void cp_async16(void* shared, const void* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
 }
+__device__ __forceinline__ void cp_async4(void* shared, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
