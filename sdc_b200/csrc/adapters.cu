@@ -81,21 +81,20 @@ template <int ROWS, int RANK, bool TRANS>
 struct ShrinkShape {
   static constexpr int kChunk = ROWS == 64 ? 64 : 256;
   static constexpr int kStages = 4;
-  static constexpr int kRowPitch = kChunk + 8;
+  static constexpr int kRowBytes = (kChunk + 8) * 2;  // 8 elements of padding: fragment rows on different banks
   static constexpr int kWeightRows = TRANS ? kChunk : RANK;
-  static constexpr int kWeightCols = TRANS ? RANK : kChunk;
-  static constexpr int kWeightPitch = kWeightCols + 8;
-  static constexpr int kStageElements = ROWS * kRowPitch + kWeightRows * kWeightPitch;
+  static constexpr int kWeightBytes = ((TRANS ? RANK : kChunk) + 8) * 2;
+  static constexpr int kStageBytes = ROWS * kRowBytes + kWeightRows * kWeightBytes;
   static constexpr int kPartRows = ROWS == 64 ? 64 : 4 * 16;
   static constexpr int kPartBytes = kPartRows * RANK * 4;
-  static constexpr int kBytes = kStages * kStageElements * 2 > kPartBytes ? kStages * kStageElements * 2 : kPartBytes;
+  static constexpr int kBytes = kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes;
 };
 
-template <typename T, int ROWS, int RANK, bool TRANS>
+template <typename T, int ROWS, int RANK, bool TRANS, bool FAST>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams p) {
   using S = ShrinkShape<ROWS, RANK, TRANS>;
   extern __shared__ __align__(16) uint8_t shared[];
-  T* stages = reinterpret_cast<T*>(shared);
+  const uint32_t stages = smem_u32(shared);
   griddep_launch_dependents();
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
@@ -105,54 +104,49 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool valid = tile.adapter >= 0 && tile.adapter < p.adapters;
   const int count = valid ? tile.count : 0;
-  const T* x = static_cast<const T*>(p.rows_in);
-  const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(valid ? tile.adapter : 0) * p.rank * p.width;
-
-  const int chunks = static_cast<int>((p.width + S::kChunk - 1) / S::kChunk);
+  const int width = static_cast<int>(p.width);
+  const int chunks = (width + S::kChunk - 1) / S::kChunk;
   const int first = min(static_cast<int>(split) * p.chunks_per_split, chunks);
   const int last = min(first + p.chunks_per_split, chunks);
 
-  // Rows beyond the tile and ranks beyond the adapter stay zero throughout.
-  for (int i = tid; i < S::kStages * S::kStageElements / 8; i += kAdapterThreads) {
-    reinterpret_cast<uint4*>(shared)[i] = make_uint4(0, 0, 0, 0);
-  }
-  constexpr int kPieces = S::kChunk / 8;            // 16-byte pieces of a row
-  constexpr int kRowStep = kAdapterThreads / kPieces;
-  constexpr int kPasses = ROWS / kRowStep;
-  const int piece = tid % kPieces;
-  const T* source[kPasses];
+  // What this thread copies of a chunk: pieces of 8 elements of the rows, and
+  // of the weight [rank, width], or [width, rank] when TRANS.
+  constexpr int kPieces = S::kChunk / 8;
+  constexpr int kRowStep = kAdapterThreads / kPieces, kRowCopies = ROWS / kRowStep;
+  constexpr int kWeightPieces = TRANS ? RANK / 8 : kPieces;
+  constexpr int kWeightStep = kAdapterThreads / kWeightPieces, kWeightCopies = S::kWeightRows / kWeightStep;
+  const int piece = tid % kPieces, row_of = tid / kPieces;
+  const int weight_piece = tid % kWeightPieces, weight_row = tid / kWeightPieces;
+  const T* source[kRowCopies];
+  uint32_t present = 0;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int row = tid / kPieces + i * kRowStep;
+  for (int i = 0; i < kRowCopies; ++i) {
+    const int row = row_of + i * kRowStep;
     const int64_t token = row < count ? token_of(p, tile.start + row) : -1;
-    source[i] = token >= 0 ? x + token * p.row_stride + piece * 8 : nullptr;
+    if (token >= 0) present |= 1u << i;
+    source[i] = static_cast<const T*>(p.rows_in) + (token >= 0 ? token * p.row_stride : 0) + piece * 8;
   }
-  __syncthreads();
+  const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(valid ? tile.adapter : 0) * p.rank * p.width;
+  weight += TRANS ? static_cast<int64_t>(weight_row) * p.rank + rank0 + weight_piece * 8
+                  : static_cast<int64_t>(rank0 + weight_row) * width + weight_piece * 8;
+  const uint32_t row_to = stages + row_of * S::kRowBytes + piece * 16;
+  const uint32_t weight_to = stages + ROWS * S::kRowBytes + weight_row * S::kWeightBytes + weight_piece * 16;
 
   auto load = [&](int chunk) {
-    T* rows = stages + ((chunk - first) % S::kStages) * S::kStageElements;
-    T* w = rows + ROWS * S::kRowPitch;
-    const int64_t k0 = static_cast<int64_t>(chunk) * S::kChunk;
+    const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
+    const int k0 = chunk * S::kChunk, left = width - k0 - piece * 8;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (source[i] == nullptr) continue;
-      const int row = tid / kPieces + i * kRowStep;
-      copy8(rows + row * S::kRowPitch + piece * 8, source[i] + k0, p.width - (k0 + piece * 8), p.vector_rows);
+    for (int i = 0; i < kRowCopies; ++i) {
+      copy8<T, FAST>(row_to + stage + i * kRowStep * S::kRowBytes, left > 0 ? source[i] + k0 : source[i],
+                     (present >> i & 1) ? left : 0);
     }
-    if constexpr (!TRANS) {  // weight [rank, width]
-      for (int i = tid; i < RANK * kPieces; i += kAdapterThreads) {
-        const int r = i / kPieces, c = i % kPieces * 8;
-        if (rank0 + r < p.rank) {
-          copy8(w + r * S::kWeightPitch + c, weight + (rank0 + r) * p.width + k0 + c, p.width - (k0 + c),
-                p.vector_weight);
-        }
-      }
-    } else {  // weight [width, rank]
-      for (int i = tid; i < S::kChunk * (RANK / 8); i += kAdapterThreads) {
-        const int k = i / (RANK / 8), c = i % (RANK / 8) * 8;
-        copy8(w + k * S::kWeightPitch + c, weight + (k0 + k) * p.rank + rank0 + c,
-              k0 + k < p.width ? p.rank - (rank0 + c) : 0, p.vector_weight);
-      }
+#pragma unroll
+    for (int i = 0; i < kWeightCopies; ++i) {
+      const int at = weight_row + i * kWeightStep;
+      const int in = TRANS ? (k0 + at < width ? p.rank - (rank0 + weight_piece * 8) : 0) : (rank0 + at < p.rank ? left : 0);
+      const T* from = weight + (TRANS ? static_cast<int64_t>(k0 + i * kWeightStep) * p.rank
+                                      : static_cast<int64_t>(i * kWeightStep) * width + k0);
+      copy8<T, FAST>(weight_to + stage + i * kWeightStep * S::kWeightBytes, in > 0 ? from : static_cast<const T*>(p.weight), in);
     }
   };
 
@@ -164,28 +158,28 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
     if (first + i < last) load(first + i);
     cp_async_commit();
   }
-  const int row0 = ROWS == 64 ? warp * 16 : 0;
+  const int k_of = ROWS == 64 ? 0 : warp * (S::kChunk / 4);
+  const uint32_t a_from = stages + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * S::kRowBytes + (k_of + (lane >> 4) * 8) * 2;
+  const uint32_t b_from =
+      stages + ROWS * S::kRowBytes +
+      (TRANS ? (k_of + ((lane >> 3) & 1) * 8 + (lane & 7)) * S::kWeightBytes + (lane >> 4) * 16
+             : ((lane >> 4) * 8 + (lane & 7)) * S::kWeightBytes + (k_of + ((lane >> 3) & 1) * 8) * 2);
   for (int chunk = first; chunk < last; ++chunk) {
     cp_async_wait<S::kStages - 2>();
     __syncthreads();
     if (chunk + S::kStages - 1 < last) load(chunk + S::kStages - 1);
     cp_async_commit();
-    const T* rows = stages + ((chunk - first) % S::kStages) * S::kStageElements;
-    const T* w = rows + ROWS * S::kRowPitch;
+    const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
     constexpr int kSteps = ROWS == 64 ? S::kChunk / 16 : S::kChunk / 64;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const int k = (ROWS == 64 ? 0 : warp * (S::kChunk / 4)) + step * 16;
       uint32_t a[4];
-      ldmatrix_x4(a, rows + (row0 + (lane & 15)) * S::kRowPitch + k + (lane >> 4) * 8);
+      ldmatrix_x4(a, a_from + stage + step * 32);
 #pragma unroll
       for (int n = 0; n < RANK / 16; ++n) {
         uint32_t b[4];
-        if constexpr (!TRANS) {
-          ldmatrix_x4(b, w + (n * 16 + (lane >> 4) * 8 + (lane & 7)) * S::kWeightPitch + k + ((lane >> 3) & 1) * 8);
-        } else {
-          ldmatrix_x4_trans(b, w + (k + ((lane >> 3) & 1) * 8 + (lane & 7)) * S::kWeightPitch + n * 16 + (lane >> 4) * 8);
-        }
+        if constexpr (!TRANS) ldmatrix_x4(b, b_from + stage + n * 16 * S::kWeightBytes + step * 32);
+        else ldmatrix_x4_trans(b, b_from + stage + step * 16 * S::kWeightBytes + n * 32);
         mma_16816<T>(acc[2 * n], a, b);
         mma_16816<T>(acc[2 * n + 1], a, b + 2);
       }
@@ -263,45 +257,48 @@ __host__ __device__ constexpr int expand_bytes(int rows, int columns, int rank_p
 // A block keeps 256 columns of one adapter's weight in shared memory and walks
 // a run of tiles: the next tile's low rows are copied and its part of base is
 // loaded into registers as soon as the current one's has been used, so loads
-// never stop. FAST: widths, strides and addresses allow 16-byte accesses to
-// base and out throughout.
-template <typename T, int ROWS, bool TRANS, bool FAST>
+// never stop. FAST: widths, strides and addresses allow 16-byte accesses
+// throughout. PAD: rank_pad, or 0 where it is read from the parameters.
+template <typename T, int ROWS, bool TRANS, bool FAST, int PAD>
 __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterParams p) {
   using S = ExpandShape<ROWS>;
   extern __shared__ __align__(16) uint8_t shared[];
+  const int pad = PAD > 0 ? PAD : p.rank_pad;
   const int width = static_cast<int>(p.width);
   const int column_blocks = (width + S::kColumns - 1) / S::kColumns;
   const int run = static_cast<int>(blockIdx.x) / column_blocks;
   const int column0 = (static_cast<int>(blockIdx.x) - run * column_blocks) * S::kColumns;
   const int first = run * p.tiles_per_block, last = min(first + p.tiles_per_block, p.tile_count);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int pitch = p.rank_pad + 8, pieces = p.rank_pad / 8;
-  uint8_t* weight_shared = shared;
-  T* low_shared = reinterpret_cast<T*>(shared + expand_weight_bytes(S::kColumns, p.rank_pad, TRANS));
-  const int low_elements = 2 * ROWS * pitch;  // of one tile
-  const bool two_buffers = low_buffers(p.rank_pad) == 2;
+  const int pitch = (pad + 8) * 2;  // bytes of a low row, and of a weight row when !TRANS
+  const int group_bytes = expand_group_bytes(pad);
+  constexpr int kTransPitch = (S::kColumns + 8) * 2;
+  const uint32_t weight_shared = smem_u32(shared);
+  const uint32_t low_shared = weight_shared + expand_weight_bytes(S::kColumns, pad, TRANS);
+  const uint32_t low_bytes = 2 * ROWS * pitch;  // of one tile
+  const bool two_buffers = low_buffers(pad) == 2;
+  const int piece_bits = PAD > 0 ? (PAD <= 16 ? 1 : PAD <= 32 ? 2 : 3) : p.piece_bits;
+  const int piece = tid & ((1 << piece_bits) - 1), piece_row = tid >> piece_bits;
+  const int piece_step = kAdapterThreads >> piece_bits;
 
   auto load_weight = [&](int adapter) {
     const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
     if constexpr (!TRANS) {
-      const int piece = (tid & ((1 << p.piece_bits) - 1)), r = piece * 8;
-      if (piece < pieces) {
-        for (int c = tid >> p.piece_bits; c < S::kColumns; c += kAdapterThreads >> p.piece_bits) {
-          T* to = reinterpret_cast<T*>(weight_shared + (c >> 5) * expand_group_bytes(p.rank_pad) +
-                                       (c & 31) * pitch * 2 + ((c >> 3) & 3) * 32) + r;
-          copy8(to, weight + static_cast<int64_t>(column0 + c) * p.rank + r, column0 + c < width ? p.rank - r : 0,
-                p.vector_weight);
-        }
+      if (piece * 8 >= pad) return;
+      for (int c = piece_row; c < S::kColumns; c += piece_step) {
+        const uint32_t to = weight_shared + (c >> 5) * group_bytes + (c & 31) * pitch + ((c >> 3) & 3) * 32 + piece * 16;
+        const int in = column0 + c < width ? p.rank - piece * 8 : 0;
+        copy8<T, FAST>(to, in > 0 ? weight + static_cast<int64_t>(column0 + c) * p.rank + piece * 8 : weight, in);
       }
     } else {
       constexpr int kPieces = S::kColumns / 8;
-      for (int i = tid; i < p.rank_pad * kPieces; i += kAdapterThreads) {
+      for (int i = tid; i < pad * kPieces; i += kAdapterThreads) {
         const int r = i / kPieces, c = i % kPieces * 8;
         const T* from = weight + r * p.width + column0 + c;
         const int left = r < p.rank ? width - (column0 + c) : 0;
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (left >= 8 && p.vector_weight) {
-          w = *reinterpret_cast<const uint4*>(from);
+        if constexpr (FAST) {
+          if (left > 0) w = *reinterpret_cast<const uint4*>(from);
         } else {
           T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
@@ -309,25 +306,22 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
             if (j < left) e[j] = from[j];
           }
         }
-        uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(weight_shared) +
-                                                   r * (S::kColumns + 8) + (c & ~31) + ((c >> 3) & 3) * 2);
-        to[0] = w.x, to[4] = w.y, to[8] = w.z, to[12] = w.w;
+        const uint32_t to = weight_shared + r * kTransPitch + (c & ~31) * 2 + ((c >> 3) & 3) * 4;
+        asm volatile("st.shared.b32 [%0], %1;\n\tst.shared.b32 [%0 + 16], %2;\n\t"
+                     "st.shared.b32 [%0 + 32], %3;\n\tst.shared.b32 [%0 + 48], %4;" ::"r"(to), "r"(w.x), "r"(w.y),
+                     "r"(w.z), "r"(w.w)
+                     : "memory");
       }
     }
   };
   auto load_low = [&](const Tile& tile, int buffer) {
-    T* to_tile = low_shared + buffer * low_elements;
-    const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * p.rank_pad;
-    const int piece = tid & ((1 << p.piece_bits) - 1), r = piece * 8;
-    if (piece >= pieces) return;
-    for (int i = tid >> p.piece_bits; i < 2 * ROWS; i += kAdapterThreads >> p.piece_bits) {
+    if (piece * 8 >= pad) return;
+    const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * pad + piece * 8;
+    const uint32_t to = low_shared + buffer * low_bytes + piece * 16;
+    for (int i = piece_row; i < 2 * ROWS; i += piece_step) {
       const int row = i % ROWS;
-      T* to = to_tile + i * pitch + r;
-      if (row < tile.count) {
-        cp_async16(to, from + (i >= ROWS ? p.slots * p.rank_pad : 0) + row * p.rank_pad + r);
-      } else {
-        *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
-      }
+      const bool in = row < tile.count;
+      cp_async16(to + i * pitch, in ? from + (i >= ROWS ? p.slots * pad : 0) + row * pad : from, in);
     }
   };
   auto adapted = [&](const Tile& tile) { return tile.adapter >= 0 && tile.adapter < p.adapters; };
@@ -336,37 +330,44 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
   // 16, 8 columns of each 32.
   const int row0 = (ROWS == 64 ? warp * 16 : 0) + (lane >> 2);
   const int column = column0 + (ROWS == 64 ? 0 : warp * 32) + (lane & 3) * 8;
-  auto look = [&](const Tile& tile, int64_t* token) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) token[h] = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
+  const int columns_left = width - column;  // column + 32 g + j lies in the matrix when 32 g + j is less
+  struct Rows {
+    const T* base[2];  // null: no base or no row
+    T* out[2];         // null: no row
   };
-  const T* base = static_cast<const T*>(p.base);
-  auto load_base = [&](int64_t token, int g) {
+  auto look = [&](const Tile& tile) {
+    Rows r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t token = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
+      r.base[h] = token >= 0 && p.base != nullptr ? static_cast<const T*>(p.base) + token * p.base_stride + column : nullptr;
+      r.out[h] = token >= 0 ? static_cast<T*>(p.out) + token * p.out_stride + column : nullptr;
+    }
+    return r;
+  };
+  auto load_base = [&](const T* from, int g) {
     Raw8<T> r;
     r.w[0] = make_uint4(0, 0, 0, 0);
-    const int left = width - (column + g * 32);
-    if (base == nullptr || token < 0 || left <= 0) return r;
-    const T* from = base + token * p.base_stride + column + g * 32;
+    if (from == nullptr) return r;
     if constexpr (FAST) {
-      r = load8(from);
+      if (32 * g < columns_left) r = load8(from + 32 * g);
     } else {
       T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (j < left) e[j] = from[j];
+        if (32 * g + j < columns_left) e[j] = from[32 * g + j];
       }
     }
     return r;
   };
 
   Tile tile = p.tiles[first];
-  int64_t token[2], next_token[2];
-  look(tile, token);
+  Rows rows = look(tile), next_rows{};
   Raw8<T> part[S::kGroups][2];
 #pragma unroll
   for (int g = 0; g < S::kGroups; ++g) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) part[g][h] = load_base(token[h], g);
+    for (int h = 0; h < 2; ++h) part[g][h] = load_base(rows.base[h], g);
   }
   int adapter = -1;  // whose weight is in shared memory
   if (adapted(tile)) load_weight(adapter = tile.adapter);
@@ -374,11 +375,21 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
   if (adapted(tile)) load_low(tile, 0);
   cp_async_commit();
   Tile next = first + 1 < last ? p.tiles[first + 1] : Tile{0, 0, -1};
+  // Fragment addresses: low rows, and the weight's columns in the order above.
+  const uint32_t low_from = low_shared + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 16;
+  uint32_t weight_from[2];
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    const int i = lane & 7, j = 2 * pair + (lane >> 4), c = (i >> 1) * 8 + j * 2 + (i & 1);
+    weight_from[pair] = weight_shared + (TRANS ? (((lane >> 3) & 1) * 8 + i) * kTransPitch + pair * 32 + (lane >> 4) * 16
+                                               : c * pitch + (c >> 3) * 32 + ((lane >> 3) & 1) * 16);
+    if (ROWS == 16) weight_from[pair] += warp * (TRANS ? 64 : group_bytes);
+  }
   for (int t = first; t < last; ++t) {
     const int buffer = two_buffers ? (t - first) & 1 : 0;
     const bool more = t + 1 < last;
     const Tile after = t + 2 < last ? p.tiles[t + 2] : Tile{0, 0, -1};
-    if (more) look(next, next_token);
+    if (more) next_rows = look(next);
     if (two_buffers && more && adapted(next)) load_low(next, buffer ^ 1);
     cp_async_commit();
     if (adapted(tile) && tile.adapter != adapter) {
@@ -390,57 +401,54 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
       cp_async_wait<1>();
     }
     __syncthreads();
-    const T* low = low_shared + buffer * low_elements + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 8;
+    const uint32_t low = low_from + buffer * low_bytes;
+    const bool mine = adapted(tile);
 #pragma unroll
     for (int g = 0; g < S::kGroups; ++g) {
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-      if (adapted(tile)) {
-        const int group = ROWS == 64 ? g : warp;
-        for (int k = 0; k < p.rank_pad; k += 16) {
+      if (mine) {
+        auto step = [&](int k) {
           uint32_t hi[4], lo[4];
-          ldmatrix_x4(hi, low + k);
-          ldmatrix_x4(lo, low + ROWS * pitch + k);
+          ldmatrix_x4(hi, low + k * 2);
+          ldmatrix_x4(lo, low + ROWS * pitch + k * 2);
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
             uint32_t b[4];
-            if constexpr (!TRANS) {
-              const int i = lane & 7, j = 2 * pair + (lane >> 4);
-              const int c = (i >> 1) * 8 + j * 2 + (i & 1);
-              ldmatrix_x4(b, reinterpret_cast<const T*>(weight_shared + group * expand_group_bytes(p.rank_pad) +
-                                                        c * pitch * 2 + (c >> 3) * 32) + k + ((lane >> 3) & 1) * 8);
-            } else {
-              ldmatrix_x4_trans(b, reinterpret_cast<const T*>(weight_shared) +
-                                       (k + ((lane >> 3) & 1) * 8 + (lane & 7)) * (S::kColumns + 8) + group * 32 +
-                                       pair * 16 + (lane >> 4) * 8);
-            }
+            if constexpr (!TRANS) ldmatrix_x4(b, weight_from[pair] + g * group_bytes + k * 2);
+            else ldmatrix_x4_trans(b, weight_from[pair] + g * 64 + k * kTransPitch);
             mma_16816<T>(acc[2 * pair], hi, b);
             mma_16816<T>(acc[2 * pair + 1], hi, b + 2);
             mma_16816<T>(acc[2 * pair], lo, b);
             mma_16816<T>(acc[2 * pair + 1], lo, b + 2);
           }
+        };
+        if constexpr (PAD > 0) {
+#pragma unroll
+          for (int k = 0; k < PAD; k += 16) step(k);
+        } else {
+          for (int k = 0; k < pad; k += 16) step(k);
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
         unpack8(part[g][h], v);
-        if (more) part[g][h] = load_base(next_token[h], g);
-        const int left = width - (column + g * 32);
-        if (token[h] < 0 || left <= 0) continue;
+        if (more) part[g][h] = load_base(next_rows.base[h], g);
+        if (rows.out[h] == nullptr || 32 * g >= columns_left) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[2 * j] += acc[j][2 * h];
           v[2 * j + 1] += acc[j][2 * h + 1];
         }
-        T* to = static_cast<T*>(p.out) + token[h] * p.out_stride + column + g * 32;
+        T* to = rows.out[h] + 32 * g;
         if constexpr (FAST) {
           store8(to, pack8<T>(v));
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (j < left) to[j] = from_float<T>(v[j]);
+            if (32 * g + j < columns_left) to[j] = from_float<T>(v[j]);
           }
         }
       }
@@ -453,8 +461,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
     }
     tile = next;
     next = after;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) token[h] = next_token[h];
+    rows = next_rows;
   }
 }
 
@@ -469,20 +476,20 @@ struct OuterShape {
   static constexpr int kTokens = 32;
   static constexpr int kStages = 4;
   static constexpr int kLook = 2 * kStages;  // token lists in flight
-  static constexpr int kRowPitch = kColumns + 8;
-  static constexpr int kLowPitch = RANK + 8;
-  static constexpr int kStageElements = kTokens * (kRowPitch + 2 * kLowPitch);
+  static constexpr int kRowBytes = (kColumns + 8) * 2;
+  static constexpr int kLowBytes = (RANK + 8) * 2;
+  static constexpr int kStageBytes = kTokens * (kRowBytes + 2 * kLowBytes);
   static constexpr int kPartPitch = RANK + 1;
   static constexpr int kPartBytes = kColumns * kPartPitch * 4;
-  static constexpr int kBytes = kStages * kStageElements * 2 > kPartBytes ? kStages * kStageElements * 2 : kPartBytes;
+  static constexpr int kBytes = kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes;
 };
 
-template <typename T, int RANK>
+template <typename T, int RANK, bool FAST>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p) {
   using S = OuterShape<RANK>;
   extern __shared__ __align__(16) uint8_t shared[];
   __shared__ int32_t tokens[S::kLook][S::kTokens];
-  T* stages = reinterpret_cast<T*>(shared);
+  const uint32_t stages = smem_u32(shared);
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const uint32_t split = cluster_ctarank();
@@ -496,38 +503,40 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
   const int first = min(static_cast<int>(split) * per_split, tiles);
   const int last = min(first + per_split, tiles);
 
-  constexpr int kPieces = S::kColumns / 8;
-  constexpr int kRowStep = kAdapterThreads / kPieces;
-  constexpr int kPasses = S::kTokens / kRowStep;
-  const int piece = tid % kPieces;
+  constexpr int kPieces = S::kColumns / 8, kRowStep = kAdapterThreads / kPieces, kRowCopies = S::kTokens / kRowStep;
+  constexpr int kLowPieces = RANK / 8, kLowStep = kAdapterThreads / kLowPieces, kLowCopies = 2 * S::kTokens / kLowStep;
+  const int piece = tid % kPieces, row_of = tid / kPieces;
+  const int low_piece = tid % kLowPieces, low_row = tid / kLowPieces;
   const T* x = static_cast<const T*>(p.rows_in) + column0 + piece * 8;
-  const int64_t columns_left = p.width - (column0 + piece * 8);
-  const T* low = static_cast<const T*>(p.low);
+  const int columns_left = static_cast<int>(p.width - column0) - piece * 8;
+  const bool low_in = rank0 + low_piece * 8 < p.rank_pad;
+  const T* low = static_cast<const T*>(p.low) + (low_in ? rank0 + low_piece * 8 : 0);
+  const uint32_t row_to = stages + row_of * S::kRowBytes + piece * 16;
+  const uint32_t low_to = stages + S::kTokens * S::kRowBytes + low_row * S::kLowBytes + low_piece * 16;
 
   // The tokens of a tile are copied kStages - 1 tiles before its rows.
   auto look = [&](int tile) {
     const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + tid;
     if (tid >= S::kTokens || tile >= last) return;
-    if (slot < end) cp_async4(&tokens[tile % S::kLook][tid], p.rows + slot);
+    if (slot < end) cp_async4(smem_u32(&tokens[tile % S::kLook][tid]), p.rows + slot);
     else tokens[tile % S::kLook][tid] = -1;
   };
   auto load = [&](int tile) {
-    T* rows = stages + ((tile - first) % S::kStages) * S::kStageElements;
-    T* lows = rows + S::kTokens * S::kRowPitch;
+    const uint32_t stage = static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int row = tid / kPieces + i * kRowStep;
-      const int64_t token = tokens[tile % S::kLook][row];
-      copy8(rows + row * S::kRowPitch + piece * 8, x + token * p.row_stride,
-            token >= 0 && token < p.tokens ? columns_left : 0, p.vector_rows);
+    for (int i = 0; i < kRowCopies; ++i) {
+      const int32_t token = tokens[tile % S::kLook][row_of + i * kRowStep];
+      const bool in = token >= 0 && token < p.tokens && columns_left > 0;
+      copy8<T, FAST>(row_to + stage + i * kRowStep * S::kRowBytes,
+                     in ? x + token * p.row_stride : static_cast<const T*>(p.rows_in), in ? columns_left : 0);
     }
-    const int64_t slot0 = begin + static_cast<int64_t>(tile) * S::kTokens;
-    for (int i = tid; i < 2 * S::kTokens * (RANK / 8); i += kAdapterThreads) {
-      const int plane = i / (S::kTokens * (RANK / 8));
-      const int row = i / (RANK / 8) % S::kTokens, r = i % (RANK / 8) * 8;
-      const bool in = slot0 + row < end && rank0 + r < p.rank_pad;
-      copy8(lows + (plane * S::kTokens + row) * S::kLowPitch + r,
-            low + (plane * p.slots + slot0 + row) * p.rank_pad + rank0 + r, in ? 8 : 0, true);
+    const int slot0 = begin + tile * S::kTokens;
+#pragma unroll
+    for (int i = 0; i < kLowCopies; ++i) {
+      const int at = low_row + i * kLowStep, row = at % S::kTokens;
+      const bool in = low_in && slot0 + row < end;
+      cp_async16(low_to + stage + i * kLowStep * S::kLowBytes,
+                 in ? low + (at / S::kTokens * p.slots + slot0 + row) * p.rank_pad : low, in);
     }
   };
 
@@ -547,29 +556,27 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
     if (first + i < last) load(first + i);
     cp_async_commit();
   }
+  const uint32_t a_from = stages + ((lane >> 4) * 8 + (lane & 7)) * S::kRowBytes + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
+  const uint32_t b_from = stages + S::kTokens * S::kRowBytes + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::kLowBytes +
+                          (lane >> 4) * 16;
   for (int tile = first; tile < last; ++tile) {
     cp_async_wait<S::kStages - 2>();
     __syncthreads();
     if (tile + S::kStages - 1 < last) load(tile + S::kStages - 1);
     look(tile + 2 * (S::kStages - 1));
     cp_async_commit();
-    const T* rows = stages + ((tile - first) % S::kStages) * S::kStageElements;
-    const T* lows = rows + S::kTokens * S::kRowPitch;
+    const uint32_t stage = static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
 #pragma unroll
     for (int k = 0; k < S::kTokens; k += 16) {
       uint32_t a[2][4];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        ldmatrix_x4_trans(a[m], rows + (k + (lane >> 4) * 8 + (lane & 7)) * S::kRowPitch + warp * 32 + m * 16 +
-                                    ((lane >> 3) & 1) * 8);
-      }
+      for (int m = 0; m < 2; ++m) ldmatrix_x4_trans(a[m], a_from + stage + k * S::kRowBytes + m * 32);
 #pragma unroll
       for (int n = 0; n < RANK / 16; ++n) {
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
           uint32_t b[4];
-          ldmatrix_x4_trans(b, lows + (plane * S::kTokens + k + ((lane >> 3) & 1) * 8 + (lane & 7)) * S::kLowPitch +
-                                   n * 16 + (lane >> 4) * 8);
+          ldmatrix_x4_trans(b, b_from + stage + (plane * S::kTokens + k) * S::kLowBytes + n * 32);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             mma_16816<T>(acc[m][2 * n], a[m], b);
@@ -672,8 +679,10 @@ int launch_shrink(AdapterParams p, int64_t tiles, cudaStream_t stream) {
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int split = split_count(tiles * rank_blocks, chunks);
   p.chunks_per_split = static_cast<int>(ceil_div(chunks, split));
-  return launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS>, p,
-                          dim3(static_cast<unsigned>(tiles * split), rank_blocks), split, S::kBytes, false, stream);
+  const dim3 grid(static_cast<unsigned>(tiles * split), rank_blocks);
+  const bool fast = p.vector_rows && p.vector_weight && p.width % 8 == 0 && (!TRANS || p.rank % 8 == 0);
+  return fast ? launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, true>, p, grid, split, S::kBytes, false, stream)
+              : launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, false>, p, grid, split, S::kBytes, false, stream);
 }
 
 template <typename T, int ROWS, bool TRANS>
@@ -705,10 +714,14 @@ int launch_expand(AdapterParams p, int64_t tiles, bool dependent, cudaStream_t s
   while ((8 << p.piece_bits) < p.rank_pad) ++p.piece_bits;
   const int shared = expand_bytes(ROWS, kColumns, p.rank_pad, TRANS);
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (p.vector_rows && p.vector_out && p.width % 8 == 0) {
-    return launch_clustered(adapter_expand<T, ROWS, TRANS, true>, p, grid, 0, shared, dependent, stream);
+  const bool fast = p.vector_rows && p.vector_out && p.vector_weight && p.width % 8 == 0 && (TRANS || p.rank % 8 == 0);
+  if (!fast) return launch_clustered(adapter_expand<T, ROWS, TRANS, false, 0>, p, grid, 0, shared, dependent, stream);
+  switch (p.rank_pad) {
+    case 16: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 16>, p, grid, 0, shared, dependent, stream);
+    case 32: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 32>, p, grid, 0, shared, dependent, stream);
+    case 64: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 64>, p, grid, 0, shared, dependent, stream);
+    default: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 0>, p, grid, 0, shared, dependent, stream);
   }
-  return launch_clustered(adapter_expand<T, ROWS, TRANS, false>, p, grid, 0, shared, dependent, stream);
 }
 
 template <typename T>
@@ -728,9 +741,10 @@ int launch_outer(const AdapterParams& p, cudaStream_t stream) {
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int64_t tiles = ceil_div(ceil_div(p.slots, p.adapters), S::kTokens);
   const int split = split_count(columns * p.adapters * rank_blocks, tiles);
-  return launch_clustered(adapter_outer<T, RANK>, p,
-                          dim3(static_cast<unsigned>(columns * split), static_cast<unsigned>(p.adapters), rank_blocks),
-                          split, S::kBytes, false, stream);
+  const dim3 grid(static_cast<unsigned>(columns * split), static_cast<unsigned>(p.adapters), rank_blocks);
+  return p.vector_rows && p.width % 8 == 0
+             ? launch_clustered(adapter_outer<T, RANK, true>, p, grid, split, S::kBytes, false, stream)
+             : launch_clustered(adapter_outer<T, RANK, false>, p, grid, split, S::kBytes, false, stream);
 }
 
 template <typename T>
