@@ -490,7 +490,8 @@ int sdc_head_norm_rotary_backward(
 
 /* Low-rank adapters of many requests. `rows` int32 [slots...] lists tokens
  * grouped by adapter, tokens without one last; `tiles` int32 [tile_count][3]
- * are runs of it: {first slot, slots (<= tile_rows, 16 or 64), adapter or -1}.
+ * are runs of it: {first slot, slots (<= tile_rows: 16, or 128 for
+ * ranks of up to 128), adapter or -1}.
  * Types: bf16 or fp16. Rank <= 256.
  *
  * shrink: low[slot, :] = scale[adapter] * x[rows[slot], :] . weight^T, weight

@@ -17,7 +17,7 @@
 // A rank r of a few dozen against widths of thousands leaves about r flops a
 // byte of the streamed matrix: all three are bound by reading x, base and dy
 // and writing y and dx once, not by the tensor cores. Tokens of one adapter
-// are gathered into tiles of 64 rows (16 when adapters have few tokens, as in
+// are gathered into tiles of 128 rows (16 when adapters have few tokens, as in
 // decoding, where the weights are the traffic); low ranks are summed over the
 // width in fp32, across the blocks of a cluster through distributed shared
 // memory, so nothing is added in an order that changes.
@@ -35,7 +35,8 @@
 namespace sdc {
 namespace {
 
-constexpr int kAdapterThreads = 128;
+constexpr int kWide = 128, kNarrow = 16;  // rows of a tile
+constexpr int kMaxWideRank = 128;         // beyond, a wide tile's low rows and weight do not fit together
 constexpr int kMaxRank = 256;
 constexpr int kMaxSplit = 8;
 
@@ -75,23 +76,24 @@ __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot
 
 // ------------------------------------------------------------------ shrink ----
 
-// ROWS 64: four warps of 16 rows; ROWS 16: four warps share the rows and take
+// ROWS kWide: eight warps of 16 rows; ROWS kNarrow: four warps share the rows and take
 // a quarter of each chunk of the width. RANK: columns of `low` per block.
 template <int ROWS, int RANK, bool TRANS>
 struct ShrinkShape {
-  static constexpr int kChunk = ROWS == 64 ? 64 : 256;
+  static constexpr int kThreads = ROWS == kWide ? 256 : 128;
+  static constexpr int kChunk = ROWS == kWide ? 64 : 256;
   static constexpr int kStages = 4;
   static constexpr int kRowBytes = (kChunk + 8) * 2;  // 8 elements of padding: fragment rows on different banks
   static constexpr int kWeightRows = TRANS ? kChunk : RANK;
   static constexpr int kWeightBytes = ((TRANS ? RANK : kChunk) + 8) * 2;
   static constexpr int kStageBytes = ROWS * kRowBytes + kWeightRows * kWeightBytes;
-  static constexpr int kPartRows = ROWS == 64 ? 64 : 4 * 16;
+  static constexpr int kPartRows = ROWS == kWide ? ROWS : 4 * ROWS;
   static constexpr int kPartBytes = kPartRows * RANK * 4;
   static constexpr int kBytes = kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes;
 };
 
 template <typename T, int ROWS, int RANK, bool TRANS, bool FAST>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams p) {
+__global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adapter_shrink(AdapterParams p) {
   using S = ShrinkShape<ROWS, RANK, TRANS>;
   extern __shared__ __align__(16) uint8_t shared[];
   const uint32_t stages = smem_u32(shared);
@@ -112,9 +114,10 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
   // What this thread copies of a chunk: pieces of 8 elements of the rows, and
   // of the weight [rank, width], or [width, rank] when TRANS.
   constexpr int kPieces = S::kChunk / 8;
-  constexpr int kRowStep = kAdapterThreads / kPieces, kRowCopies = ROWS / kRowStep;
+  constexpr int kRowStep = S::kThreads / kPieces, kRowCopies = ROWS / kRowStep;
   constexpr int kWeightPieces = TRANS ? RANK / 8 : kPieces;
-  constexpr int kWeightStep = kAdapterThreads / kWeightPieces, kWeightCopies = S::kWeightRows / kWeightStep;
+  constexpr int kWeightStep = S::kThreads / kWeightPieces;
+  constexpr int kWeightCopies = (S::kWeightRows + kWeightStep - 1) / kWeightStep;
   const int piece = tid % kPieces, row_of = tid / kPieces;
   const int weight_piece = tid % kWeightPieces, weight_row = tid / kWeightPieces;
   const T* source[kRowCopies];
@@ -143,6 +146,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
 #pragma unroll
     for (int i = 0; i < kWeightCopies; ++i) {
       const int at = weight_row + i * kWeightStep;
+      if (S::kWeightRows % kWeightStep != 0 && at >= S::kWeightRows) continue;
       const int in = TRANS ? (k0 + at < width ? p.rank - (rank0 + weight_piece * 8) : 0) : (rank0 + at < p.rank ? left : 0);
       const T* from = weight + (TRANS ? static_cast<int64_t>(k0 + i * kWeightStep) * p.rank
                                       : static_cast<int64_t>(i * kWeightStep) * width + k0);
@@ -158,8 +162,8 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
     if (first + i < last) load(first + i);
     cp_async_commit();
   }
-  const int k_of = ROWS == 64 ? 0 : warp * (S::kChunk / 4);
-  const uint32_t a_from = stages + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * S::kRowBytes + (k_of + (lane >> 4) * 8) * 2;
+  const int k_of = ROWS == kWide ? 0 : warp * (S::kChunk / 4);
+  const uint32_t a_from = stages + ((ROWS == kWide ? warp * 16 : 0) + (lane & 15)) * S::kRowBytes + (k_of + (lane >> 4) * 8) * 2;
   const uint32_t b_from =
       stages + ROWS * S::kRowBytes +
       (TRANS ? (k_of + ((lane >> 3) & 1) * 8 + (lane & 7)) * S::kWeightBytes + (lane >> 4) * 16
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
     if (chunk + S::kStages - 1 < last) load(chunk + S::kStages - 1);
     cp_async_commit();
     const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
-    constexpr int kSteps = ROWS == 64 ? S::kChunk / 16 : S::kChunk / 64;
+    constexpr int kSteps = ROWS == kWide ? S::kChunk / 16 : S::kChunk / 64;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
       uint32_t a[4];
@@ -203,15 +207,15 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
   const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
   T* high = static_cast<T*>(p.low);
   T* low = high + p.slots * p.rank_pad;
-  for (int e = static_cast<int>(split) * kAdapterThreads + tid; e < count * RANK;
-       e += static_cast<int>(splits) * kAdapterThreads) {
+  for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * RANK; e += static_cast<int>(splits) * S::kThreads) {
     const int row = e / RANK, c = e % RANK;
     if (rank0 + c >= p.rank_pad) continue;
     float v = 0.f;
+#pragma unroll 4
     for (uint32_t s = 0; s < splits; ++s) {
       const uint32_t from = mapa_shared(part, s) + e * 4;
       v += load_cluster_f32(from);
-      if constexpr (ROWS == 16) {
+      if constexpr (ROWS == kNarrow) {
 #pragma unroll
         for (int other = 1; other < 4; ++other) v += load_cluster_f32(from + other * 16 * RANK * 4);
       }
@@ -228,15 +232,17 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink(AdapterParams 
 
 // ------------------------------------------------------------------ expand ----
 
-// ROWS 64: a warp takes 16 rows of 256 columns; ROWS 16: all 16 rows of 32 of
+// ROWS kWide: a warp takes 16 rows of 256 columns; ROWS kNarrow: all 16 rows of 32 of
 // 128 columns. A thread's accumulators over four 8-column tiles are made 8
 // neighbouring columns by assigning column 8 q + 2 j + b of 32 to element
 // 2 q + b of tile j: base and out then move in 16-byte words straight between
 // registers and memory.
 template <int ROWS>
 struct ExpandShape {
-  static constexpr int kColumns = ROWS == 64 ? 256 : 128;
-  static constexpr int kGroups = ROWS == 64 ? 8 : 1;  // 32-column groups per warp
+  static constexpr int kThreads = ROWS == kWide ? 256 : 128;
+  static constexpr int kBlocks = ROWS == kWide ? 2 : 4;  // at least, on an SM
+  static constexpr int kColumns = ROWS == kWide ? 256 : 128;
+  static constexpr int kGroups = ROWS == kWide ? 8 : 1;  // 32-column groups per warp
 };
 
 // Shared layout of the weight: !TRANS (weight [width, rank]): column-major
@@ -260,7 +266,7 @@ __host__ __device__ constexpr int expand_bytes(int rows, int columns, int rank_p
 // never stop. FAST: widths, strides and addresses allow 16-byte accesses
 // throughout. PAD: rank_pad, or 0 where it is read from the parameters.
 template <typename T, int ROWS, bool TRANS, bool FAST, int PAD>
-__global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterParams p) {
+__global__ void __launch_bounds__(ExpandShape<ROWS>::kThreads, ExpandShape<ROWS>::kBlocks) adapter_expand(AdapterParams p) {
   using S = ExpandShape<ROWS>;
   extern __shared__ __align__(16) uint8_t shared[];
   const int pad = PAD > 0 ? PAD : p.rank_pad;
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
   const bool two_buffers = low_buffers(pad) == 2;
   const int piece_bits = PAD > 0 ? (PAD <= 16 ? 1 : PAD <= 32 ? 2 : 3) : p.piece_bits;
   const int piece = tid & ((1 << piece_bits) - 1), piece_row = tid >> piece_bits;
-  const int piece_step = kAdapterThreads >> piece_bits;
+  const int piece_step = S::kThreads >> piece_bits;
 
   auto load_weight = [&](int adapter) {
     const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
@@ -292,7 +298,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
       }
     } else {
       constexpr int kPieces = S::kColumns / 8;
-      for (int i = tid; i < pad * kPieces; i += kAdapterThreads) {
+      for (int i = tid; i < pad * kPieces; i += S::kThreads) {
         const int r = i / kPieces, c = i % kPieces * 8;
         const T* from = weight + r * p.width + column0 + c;
         const int left = r < p.rank ? width - (column0 + c) : 0;
@@ -328,34 +334,36 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
 
   // This thread's part of base and out: rows lane / 4 and lane / 4 + 8 of its
   // 16, 8 columns of each 32.
-  const int row0 = (ROWS == 64 ? warp * 16 : 0) + (lane >> 2);
-  const int column = column0 + (ROWS == 64 ? 0 : warp * 32) + (lane & 3) * 8;
+  const int row0 = (ROWS == kWide ? warp * 16 : 0) + (lane >> 2);
+  const int column = column0 + (ROWS == kWide ? 0 : warp * 32) + (lane & 3) * 8;
   const int columns_left = width - column;  // column + 32 g + j lies in the matrix when 32 g + j is less
   struct Rows {
-    const T* base[2];  // null: no base or no row
-    T* out[2];         // null: no row
+    const T* base[2];
+    T* out[2];
+    int base_limit[2], out_limit[2];  // columns_left where there is a base and a row, else 0
   };
   auto look = [&](const Tile& tile) {
     Rows r;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t token = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
-      r.base[h] = token >= 0 && p.base != nullptr ? static_cast<const T*>(p.base) + token * p.base_stride + column : nullptr;
-      r.out[h] = token >= 0 ? static_cast<T*>(p.out) + token * p.out_stride + column : nullptr;
+      r.base[h] = static_cast<const T*>(p.base) + token * p.base_stride + column;
+      r.out[h] = static_cast<T*>(p.out) + token * p.out_stride + column;
+      r.out_limit[h] = token >= 0 ? columns_left : 0;
+      r.base_limit[h] = p.base != nullptr ? r.out_limit[h] : 0;
     }
     return r;
   };
-  auto load_base = [&](const T* from, int g) {
+  auto load_base = [&](const Rows& rows, int h, int g) {
     Raw8<T> r;
     r.w[0] = make_uint4(0, 0, 0, 0);
-    if (from == nullptr) return r;
     if constexpr (FAST) {
-      if (32 * g < columns_left) r = load8(from + 32 * g);
+      if (32 * g < rows.base_limit[h]) r = load8(rows.base[h] + 32 * g);
     } else {
       T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (32 * g + j < columns_left) e[j] = from[32 * g + j];
+        if (32 * g + j < rows.base_limit[h]) e[j] = rows.base[h][32 * g + j];
       }
     }
     return r;
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
 #pragma unroll
   for (int g = 0; g < S::kGroups; ++g) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) part[g][h] = load_base(rows.base[h], g);
+    for (int h = 0; h < 2; ++h) part[g][h] = load_base(rows, h, g);
   }
   int adapter = -1;  // whose weight is in shared memory
   if (adapted(tile)) load_weight(adapter = tile.adapter);
@@ -376,20 +384,20 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
   cp_async_commit();
   Tile next = first + 1 < last ? p.tiles[first + 1] : Tile{0, 0, -1};
   // Fragment addresses: low rows, and the weight's columns in the order above.
-  const uint32_t low_from = low_shared + ((ROWS == 64 ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 16;
+  const uint32_t low_from = low_shared + ((ROWS == kWide ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 16;
   uint32_t weight_from[2];
 #pragma unroll
   for (int pair = 0; pair < 2; ++pair) {
     const int i = lane & 7, j = 2 * pair + (lane >> 4), c = (i >> 1) * 8 + j * 2 + (i & 1);
     weight_from[pair] = weight_shared + (TRANS ? (((lane >> 3) & 1) * 8 + i) * kTransPitch + pair * 32 + (lane >> 4) * 16
                                                : c * pitch + (c >> 3) * 32 + ((lane >> 3) & 1) * 16);
-    if (ROWS == 16) weight_from[pair] += warp * (TRANS ? 64 : group_bytes);
+    if (ROWS == kNarrow) weight_from[pair] += warp * (TRANS ? 64 : group_bytes);
   }
   for (int t = first; t < last; ++t) {
     const int buffer = two_buffers ? (t - first) & 1 : 0;
     const bool more = t + 1 < last;
     const Tile after = t + 2 < last ? p.tiles[t + 2] : Tile{0, 0, -1};
-    if (more) next_rows = look(next);
+    next_rows = look(next);
     if (two_buffers && more && adapted(next)) load_low(next, buffer ^ 1);
     cp_async_commit();
     if (adapted(tile) && tile.adapter != adapter) {
@@ -402,12 +410,19 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
     }
     __syncthreads();
     const uint32_t low = low_from + buffer * low_bytes;
-    const bool mine = adapted(tile);
+    auto group = [&](int g, bool mine) {
+      float acc[4][4];  // base, to which the products are added
 #pragma unroll
-    for (int g = 0; g < S::kGroups; ++g) {
-      float acc[4][4];
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        unpack8(part[g][h], v);
+        part[g][h] = load_base(next_rows, h, g);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+          acc[j][2 * h] = v[2 * j];
+          acc[j][2 * h + 1] = v[2 * j + 1];
+        }
+      }
       if (mine) {
         auto step = [&](int k) {
           uint32_t hi[4], lo[4];
@@ -434,24 +449,28 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
-        unpack8(part[g][h], v);
-        if (more) part[g][h] = load_base(next_rows.base[h], g);
-        if (rows.out[h] == nullptr || 32 * g >= columns_left) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[2 * j] += acc[j][2 * h];
-          v[2 * j + 1] += acc[j][2 * h + 1];
+          v[2 * j] = acc[j][2 * h];
+          v[2 * j + 1] = acc[j][2 * h + 1];
         }
         T* to = rows.out[h] + 32 * g;
         if constexpr (FAST) {
-          store8(to, pack8<T>(v));
+          if (32 * g < rows.out_limit[h]) store8(to, pack8<T>(v));
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (32 * g + j < columns_left) to[j] = from_float<T>(v[j]);
+            if (32 * g + j < rows.out_limit[h]) to[j] = from_float<T>(v[j]);
           }
         }
       }
+    };
+    if (adapted(tile)) {
+#pragma unroll
+      for (int g = 0; g < S::kGroups; ++g) group(g, true);
+    } else {
+#pragma unroll
+      for (int g = 0; g < S::kGroups; ++g) group(g, false);
     }
     if (!two_buffers) {
       __syncthreads();
@@ -472,7 +491,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 4) adapter_expand(AdapterPara
 // adapter's tokens.
 template <int RANK>
 struct OuterShape {
-  static constexpr int kColumns = 128;
+  static constexpr int kThreads = 256;
+  static constexpr int kColumns = 256;
   static constexpr int kTokens = 32;
   static constexpr int kStages = 4;
   static constexpr int kLook = 2 * kStages;  // token lists in flight
@@ -485,7 +505,7 @@ struct OuterShape {
 };
 
 template <typename T, int RANK, bool FAST>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p) {
+__global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(AdapterParams p) {
   using S = OuterShape<RANK>;
   extern __shared__ __align__(16) uint8_t shared[];
   __shared__ int32_t tokens[S::kLook][S::kTokens];
@@ -503,8 +523,9 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
   const int first = min(static_cast<int>(split) * per_split, tiles);
   const int last = min(first + per_split, tiles);
 
-  constexpr int kPieces = S::kColumns / 8, kRowStep = kAdapterThreads / kPieces, kRowCopies = S::kTokens / kRowStep;
-  constexpr int kLowPieces = RANK / 8, kLowStep = kAdapterThreads / kLowPieces, kLowCopies = 2 * S::kTokens / kLowStep;
+  constexpr int kPieces = S::kColumns / 8, kRowStep = S::kThreads / kPieces, kRowCopies = S::kTokens / kRowStep;
+  constexpr int kLowPieces = RANK / 8, kLowStep = S::kThreads / kLowPieces;
+  constexpr int kLowCopies = (2 * S::kTokens + kLowStep - 1) / kLowStep;
   const int piece = tid % kPieces, row_of = tid / kPieces;
   const int low_piece = tid % kLowPieces, low_row = tid / kLowPieces;
   const T* x = static_cast<const T*>(p.rows_in) + column0 + piece * 8;
@@ -534,6 +555,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
 #pragma unroll
     for (int i = 0; i < kLowCopies; ++i) {
       const int at = low_row + i * kLowStep, row = at % S::kTokens;
+      if (2 * S::kTokens % kLowStep != 0 && at >= 2 * S::kTokens) continue;
       const bool in = low_in && slot0 + row < end;
       cp_async16(low_to + stage + i * kLowStep * S::kLowBytes,
                  in ? low + (at / S::kTokens * p.slots + slot0 + row) * p.rank_pad : low, in);
@@ -605,12 +627,13 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
   cluster_sync();
   T* out = static_cast<T*>(p.out) + static_cast<int64_t>(adapter) * p.rank * p.width;
   const bool columns_fast = p.out_stride == 1;  // neighbouring threads write neighbouring elements
-  for (int e = static_cast<int>(split) * kAdapterThreads + tid; e < S::kColumns * RANK;
-       e += static_cast<int>(splits) * kAdapterThreads) {
+  for (int e = static_cast<int>(split) * S::kThreads + tid; e < S::kColumns * RANK;
+       e += static_cast<int>(splits) * S::kThreads) {
     const int c = columns_fast ? e % S::kColumns : e / RANK;
     const int r = columns_fast ? e / S::kColumns : e % RANK;
     if (column0 + c >= p.width || rank0 + r >= p.rank) continue;
     float v = 0.f;
+#pragma unroll 4
     for (uint32_t s = 0; s < splits; ++s) v += load_cluster_f32(mapa_shared(part, s) + (c * S::kPartPitch + r) * 4);
     out[(column0 + c) * p.out_stride + (rank0 + r) * p.out_rank_stride] = from_float<T>(v);
   }
@@ -620,14 +643,14 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_outer(AdapterParams p
 // -------------------------------------------------------------------- host ----
 
 template <typename Kernel>
-int launch_clustered(Kernel kernel, const AdapterParams& p, dim3 grid, int cluster, int shared, bool dependent,
-                     cudaStream_t stream) {
+int launch_clustered(Kernel kernel, const AdapterParams& p, dim3 grid, int threads, int cluster, int shared,
+                     bool dependent, cudaStream_t stream) {
   if (shared > 48 * 1024) {
     SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
   }
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
-  config.blockDim = dim3(kAdapterThreads);
+  config.blockDim = dim3(static_cast<unsigned>(threads));
   config.dynamicSmemBytes = static_cast<size_t>(shared);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
@@ -664,12 +687,11 @@ int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
 bool vector_rows(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
-// Blocks that share a tile's sum: enough for two blocks on every SM, as long
-// as each keeps two chunks.
-int split_count(int64_t blocks, int64_t chunks) {
-  int split = 1;
-  while (split < kMaxSplit && blocks * split < 2 * sm_count() && chunks >= 4 * split) split *= 2;
-  return split;
+// Blocks that share a tile's sum: as many as fill the SMs' `resident` blocks
+// each once, as long as each keeps two chunks.
+int split_count(int64_t blocks, int64_t chunks, int resident) {
+  const int64_t wanted = std::min<int64_t>(static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(blocks, 1), chunks / 2);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, kMaxSplit)));
 }
 
 template <typename T, int ROWS, int RANK, bool TRANS>
@@ -677,12 +699,12 @@ int launch_shrink(AdapterParams p, int64_t tiles, cudaStream_t stream) {
   using S = ShrinkShape<ROWS, RANK, TRANS>;
   const int64_t chunks = ceil_div(p.width, S::kChunk);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
-  const int split = split_count(tiles * rank_blocks, chunks);
+  const int split = split_count(tiles * rank_blocks, chunks, ROWS == kWide ? 2 : 4);
   p.chunks_per_split = static_cast<int>(ceil_div(chunks, split));
   const dim3 grid(static_cast<unsigned>(tiles * split), rank_blocks);
   const bool fast = p.vector_rows && p.vector_weight && p.width % 8 == 0 && (!TRANS || p.rank % 8 == 0);
-  return fast ? launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, true>, p, grid, split, S::kBytes, false, stream)
-              : launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, false>, p, grid, split, S::kBytes, false, stream);
+  return fast ? launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, true>, p, grid, S::kThreads, split, S::kBytes, false, stream)
+              : launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, false>, p, grid, S::kThreads, split, S::kBytes, false, stream);
 }
 
 template <typename T, int ROWS, bool TRANS>
@@ -696,42 +718,44 @@ int shrink_by_rank(const AdapterParams& p, int64_t tiles, cudaStream_t stream) {
 
 template <typename T>
 int shrink_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tiles, cudaStream_t stream) {
-  if (tile_rows == 64) return trans ? shrink_by_rank<T, 64, true>(p, tiles, stream) : shrink_by_rank<T, 64, false>(p, tiles, stream);
-  return trans ? shrink_by_rank<T, 16, true>(p, tiles, stream) : shrink_by_rank<T, 16, false>(p, tiles, stream);
+  if (tile_rows == kWide) return trans ? shrink_by_rank<T, kWide, true>(p, tiles, stream) : shrink_by_rank<T, kWide, false>(p, tiles, stream);
+  return trans ? shrink_by_rank<T, kNarrow, true>(p, tiles, stream) : shrink_by_rank<T, kNarrow, false>(p, tiles, stream);
 }
 
 template <typename T, int ROWS, bool TRANS>
 int launch_expand(AdapterParams p, int64_t tiles, bool dependent, cudaStream_t stream) {
-  constexpr int kColumns = ExpandShape<ROWS>::kColumns;
+  using S = ExpandShape<ROWS>;
+  constexpr int kColumns = S::kColumns;
   const int64_t column_blocks = ceil_div(p.width, kColumns);
-  // Runs of tiles that fill the SMs' four blocks each once; tiles of few rows
+  // Runs of tiles that fill the SMs' blocks once; tiles of few rows
   // are bound by the weight, of which each then wants its own.
   p.tile_count = static_cast<int>(tiles);
-  const int64_t runs = std::max<int64_t>(1, 4 * sm_count() / column_blocks);
-  p.tiles_per_block = ROWS == 64 ? static_cast<int>(ceil_div(tiles, runs)) : 1;
+  const int64_t runs = std::max<int64_t>(1, S::kBlocks * sm_count() / column_blocks);
+  p.tiles_per_block = ROWS == kWide ? static_cast<int>(ceil_div(tiles, runs)) : 1;
   const int64_t blocks = column_blocks * ceil_div(tiles, p.tiles_per_block);
   SDC_REQUIRE(blocks <= INT_MAX, "low-rank adapters have too many tiles for one launch");
   while ((8 << p.piece_bits) < p.rank_pad) ++p.piece_bits;
+  dependent = dependent && ROWS == kNarrow;  // blocks of long runs that start early, where there is room, end late
   const int shared = expand_bytes(ROWS, kColumns, p.rank_pad, TRANS);
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool fast = p.vector_rows && p.vector_out && p.vector_weight && p.width % 8 == 0 && (TRANS || p.rank % 8 == 0);
-  if (!fast) return launch_clustered(adapter_expand<T, ROWS, TRANS, false, 0>, p, grid, 0, shared, dependent, stream);
+  if (!fast) return launch_clustered(adapter_expand<T, ROWS, TRANS, false, 0>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
   switch (p.rank_pad) {
-    case 16: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 16>, p, grid, 0, shared, dependent, stream);
-    case 32: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 32>, p, grid, 0, shared, dependent, stream);
-    case 64: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 64>, p, grid, 0, shared, dependent, stream);
-    default: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 0>, p, grid, 0, shared, dependent, stream);
+    case 16: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 16>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
+    case 32: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 32>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
+    case 64: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 64>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
+    default: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 0>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
   }
 }
 
 template <typename T>
 int expand_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tiles, bool dependent, cudaStream_t stream) {
-  if (tile_rows == 64) {
-    return trans ? launch_expand<T, 64, true>(p, tiles, dependent, stream)
-                 : launch_expand<T, 64, false>(p, tiles, dependent, stream);
+  if (tile_rows == kWide) {
+    return trans ? launch_expand<T, kWide, true>(p, tiles, dependent, stream)
+                 : launch_expand<T, kWide, false>(p, tiles, dependent, stream);
   }
-  return trans ? launch_expand<T, 16, true>(p, tiles, dependent, stream)
-               : launch_expand<T, 16, false>(p, tiles, dependent, stream);
+  return trans ? launch_expand<T, kNarrow, true>(p, tiles, dependent, stream)
+               : launch_expand<T, kNarrow, false>(p, tiles, dependent, stream);
 }
 
 template <typename T, int RANK>
@@ -740,11 +764,11 @@ int launch_outer(const AdapterParams& p, cudaStream_t stream) {
   const int64_t columns = ceil_div(p.width, S::kColumns);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int64_t tiles = ceil_div(ceil_div(p.slots, p.adapters), S::kTokens);
-  const int split = split_count(columns * p.adapters * rank_blocks, tiles);
+  const int split = split_count(columns * p.adapters * rank_blocks, tiles, 2);
   const dim3 grid(static_cast<unsigned>(columns * split), static_cast<unsigned>(p.adapters), rank_blocks);
   return p.vector_rows && p.width % 8 == 0
-             ? launch_clustered(adapter_outer<T, RANK, true>, p, grid, split, S::kBytes, false, stream)
-             : launch_clustered(adapter_outer<T, RANK, false>, p, grid, split, S::kBytes, false, stream);
+             ? launch_clustered(adapter_outer<T, RANK, true>, p, grid, S::kThreads, split, S::kBytes, false, stream)
+             : launch_clustered(adapter_outer<T, RANK, false>, p, grid, S::kThreads, split, S::kBytes, false, stream);
 }
 
 template <typename T>
@@ -773,7 +797,8 @@ int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride, int64_t token
   using namespace sdc;
   int rc = check_adapters(dtype, tokens, width, rank, adapters);
   if (rc != SDC_OK) return rc;
-  SDC_REQUIRE(tile_rows == 16 || tile_rows == 64, "low-rank adapter tiles have 16 or 64 rows");
+  SDC_REQUIRE(tile_rows == kNarrow || (tile_rows == kWide && rank <= kMaxWideRank),
+              "low-rank adapter tiles have 16 rows, or 128 for ranks of up to 128");
   SDC_REQUIRE(tile_count >= 0 && tile_count <= INT_MAX / kMaxSplit, "low-rank adapters have too many tiles for one launch");
   if (tile_count == 0) return SDC_OK;
   SDC_REQUIRE(x != nullptr && rows != nullptr && tiles != nullptr && weight != nullptr && low != nullptr && aligned16(low),
@@ -807,7 +832,8 @@ int sdc_adapter_expand(int dtype, const void* base, int64_t base_stride, int64_t
   using namespace sdc;
   int rc = check_adapters(dtype, tokens, width, rank, adapters);
   if (rc != SDC_OK) return rc;
-  SDC_REQUIRE(tile_rows == 16 || tile_rows == 64, "low-rank adapter tiles have 16 or 64 rows");
+  SDC_REQUIRE(tile_rows == kNarrow || (tile_rows == kWide && rank <= kMaxWideRank),
+              "low-rank adapter tiles have 16 rows, or 128 for ranks of up to 128");
   SDC_REQUIRE(tile_count >= 0 && tile_count <= INT_MAX, "low-rank adapters have too many tiles for one launch");
   if (tile_count == 0) return SDC_OK;
   SDC_REQUIRE(rows != nullptr && tiles != nullptr && weight != nullptr && (low != nullptr || slots == 0) && out != nullptr &&

@@ -28,7 +28,7 @@ template <typename T>
 __device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, const uint32_t* b);
 template <>
 __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float* d, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -36,7 +36,7 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float* d, const uint32_
 }
 template <>
 __device__ __forceinline__ void mma_16816<__half>(float* d, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])

@@ -28,6 +28,7 @@ namespace {
 constexpr int kRotaryThreads = 256;
 constexpr int kForwardHeads = 4;
 constexpr int kBackwardHeads = 2;
+constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;  // on an SM at least
 constexpr int kMaxHeadDim = 512;  // 32 lanes of 16 elements
 
 struct RotaryParams {
@@ -207,7 +208,7 @@ __device__ __forceinline__ float group_sum(float x) {
 }
 
 template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_forward(RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, kForwardBlocks) rotary_forward(RotaryParams p) {
   constexpr int kGroups = kRotaryThreads / LANES;
   const uint32_t item = blockIdx.x * kGroups + threadIdx.x / LANES;
   const uint32_t token = item / p.chunks;
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_forward(RotaryParams p)
 // 16 weight gradients stay in registers for the whole launch; the block adds
 // its groups' sums in a fixed order and writes one partial per role.
 template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_backward(RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, kBackwardBlocks) rotary_backward(RotaryParams p) {
   constexpr int kGroups = kRotaryThreads / LANES;
   __shared__ float sums[kRotaryThreads * 16];
   const uint32_t group = blockIdx.x * kGroups + threadIdx.x / LANES;
@@ -364,24 +365,28 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_backward(RotaryParams p
   }
 }
 
-// dweight[role][e] = sum over blocks, ascending within each of 8 strands, the
-// strands added in a fixed order.
+// dweight[role][e] = sum over blocks: 32 strands of every 32nd block, each
+// ascending, joined in a fixed order.
 template <typename W>
-__global__ void __launch_bounds__(256) rotary_weight_grad(const float* partials, int blocks, int dim, int columns,
-                                                          W* dq, W* dk) {
-  __shared__ float strand[8][32];
-  const int column = blockIdx.x * 32 + threadIdx.x;
+__global__ void __launch_bounds__(1024) rotary_weight_grad(const float* partials, int blocks, int dim, int columns,
+                                                           W* dq, W* dk) {
+  __shared__ float strand[32][33];
+  const int lane = threadIdx.x, y = threadIdx.y;
+  const int column = blockIdx.x * 32 + lane;
   float total = 0.f;
   if (column < columns) {
-    for (int b = threadIdx.y; b < blocks; b += 8) total += partials[static_cast<int64_t>(b) * 2 * dim + column];
+#pragma unroll 4
+    for (int b = y; b < blocks; b += 32) total += partials[static_cast<int64_t>(b) * 2 * dim + column];
   }
-  strand[threadIdx.y][threadIdx.x] = total;
+  strand[y][lane] = total;
   __syncthreads();
-  if (threadIdx.y == 0 && column < columns) {
-    total = ((strand[0][threadIdx.x] + strand[1][threadIdx.x]) + (strand[2][threadIdx.x] + strand[3][threadIdx.x])) +
-            ((strand[4][threadIdx.x] + strand[5][threadIdx.x]) + (strand[6][threadIdx.x] + strand[7][threadIdx.x]));
-    if (column < dim) dq[column] = from_float<W>(total);
-    else dk[column - dim] = from_float<W>(total);
+  total = strand[lane][y];  // column y's strands, one a lane
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2) total += __shfl_xor_sync(0xffffffffu, total, step);
+  const int mine = blockIdx.x * 32 + y;
+  if (lane == 0 && mine < columns) {
+    if (mine < dim) dq[mine] = from_float<W>(total);
+    else dk[mine - dim] = from_float<W>(total);
   }
 }
 
@@ -576,7 +581,7 @@ int sdc_head_norm_rotary_backward(int dtype, const void* dq_out, const int64_t* 
   const unsigned grid = static_cast<unsigned>(ceil_div(columns, 32));
   auto reduce = [&](auto element) {
     using W = decltype(element);
-    rotary_weight_grad<W><<<grid, dim3(32, 8), 0, stream>>>(p.partials, blocks, dim, columns, static_cast<W*>(dq_weight),
+    rotary_weight_grad<W><<<grid, dim3(32, 32), 0, stream>>>(p.partials, blocks, dim, columns, static_cast<W*>(dq_weight),
                                                             static_cast<W*>(dk_weight));
   };
   if (weight_f32 || dtype == kF32) reduce(float{});

@@ -209,7 +209,7 @@ AdapterArgs check_adapters(const Tensor& x, const Tensor& a, const Tensor& b, Op
                   tiles.dim() == 2 && tiles.size(1) == 3,
               "the adapter batch was made for another number of tokens or adapters");
   TORCH_CHECK(slots >= 0 && slots <= x.size(0) && active >= 0 && active <= tiles.size(0) &&
-                  (tile_rows == 16 || tile_rows == 64),
+                  (tile_rows == 16 || tile_rows == 128),
               "the adapter batch is inconsistent");
   return {x.size(0), x.size(1), b.size(1), slots, active, tiles.size(0), x.scalar_type() == at::kBFloat16 ? 1 : 2,
           static_cast<int>(a.size(0)), static_cast<int>(a.size(1)), static_cast<int>(tile_rows)};

@@ -9,9 +9,10 @@ from .. import ops
 _OP, _OP_IN_PLACE = ops.low_rank_adapters.default, ops.low_rank_adapters_.default
 
 # Rows of a tile. With at least this many tokens an adapter on average, tiles
-# of 64 rows share one read of the adapter's weights; below, most of their rows
-# would be empty and tiles of 16 do less for the same traffic.
-_WIDE_TILE, _NARROW_TILE, _WIDE_FROM = 64, 16, 32
+# of 128 rows share one read of the adapter's weights; below, most of their rows
+# would be empty and tiles of 16 do less for the same traffic. Ranks beyond
+# _WIDE_RANK leave no room for wide tiles beside the weight.
+_WIDE_TILE, _NARROW_TILE, _WIDE_FROM, _WIDE_RANK = 128, 16, 32, 128
 
 
 def _tiles(offsets, tokens, rows):
@@ -56,13 +57,20 @@ class AdapterBatch:
         slots = int(offsets[-1])
         used = int((np.diff(offsets) > 0).sum())
         self.tokens, self.count, self.slots = tokens, int(count), slots
-        self.tile_rows = _WIDE_TILE if used and slots >= _WIDE_FROM * used else _NARROW_TILE
-        tiles, self.active = _tiles(offsets, tokens, self.tile_rows)
         rows = np.argsort(of_token, kind="stable").astype(np.int32)
-        packed = torch.from_numpy(np.concatenate((rows, offsets.astype(np.int32), tiles.reshape(-1)))).to(device)
-        self.rows, self.groups, tiles = packed.split((tokens, count + 1, tiles.size))
-        self.tiles = tiles.view(-1, 3)
-        self.arguments = (self.rows, self.groups, self.tiles, self.slots, self.active, self.tile_rows)
+        narrow, narrow_active = _tiles(offsets, tokens, _NARROW_TILE)
+        wide, wide_active = narrow[:0], 0
+        if used and slots >= _WIDE_FROM * used:
+            wide, wide_active = _tiles(offsets, tokens, _WIDE_TILE)
+        packed = torch.from_numpy(np.concatenate((rows, offsets.astype(np.int32), narrow.reshape(-1),
+                                                  wide.reshape(-1)))).to(device)
+        self.rows, self.groups, narrow, wide = packed.split((tokens, count + 1, narrow.size, wide.size))
+        self._narrow = (self.rows, self.groups, narrow.view(-1, 3), slots, narrow_active, _NARROW_TILE)
+        self._wide = (self.rows, self.groups, wide.view(-1, 3), slots, wide_active, _WIDE_TILE)
+
+    def arguments(self, rank):
+        """The kernels' view of the batch for adapters of a rank."""
+        return self._wide if self._wide[4] and rank <= _WIDE_RANK else self._narrow
 
 
 def _check(x, batch):
@@ -86,11 +94,11 @@ def low_rank_adapters(base, x, a, b, batch, scale=None):
     rows are kept in 32 bits up to the second product, which takes them as two
     16-bit terms; in fp16 they overflow beyond 65504 like the type does."""
     _check(x, batch)
-    return _OP(base, x, a, b, scale, *batch.arguments)[0]
+    return _OP(base, x, a, b, scale, *batch.arguments(a.shape[1]))[0]
 
 
 def low_rank_adapters_(base, x, a, b, batch, scale=None):
     """``low_rank_adapters`` into ``base``: rows without an adapter are not touched."""
     _check(x, batch)
-    _OP_IN_PLACE(base, x, a, b, scale, *batch.arguments)
+    _OP_IN_PLACE(base, x, a, b, scale, *batch.arguments(a.shape[1]))
     return base

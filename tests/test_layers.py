@@ -17,18 +17,21 @@ from sdc_b200.layers import (AdapterBatch, distillation_loss, head_norm_rotary, 
 def test_adapter_batch_lists_every_token_once_under_its_adapter(lengths, adapters, count):
     batch = AdapterBatch(lengths, adapters, count, device="cpu")
     of_token = np.repeat(np.asarray(adapters, dtype=np.int64), lengths)
-    rows, groups, tiles = (t.numpy() for t in (batch.rows, batch.groups, batch.tiles))
-    assert sorted(rows.tolist()) == list(range(len(of_token)))
-    assert batch.slots == int((of_token >= 0).sum()) == groups[-1]
-    for g in range(count):
-        assert rows[groups[g]:groups[g + 1]].tolist() == np.flatnonzero(of_token == g).tolist()
-    seen = np.zeros(len(of_token), dtype=int)
-    for i, (first, slots, adapter) in enumerate(tiles):
-        assert 1 <= slots <= batch.tile_rows
-        assert (adapter >= 0) == (i < batch.active)
-        assert (of_token[rows[first:first + slots]] == adapter).all()
-        seen[first:first + slots] += 1
-    assert (seen == 1).all()
+    for rank in (1, 128, 129, 256):
+        rows, groups, tiles, slots, active, tile_rows = batch.arguments(rank)
+        rows, groups, tiles = (t.numpy() for t in (rows, groups, tiles))
+        assert tile_rows == 16 or (tile_rows == 128 and rank <= 128)
+        assert sorted(rows.tolist()) == list(range(len(of_token)))
+        assert slots == int((of_token >= 0).sum()) == groups[-1]
+        for g in range(count):
+            assert rows[groups[g]:groups[g + 1]].tolist() == np.flatnonzero(of_token == g).tolist()
+        seen = np.zeros(len(of_token), dtype=int)
+        for i, (first, length, adapter) in enumerate(tiles):
+            assert 1 <= length <= tile_rows
+            assert (adapter >= 0) == (i < active)
+            assert (of_token[rows[first:first + length]] == adapter).all()
+            seen[first:first + length] += 1
+        assert (seen == 1).all()
 
 
 def test_adapter_batch_refusals():
@@ -82,7 +85,7 @@ def test_argument_contracts_are_checked_before_launch():
         return lib.sdc_adapter_shrink(dtype, fake, 64, 4, fake, fake, tiles, tile_rows, fake, adapters, rank, width, 0,
                                       None, low, 4, None)
 
-    for kwargs, text in ((dict(dtype=0), "BF16"), (dict(tile_rows=32), "16 or 64"), (dict(rank=257), "256"),
+    for kwargs, text in ((dict(dtype=0), "BF16"), (dict(tile_rows=32), "16 rows"), (dict(rank=257), "256"), (dict(rank=129, tile_rows=128), "up to 128"),
                          (dict(adapters=0), "adapters"), (dict(width=0), "positive"), (dict(low=None), "null"),
                          (dict(low=fake + 8), "aligned")):
         assert shrink(**kwargs) == capi.SDC_ERR_INVALID and text in capi.last_error(), kwargs
