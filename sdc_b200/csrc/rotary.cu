@@ -13,22 +13,27 @@
 // of each, so the rotation needs no exchange between threads; in the common
 // forms its 16 elements are two (16-bit types) or four (fp32) 16-byte words.
 // dim/16 neighbouring lanes share a head and exchange only the sum of squares
-// (and, backward, of products). A group of lanes takes up to kForwardHeads
-// heads of one token: all their loads are issued before the first is used,
-// and the angles and weights are read once for them.
+// (and, backward, of products). A group of lanes keeps a few heads of every
+// so manieth token, so weights are read once and angles once for its heads;
+// the heads of the tokens to come are copied to shared memory meanwhile, each
+// thread its own words, so that no barrier is needed and loads never stop.
 #include <algorithm>
 #include <climits>
 #include <cmath>
 
-#include "layers.cuh"
+#include "mma.cuh"
 
 namespace sdc {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kForwardHeads = 4;
-constexpr int kBackwardHeads = 2;
-constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;  // on an SM at least
+// Heads of a group, by the type's size: two blocks share an SM's shared memory.
+template <typename T>
+constexpr int kForwardHeads = sizeof(T) == 2 ? 4 : 2;
+template <typename T>
+constexpr int kBackwardHeads = sizeof(T) == 2 ? 2 : 1;
+constexpr int kRotaryBlocks = 2;  // on an SM
+constexpr int kStages = 3;        // tokens of a group under way
 constexpr int kMaxHeadDim = 512;  // 32 lanes of 16 elements
 
 struct RotaryParams {
@@ -53,13 +58,18 @@ struct RotaryParams {
   float* partials;       // backward: [blocks][2][dim]
 };
 
+__device__ __forceinline__ int64_t load_position(const RotaryParams& p, uint32_t token) {
+  const int64_t batch = token / p.sequence, seq = token - static_cast<uint32_t>(batch) * p.sequence;
+  const int64_t at = batch * p.position_strides[0] + seq * p.position_strides[1];
+  return p.positions_64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+}
+
 // The position's cosine and sine for this lane's 8 pairs; identity beyond the
 // rotary pairs. A position outside the table gives NaN, not a stray read.
-__device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t batch, int64_t seq, int first_pair,
-                                            float* cosine, float* sine) {
-  const int64_t at = batch * p.position_strides[0] + seq * p.position_strides[1];
-  const int64_t position = p.positions_64 ? static_cast<const int64_t*>(p.positions)[at]
-                                          : static_cast<const int32_t*>(p.positions)[at];
+struct Angles {
+  float cosine[8], sine[8];
+};
+__device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t position, int first_pair, Angles& a) {
   const int half = p.rotary / 2;
   const bool inside = position >= 0 && position < p.table_rows;
   const float* row = p.table + (inside ? position : 0) * p.rotary;
@@ -68,8 +78,8 @@ __device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t batch
     for (int i = 0; i < 2; ++i) {
       const float4 c = reinterpret_cast<const float4*>(row + first_pair)[i];
       const float4 s = reinterpret_cast<const float4*>(row + half + first_pair)[i];
-      cosine[4 * i] = c.x, cosine[4 * i + 1] = c.y, cosine[4 * i + 2] = c.z, cosine[4 * i + 3] = c.w;
-      sine[4 * i] = s.x, sine[4 * i + 1] = s.y, sine[4 * i + 2] = s.z, sine[4 * i + 3] = s.w;
+      a.cosine[4 * i] = c.x, a.cosine[4 * i + 1] = c.y, a.cosine[4 * i + 2] = c.z, a.cosine[4 * i + 3] = c.w;
+      a.sine[4 * i] = s.x, a.sine[4 * i + 1] = s.y, a.sine[4 * i + 2] = s.z, a.sine[4 * i + 3] = s.w;
     }
     return;
   }
@@ -78,8 +88,8 @@ __device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t batch
   for (int i = 0; i < 8; ++i) {
     const int pair = first_pair + i;
     const bool turned = pair < half;
-    cosine[i] = turned ? (inside ? row[pair] : nan) : 1.f;
-    sine[i] = turned ? (inside ? row[half + pair] : nan) : 0.f;
+    a.cosine[i] = turned ? (inside ? row[pair] : nan) : 1.f;
+    a.sine[i] = turned ? (inside ? row[half + pair] : nan) : 0.f;
   }
 }
 
@@ -127,6 +137,28 @@ struct HeadIO {
         a[i] = in ? head[element_of<INTERLEAVED>(pair, 0, rotary)] : from_float<T>(0.f);
         b[i] = in ? head[element_of<INTERLEAVED>(pair, 1, rotary)] : from_float<T>(0.f);
       }
+    }
+    return r;
+  }
+  // The same through this thread's own words of shared memory: words `at`,
+  // `at` + kRotaryThreads, ... of 16 bytes.
+  static constexpr int kWords = 2 * static_cast<int>(sizeof(Raw8<T>)) / 16;
+  __device__ __forceinline__ void issue(const T* head, uint32_t at) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      const T* run = head + (i < kWords / 2 ? low_run() : high_run());
+      cp_async16(at + i * kRotaryThreads * 16, reinterpret_cast<const uint4*>(run) + i % (kWords / 2));
+    }
+  }
+  __device__ __forceinline__ Raw fetch(uint32_t at) const {
+    Raw r;
+    uint4* words[2] = {r.a.w, r.b.w};
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      uint4& w = words[i / (kWords / 2)][i % (kWords / 2)];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                   : "r"(at + i * kRotaryThreads * 16));
     }
     return r;
   }
@@ -207,115 +239,167 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
-__global__ void __launch_bounds__(kRotaryThreads, kForwardBlocks) rotary_forward(RotaryParams p) {
-  constexpr int kGroups = kRotaryThreads / LANES;
-  const uint32_t item = blockIdx.x * kGroups + threadIdx.x / LANES;
-  const uint32_t token = item / p.chunks;
-  const uint32_t chunk = item - token * p.chunks;
-  const HeadIO<T, INTERLEAVED, VECTOR> io(p, threadIdx.x % LANES);
-  // Whole groups are idle or active; idle lanes still take part in the sums.
-  const bool live = token < p.tokens && io.active;
-  const int role = chunk >= p.q_chunks;
-  const int head0 = static_cast<int>(chunk - (role ? p.q_chunks : 0)) * kForwardHeads;
-  const int64_t batch = live ? token / p.sequence : 0, seq = live ? token % p.sequence : 0;
-  const T* x = static_cast<const T*>(p.x[role]) + batch * p.xs[role][0] + seq * p.xs[role][1];
-  T* y = static_cast<T*>(p.y[role]) + static_cast<int64_t>(token) * p.heads[role] * p.dim;
+// What a group of lanes works on: one chunk of heads of every walkers-th token.
+// All lanes of a warp run the same number of rounds (their sums are exchanged
+// by the whole warp); lanes without work there are not `live`.
+template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int HEADS, int TENSORS>
+struct Walk {
+  using IO = HeadIO<T, INTERLEAVED, VECTOR>;
+  static constexpr int kGroups = kRotaryThreads / LANES;
+  static constexpr int kStageBytes = TENSORS * HEADS * IO::kWords * kRotaryThreads * 16;
+  const RotaryParams& p;
+  const IO io;
+  uint32_t walkers, walker, shared;
+  int role, head0, heads;
+  bool working;
 
-  typename HeadIO<T, INTERLEAVED, VECTOR>::Raw raw[kForwardHeads];
-#pragma unroll
-  for (int h = 0; h < kForwardHeads; ++h) {
-    if (live && head0 + h < p.heads[role]) raw[h] = io.load(x + (head0 + h) * p.xs[role][2]);
+  __device__ __forceinline__ Walk(const RotaryParams& params, uint32_t shared_base)
+      : p(params), io(params, threadIdx.x % LANES), shared(shared_base + threadIdx.x * 16) {
+    const uint32_t group = blockIdx.x * kGroups + threadIdx.x / LANES;
+    walkers = gridDim.x * kGroups / p.chunks;
+    walker = group / p.chunks;
+    const uint32_t chunk = group - walker * p.chunks;
+    role = chunk >= p.q_chunks;
+    head0 = static_cast<int>(chunk - (role ? p.q_chunks : 0)) * HEADS;
+    heads = min(HEADS, p.heads[role] - head0);
+    working = walker < walkers && io.active;
   }
-  float cosine[8], sine[8], w[16];
+  __device__ __forceinline__ uint32_t rounds() const { return (p.tokens + walkers - 1) / walkers; }
+  __device__ __forceinline__ uint32_t token(uint32_t round) const { return round * walkers + walker; }
+  __device__ __forceinline__ bool live(uint32_t round) const { return working && token(round) < p.tokens; }
+  __device__ __forceinline__ const T* head_at(const void* base, const int64_t* strides, uint32_t token, int h) const {
+    const uint32_t batch = token / p.sequence, seq = token - batch * p.sequence;
+    return static_cast<const T*>(base) + batch * strides[0] + seq * strides[1] + (head0 + h) * strides[2];
+  }
+  __device__ __forceinline__ uint32_t slot(uint32_t round, int tensor, int h) const {
+    return shared + round % kStages * kStageBytes + (tensor * HEADS + h) * IO::kWords * kRotaryThreads * 16;
+  }
+  // Starts the copies of a round's heads (tensor 0: x, 1: dy).
+  __device__ __forceinline__ void issue(uint32_t round, int tensor, const void* base, const int64_t* strides) const {
+    if (!VECTOR || !live(round)) return;
+    const T* first = head_at(base, strides, token(round), 0);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      if (h < heads) io.issue(first + h * strides[2], slot(round, tensor, h));
+    }
+  }
+  __device__ __forceinline__ typename IO::Raw head(uint32_t round, int tensor, const void* base, const int64_t* strides,
+                                                   int h) const {
+    if constexpr (VECTOR) return io.fetch(slot(round, tensor, h));
+    else return io.load(head_at(base, strides, token(round), h));
+  }
+};
+
+template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
+__global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(RotaryParams p) {
+  extern __shared__ uint4 copies[];
+  constexpr int kHeads = kForwardHeads<T>;
+  const Walk<T, LANES, INTERLEAVED, VECTOR, kHeads, 1> walk(p, smem_u32(copies));
+  const int role = walk.role;
+  const uint32_t rounds = walk.rounds();
+#pragma unroll
+  for (uint32_t round = 0; round < kStages - 1; ++round) {
+    walk.issue(round, 0, p.x[role], p.xs[role]);
+    cp_async_commit();
+  }
+  // Angles one round ahead, positions two.
+  Angles angles, next_angles;
+  int64_t position = 0;
+  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io.first_pair, next_angles);
+  if (walk.live(1)) position = load_position(p, walk.token(1));
+  float w[16];
   const bool norm = p.weight[role] != nullptr;
-  if (live) {
-    load_angles(p, batch, seq, io.first_pair, cosine, sine);
-    if (norm) io.weights(p.weight[role], p.weight_f32, p.vector_weight, w);
-  }
+  if (norm && walk.working) walk.io.weights(p.weight[role], p.weight_f32, p.vector_weight, w);
+
+  for (uint32_t round = 0; round < rounds; ++round) {
+    walk.issue(round + kStages - 1, 0, p.x[role], p.xs[role]);
+    cp_async_commit();
+    angles = next_angles;
+    if (walk.live(round + 1)) load_angles(p, position, walk.io.first_pair, next_angles);
+    if (walk.live(round + 2)) position = load_position(p, walk.token(round + 2));
+    cp_async_wait<kStages - 1>();
+    const bool live = walk.live(round);
+    T* y = static_cast<T*>(p.y[role]) + (static_cast<int64_t>(walk.token(round)) * p.heads[role] + walk.head0) * p.dim;
 #pragma unroll
-  for (int h = 0; h < kForwardHeads; ++h) {
-    const bool mine = live && head0 + h < p.heads[role];
-    float v[16];
-    if (mine) io.unpack(raw[h], v);
-    if (norm) {
-      float squares = 0.f;
-      if (mine) {
+    for (int h = 0; h < kHeads; ++h) {
+      const bool mine = live && h < walk.heads;
+      float v[16];
+      if (mine) walk.io.unpack(walk.head(round, 0, p.x[role], p.xs[role], h), v);
+      if (norm) {
+        float squares = 0.f;
+        if (mine) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) squares = fmaf(v[i], v[i], squares);
+          for (int i = 0; i < 16; ++i) squares = fmaf(v[i], v[i], squares);
+        }
+        const float r = rsqrtf(group_sum<LANES>(squares) * p.inv_dim + p.eps);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
       }
-      const float r = rsqrtf(group_sum<LANES>(squares) * p.inv_dim + p.eps);
+      if (!mine) continue;
+      float out[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
+      for (int i = 0; i < 8; ++i) {
+        out[i] = v[i] * angles.cosine[i] - v[8 + i] * angles.sine[i];
+        out[8 + i] = v[8 + i] * angles.cosine[i] + v[i] * angles.sine[i];
+      }
+      walk.io.store(y + h * p.dim, out);
     }
-    if (!mine) continue;
-    float out[16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      out[i] = v[i] * cosine[i] - v[8 + i] * sine[i];
-      out[8 + i] = v[8 + i] * cosine[i] + v[i] * sine[i];
-    }
-    io.store(y + (head0 + h) * p.dim, out);
   }
 }
 
-// A group keeps one chunk of heads and walks the tokens, so that a thread's
-// 16 weight gradients stay in registers for the whole launch; the block adds
-// its groups' sums in a fixed order and writes one partial per role.
+// As the forward pass, over x and dy; a thread's 16 weight gradients stay in
+// registers for the whole launch, the block adds its groups' sums in a fixed
+// order and writes one partial per role.
 template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
-__global__ void __launch_bounds__(kRotaryThreads, kBackwardBlocks) rotary_backward(RotaryParams p) {
-  constexpr int kGroups = kRotaryThreads / LANES;
-  __shared__ float sums[kRotaryThreads * 16];
-  const uint32_t group = blockIdx.x * kGroups + threadIdx.x / LANES;
-  const uint32_t walkers = gridDim.x * kGroups / p.chunks;
-  const uint32_t walker = group / p.chunks;
-  const uint32_t chunk = group - walker * p.chunks;
-  const HeadIO<T, INTERLEAVED, VECTOR> io(p, threadIdx.x % LANES);
-  const int role = chunk >= p.q_chunks;
-  const int head0 = static_cast<int>(chunk - (role ? p.q_chunks : 0)) * kBackwardHeads;
+__global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward(RotaryParams p) {
+  extern __shared__ uint4 copies[];
+  constexpr int kHeads = kBackwardHeads<T>;
+  using W = Walk<T, LANES, INTERLEAVED, VECTOR, kHeads, 2>;
+  const W walk(p, smem_u32(copies));
+  const int role = walk.role;
   const bool norm = p.weight[role] != nullptr;
-  const bool working = walker < walkers;
+  const uint32_t rounds = walk.rounds();
+  auto issue = [&](uint32_t round) {
+    walk.issue(round, 1, p.dy[role], p.dys[role]);
+    if (norm) walk.issue(round, 0, p.x[role], p.xs[role]);
+    cp_async_commit();
+  };
+#pragma unroll
+  for (uint32_t round = 0; round < kStages - 1; ++round) issue(round);
+  Angles angles, next_angles;
+  int64_t position = 0;
+  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io.first_pair, next_angles);
+  if (walk.live(1)) position = load_position(p, walk.token(1));
   float w[16], dw[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) dw[i] = 0.f, w[i] = 1.f;
-  if (norm && io.active) io.weights(p.weight[role], p.weight_f32, p.vector_weight, w);
+  if (norm && walk.working) walk.io.weights(p.weight[role], p.weight_f32, p.vector_weight, w);
 
-  // All lanes of a warp run the same number of rounds: the sums are exchanged
-  // by the whole warp.
-  const uint32_t rounds = (p.tokens + walkers - 1) / walkers;
   for (uint32_t round = 0; round < rounds; ++round) {
-    const uint32_t token = round * walkers + walker;
-    const bool live = working && token < p.tokens && io.active;
-    const int64_t batch = live ? token / p.sequence : 0, seq = live ? token % p.sequence : 0;
-    const T* x = static_cast<const T*>(p.x[role]) + batch * p.xs[role][0] + seq * p.xs[role][1];
-    const T* dy = static_cast<const T*>(p.dy[role]) + batch * p.dys[role][0] + seq * p.dys[role][1];
-    T* dx = static_cast<T*>(p.y[role]) + static_cast<int64_t>(token) * p.heads[role] * p.dim;
-    typename HeadIO<T, INTERLEAVED, VECTOR>::Raw rx[kBackwardHeads], rdy[kBackwardHeads];
+    issue(round + kStages - 1);
+    angles = next_angles;
+    if (walk.live(round + 1)) load_angles(p, position, walk.io.first_pair, next_angles);
+    if (walk.live(round + 2)) position = load_position(p, walk.token(round + 2));
+    cp_async_wait<kStages - 1>();
+    const bool live = walk.live(round);
+    T* dx = static_cast<T*>(p.y[role]) + (static_cast<int64_t>(walk.token(round)) * p.heads[role] + walk.head0) * p.dim;
 #pragma unroll
-    for (int h = 0; h < kBackwardHeads; ++h) {
-      if (!live || head0 + h >= p.heads[role]) continue;
-      rdy[h] = io.load(dy + (head0 + h) * p.dys[role][2]);
-      if (norm) rx[h] = io.load(x + (head0 + h) * p.xs[role][2]);
-    }
-    float cosine[8], sine[8];
-    if (live) load_angles(p, batch, seq, io.first_pair, cosine, sine);
-#pragma unroll
-    for (int h = 0; h < kBackwardHeads; ++h) {
-      const bool mine = live && head0 + h < p.heads[role];
+    for (int h = 0; h < kHeads; ++h) {
+      const bool mine = live && h < walk.heads;
       float v[16], g[16];
       if (mine) {
         float dv[16];
-        io.unpack(rdy[h], dv);
+        walk.io.unpack(walk.head(round, 1, p.dy[role], p.dys[role], h), dv);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          g[i] = dv[i] * cosine[i] + dv[8 + i] * sine[i];
-          g[8 + i] = dv[8 + i] * cosine[i] - dv[i] * sine[i];
+          g[i] = dv[i] * angles.cosine[i] + dv[8 + i] * angles.sine[i];
+          g[8 + i] = dv[8 + i] * angles.cosine[i] - dv[i] * angles.sine[i];
         }
       }
       if (norm) {
         float squares = 0.f, products = 0.f;
         if (mine) {
-          io.unpack(rx[h], v);
+          walk.io.unpack(walk.head(round, 0, p.x[role], p.xs[role], h), v);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             squares = fmaf(v[i], v[i], squares);
@@ -333,14 +417,18 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardBlocks) rotary_backwa
           }
         }
       }
-      if (mine) io.store(dx + (head0 + h) * p.dim, g);
+      if (mine) walk.io.store(dx + h * p.dim, g);
     }
   }
   if (p.partials == nullptr) return;
 
   // sums[group][16 * lane + i]: element order within a lane as in unpack().
+  // (The copies are all used: their place is free.)
+  constexpr int kGroups = W::kGroups;
+  float* sums = reinterpret_cast<float*>(copies);
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sums[threadIdx.x * 16 + i] = working ? dw[i] : 0.f;
+  for (int i = 0; i < 16; ++i) sums[threadIdx.x * 16 + i] = walk.working ? dw[i] : 0.f;
   __syncthreads();
   const uint32_t first_group = blockIdx.x * kGroups;
   for (int e = threadIdx.x; e < 2 * p.dim; e += kRotaryThreads) {
@@ -396,32 +484,40 @@ int lanes_for(int dim) {
   return lanes;
 }
 
-int backward_blocks(int64_t tokens, uint32_t chunks, int dim) {
+// Enough blocks for every (token, chunk), at most the resident ones, at least
+// one group per chunk.
+int rotary_blocks(int64_t tokens, uint32_t chunks, int dim) {
   const int groups = kRotaryThreads / lanes_for(dim);
-  // Enough blocks for every (token, chunk), at most 4 resident blocks per SM,
-  // at least one group per chunk.
   const int64_t wanted = ceil_div(tokens * chunks, groups);
   const int64_t least = ceil_div(chunks, groups);
-  return static_cast<int>(std::max(least, std::min<int64_t>(wanted, static_cast<int64_t>(sm_count()) * 4)));
+  return static_cast<int>(std::max(least, std::min<int64_t>(wanted, static_cast<int64_t>(sm_count()) * kRotaryBlocks)));
 }
 
 template <typename T, bool INTERLEAVED, bool VECTOR>
 int launch_rotary(const RotaryParams& p, bool backward, int blocks, cudaStream_t stream) {
-  auto run = [&](auto lanes) {
+  auto run = [&](auto lanes) -> int {
     constexpr int L = decltype(lanes)::value;
-    if (backward) rotary_backward<T, L, INTERLEAVED, VECTOR><<<blocks, kRotaryThreads, 0, stream>>>(p);
-    else rotary_forward<T, L, INTERLEAVED, VECTOR><<<blocks, kRotaryThreads, 0, stream>>>(p);
+    void (*kernel)(RotaryParams) = backward ? rotary_backward<T, L, INTERLEAVED, VECTOR> : rotary_forward<T, L, INTERLEAVED, VECTOR>;
+    constexpr int kForward = Walk<T, L, INTERLEAVED, VECTOR, kForwardHeads<T>, 1>::kStageBytes;
+    constexpr int kBackward = Walk<T, L, INTERLEAVED, VECTOR, kBackwardHeads<T>, 2>::kStageBytes;
+    constexpr int kSums = kRotaryThreads * 16 * 4;
+    // Without the copies only the weight gradients' sums need shared memory.
+    const int shared = VECTOR ? kStages * (backward ? kBackward : kForward) : backward ? kSums : 0;
+    if (shared > 48 * 1024) {
+      SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+    }
+    kernel<<<blocks, kRotaryThreads, shared, stream>>>(p);
+    SDC_CUDA_CHECK(cudaGetLastError());
+    return SDC_OK;
   };
   switch (lanes_for(p.dim)) {
-    case 1: run(std::integral_constant<int, 1>{}); break;
-    case 2: run(std::integral_constant<int, 2>{}); break;
-    case 4: run(std::integral_constant<int, 4>{}); break;
-    case 8: run(std::integral_constant<int, 8>{}); break;
-    case 16: run(std::integral_constant<int, 16>{}); break;
-    default: run(std::integral_constant<int, 32>{}); break;
+    case 1: return run(std::integral_constant<int, 1>{});
+    case 2: return run(std::integral_constant<int, 2>{});
+    case 4: return run(std::integral_constant<int, 4>{});
+    case 8: return run(std::integral_constant<int, 8>{});
+    case 16: return run(std::integral_constant<int, 16>{});
+    default: return run(std::integral_constant<int, 32>{});
   }
-  SDC_CUDA_CHECK(cudaGetLastError());
-  return SDC_OK;
 }
 
 int dispatch_rotary(const RotaryParams& p, int dtype, bool interleaved, bool vector, bool backward, int blocks,
@@ -517,20 +613,20 @@ int sdc_head_norm_rotary(int dtype, const void* q, const int64_t* q_strides, con
   RotaryParams p{};
   int rc = fill_params(p, dtype, q, q_strides, k, k_strides, batch, sequence, heads_q, heads_k, dim, table,
                        table_rows, rotary, positions, positions_64, position_strides, q_weight, k_weight, weight_f32,
-                       eps, q_out, k_out, kForwardHeads);
+                       eps, q_out, k_out, dtype == kF32 ? kForwardHeads<float> : kForwardHeads<__half>);
   if (rc != SDC_OK || batch == 0 || sequence == 0) return rc;
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
-  const int groups = kRotaryThreads / lanes_for(dim);
-  const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(p.tokens) * p.chunks, groups));
+  const int blocks = rotary_blocks(p.tokens, p.chunks, dim);
   return dispatch_rotary(p, dtype, interleaved != 0, vector_layout(p, dtype, interleaved != 0), false, blocks, stream);
 }
 
 size_t sdc_head_norm_rotary_workspace_bytes(int64_t batch, int64_t sequence, int heads_q, int heads_k, int dim) {
   using namespace sdc;
   if (batch <= 0 || sequence <= 0 || heads_q <= 0 || heads_k < 0 || dim < 2 || dim > kMaxHeadDim) return 0;
-  const uint32_t chunks = static_cast<uint32_t>(ceil_div(heads_q, kBackwardHeads) + ceil_div(heads_k, kBackwardHeads));
-  return static_cast<size_t>(backward_blocks(batch * sequence, chunks, dim)) * 2 * dim * sizeof(float);
+  // As many chunks as there are heads, the most that any type has.
+  const uint32_t chunks = static_cast<uint32_t>(heads_q + heads_k);
+  return static_cast<size_t>(rotary_blocks(batch * sequence, chunks, dim)) * 2 * dim * sizeof(float);
 }
 
 int sdc_head_norm_rotary_backward(int dtype, const void* dq_out, const int64_t* dq_strides, const void* dk_out,
@@ -545,7 +641,7 @@ int sdc_head_norm_rotary_backward(int dtype, const void* dq_out, const int64_t* 
   RotaryParams p{};
   int rc = fill_params(p, dtype, q, q_strides, k, k_strides, batch, sequence, heads_q, heads_k, dim, table,
                        table_rows, rotary, positions, positions_64, position_strides, q_weight, k_weight, weight_f32,
-                       eps, dq, dk, kBackwardHeads);
+                       eps, dq, dk, dtype == kF32 ? kBackwardHeads<float> : kBackwardHeads<__half>);
   if (rc != SDC_OK) return rc;
   const bool norm = q_weight != nullptr;
   SDC_REQUIRE(!norm || (dq_weight != nullptr && (heads_k == 0 || dk_weight != nullptr)),
@@ -562,7 +658,7 @@ int sdc_head_norm_rotary_backward(int dtype, const void* dq_out, const int64_t* 
       p.dys[0][i] = dq_strides[i];
       p.dys[1][i] = heads_k > 0 ? dk_strides[i] : 0;
     }
-    blocks = backward_blocks(p.tokens, p.chunks, dim);
+    blocks = rotary_blocks(p.tokens, p.chunks, dim);
     if (norm) {
       if (workspace == nullptr || workspace_bytes < static_cast<size_t>(blocks) * 2 * dim * sizeof(float)) {
         return fail(SDC_ERR_WORKSPACE, "head norm rotation workspace is missing or too small");
