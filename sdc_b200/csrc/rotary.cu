@@ -27,13 +27,10 @@ namespace sdc {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-// Heads of a group, by the type's size: two blocks share an SM's shared memory.
-template <typename T>
-constexpr int kForwardHeads = sizeof(T) == 2 ? 4 : 2;
-template <typename T>
-constexpr int kBackwardHeads = sizeof(T) == 2 ? 2 : 1;
 constexpr int kRotaryBlocks = 2;  // on an SM
-constexpr int kStages = 3;        // tokens of a group under way
+// Tokens of a group under way, by the 16-byte words that a thread copies of
+// one: two blocks share an SM's shared memory.
+constexpr int stages_for(int words) { return words >= 8 ? 3 : words >= 4 ? 5 : 8; }
 constexpr int kMaxHeadDim = 512;  // 32 lanes of 16 elements
 
 struct RotaryParams {
@@ -52,6 +49,7 @@ struct RotaryParams {
   uint32_t chunks;       // head chunks per token: q's, then k's
   uint32_t q_chunks;
   int heads[2];
+  int group_heads;       // heads of a group
   int dim, rotary;
   float eps, inv_dim;
   bool positions_64, weight_f32, vector_table, vector_weight;
@@ -64,60 +62,39 @@ __device__ __forceinline__ int64_t load_position(const RotaryParams& p, uint32_t
   return p.positions_64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
 }
 
-// The position's cosine and sine for this lane's 8 pairs; identity beyond the
-// rotary pairs. A position outside the table gives NaN, not a stray read.
-struct Angles {
-  float cosine[8], sine[8];
-};
-__device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t position, int first_pair, Angles& a) {
-  const int half = p.rotary / 2;
-  const bool inside = position >= 0 && position < p.table_rows;
-  const float* row = p.table + (inside ? position : 0) * p.rotary;
-  if (inside && p.vector_table && first_pair + 8 <= half) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 c = reinterpret_cast<const float4*>(row + first_pair)[i];
-      const float4 s = reinterpret_cast<const float4*>(row + half + first_pair)[i];
-      a.cosine[4 * i] = c.x, a.cosine[4 * i + 1] = c.y, a.cosine[4 * i + 2] = c.z, a.cosine[4 * i + 3] = c.w;
-      a.sine[4 * i] = s.x, a.sine[4 * i + 1] = s.y, a.sine[4 * i + 2] = s.z, a.sine[4 * i + 3] = s.w;
-    }
-    return;
-  }
-  const float nan = __int_as_float(0x7fffffff);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int pair = first_pair + i;
-    const bool turned = pair < half;
-    a.cosine[i] = turned ? (inside ? row[pair] : nan) : 1.f;
-    a.sine[i] = turned ? (inside ? row[half + pair] : nan) : 0.f;
-  }
-}
-
-// Where this lane's pairs lie in a head: member 0 and member 1 of pair i are
-// at first + i * step and second + i * step.
-struct PairLayout {
-  int first, second, step;
-};
-
 template <bool INTERLEAVED>
 __device__ __forceinline__ int element_of(int pair, int member, int rotary) {
   if (!INTERLEAVED && pair < rotary / 2) return pair + member * (rotary / 2);
   return 2 * pair + member;  // passing elements pair up in order as well
 }
 
-// v[i], v[8 + i]: members of pair i. VECTOR: the 8 pairs are two runs of 8
-// elements (half-split rotary pairs) or one run of 16.
+// v[i], v[8 + i]: members of this lane's pair i. VECTOR: the 8 pairs are two
+// runs of 8 elements, and neighbouring lanes' runs are neighbours: half-split
+// rotary pairs have their first members in one and their second in the other;
+// interleaved or passing pairs lie within a run, the lanes' first runs in the
+// first half of their part of the head, their second runs in the other.
 template <typename T, bool INTERLEAVED, bool VECTOR>
 struct HeadIO {
-  int first_pair, rotary, pairs;
+  int first_pair, rotary, pairs, low_run, high_run;
   bool active, split;
 
   __device__ __forceinline__ HeadIO(const RotaryParams& p, int lane)
       : first_pair(lane * 8), rotary(p.rotary), pairs(p.dim / 2), active(lane * 8 < p.dim / 2),
-        split(!INTERLEAVED && lane * 8 < p.rotary / 2) {}
-
-  __device__ __forceinline__ int low_run() const { return split ? first_pair : 2 * first_pair; }
-  __device__ __forceinline__ int high_run() const { return split ? first_pair + rotary / 2 : 2 * first_pair + 8; }
+        split(!INTERLEAVED && lane * 8 < p.rotary / 2) {
+    const int part = INTERLEAVED ? 0 : p.rotary;  // where interleaved or passing pairs begin
+    low_run = split ? first_pair : part + first_pair - part / 2;
+    high_run = split ? first_pair + rotary / 2 : low_run + (p.dim - part) / 2;
+  }
+  __device__ __forceinline__ int element(int i, int member) const {
+    if (!VECTOR) return element_of<INTERLEAVED>(first_pair + i, member, rotary);
+    if (split) return (member ? high_run : low_run) + i;
+    return (i < 4 ? low_run + 2 * i : high_run + 2 * (i - 4)) + member;
+  }
+  // Index of pair i's angle (rotary / 2 or more: none).
+  __device__ __forceinline__ int angle(int i) const {
+    if (!VECTOR || !INTERLEAVED) return first_pair + i;
+    return element(i, 0) / 2;
+  }
 
   struct Raw {
     Raw8<T> a, b;
@@ -125,8 +102,8 @@ struct HeadIO {
   __device__ __forceinline__ Raw load(const T* head) const {
     Raw r;
     if constexpr (VECTOR) {
-      r.a = load8(head + low_run());
-      r.b = load8(head + high_run());
+      r.a = load8(head + low_run);
+      r.b = load8(head + high_run);
     } else {
       T* a = reinterpret_cast<T*>(&r.a);
       T* b = reinterpret_cast<T*>(&r.b);
@@ -146,7 +123,7 @@ struct HeadIO {
   __device__ __forceinline__ void issue(const T* head, uint32_t at) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-      const T* run = head + (i < kWords / 2 ? low_run() : high_run());
+      const T* run = head + (i < kWords / 2 ? low_run : high_run);
       cp_async16(at + i * kRotaryThreads * 16, reinterpret_cast<const uint4*>(run) + i % (kWords / 2));
     }
   }
@@ -168,14 +145,14 @@ struct HeadIO {
     float a[8], b[8];
     unpack8(ra, a);
     unpack8(rb, b);
-    const bool runs = VECTOR && !split;  // 16 elements in order: even ones are the first members
+    const bool runs = !split;  // even elements are the first members
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (VECTOR) {
         const float e0 = i < 4 ? a[(2 * i) & 7] : b[(2 * i) & 7];
         const float e1 = i < 4 ? a[(2 * i + 1) & 7] : b[(2 * i + 1) & 7];
-        v[i] = INTERLEAVED || runs ? e0 : a[i];
-        v[8 + i] = INTERLEAVED || runs ? e1 : b[i];
+        v[i] = runs ? e0 : a[i];
+        v[8 + i] = runs ? e1 : b[i];
       } else {
         v[i] = a[i];
         v[8 + i] = b[i];
@@ -187,14 +164,14 @@ struct HeadIO {
       float a[8], b[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool runs = INTERLEAVED || !split;
+        const bool runs = !split;
         a[2 * i] = runs ? v[i] : v[2 * i];
         a[2 * i + 1] = runs ? v[8 + i] : v[2 * i + 1];
         b[2 * i] = runs ? v[4 + i] : v[8 + 2 * i];
         b[2 * i + 1] = runs ? v[12 + i] : v[8 + 2 * i + 1];
       }
-      store8(head + low_run(), pack8<T>(a));
-      store8(head + high_run(), pack8<T>(b));
+      store8(head + low_run, pack8<T>(a));
+      store8(head + high_run, pack8<T>(b));
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -210,7 +187,7 @@ struct HeadIO {
     if (VECTOR && vector) {
       if (f32) {
         const float* from = static_cast<const float*>(weight);
-        unpack_runs<float>(load8(from + low_run()), load8(from + high_run()), w);
+        unpack_runs<float>(load8(from + low_run), load8(from + high_run), w);
       } else {
         unpack(load(static_cast<const T*>(weight)), w);
       }
@@ -220,10 +197,9 @@ struct HeadIO {
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
       for (int member = 0; member < 2; ++member) {
-        const int pair = first_pair + i;
-        const int e = element_of<INTERLEAVED>(pair, member, rotary);
+        const int e = element(i, member);
         float value = 0.f;
-        if (pair < pairs) {
+        if (first_pair + i < pairs) {
           value = f32 ? static_cast<const float*>(weight)[e] : to_float(static_cast<const T*>(weight)[e]);
         }
         w[8 * member + i] = value;
@@ -231,6 +207,37 @@ struct HeadIO {
     }
   }
 };
+
+// The position's cosine and sine for this lane's 8 pairs; identity beyond the
+// rotary pairs. A position outside the table gives NaN, not a stray read.
+struct Angles {
+  float cosine[8], sine[8];
+};
+template <typename IO>
+__device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t position, const IO& io, Angles& a) {
+  const int half = p.rotary / 2;
+  const bool inside = position >= 0 && position < p.table_rows;
+  const float* row = p.table + (inside ? position : 0) * p.rotary;
+  const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const int first = io.angle(4 * part);
+    if (inside && p.vector_table && first + 4 <= half) {
+      const float4 c = *reinterpret_cast<const float4*>(row + first);
+      const float4 s = *reinterpret_cast<const float4*>(row + half + first);
+      a.cosine[4 * part] = c.x, a.cosine[4 * part + 1] = c.y, a.cosine[4 * part + 2] = c.z, a.cosine[4 * part + 3] = c.w;
+      a.sine[4 * part] = s.x, a.sine[4 * part + 1] = s.y, a.sine[4 * part + 2] = s.z, a.sine[4 * part + 3] = s.w;
+      continue;
+    }
+#pragma unroll
+    for (int i = 4 * part; i < 4 * part + 4; ++i) {
+      const int pair = io.angle(i);
+      const bool turned = pair < half;
+      a.cosine[i] = turned ? (inside ? row[pair] : nan) : 1.f;
+      a.sine[i] = turned ? (inside ? row[half + pair] : nan) : 0.f;
+    }
+  }
+}
 
 template <int LANES>
 __device__ __forceinline__ float group_sum(float x) {
@@ -246,6 +253,7 @@ template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int HEADS, int T
 struct Walk {
   using IO = HeadIO<T, INTERLEAVED, VECTOR>;
   static constexpr int kGroups = kRotaryThreads / LANES;
+  static constexpr int kStages = stages_for(TENSORS * HEADS * IO::kWords);
   static constexpr int kStageBytes = TENSORS * HEADS * IO::kWords * kRotaryThreads * 16;
   const RotaryParams& p;
   const IO io;
@@ -290,11 +298,12 @@ struct Walk {
   }
 };
 
-template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
+template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int kHeads>
 __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(RotaryParams p) {
   extern __shared__ uint4 copies[];
-  constexpr int kHeads = kForwardHeads<T>;
-  const Walk<T, LANES, INTERLEAVED, VECTOR, kHeads, 1> walk(p, smem_u32(copies));
+  using W = Walk<T, LANES, INTERLEAVED, VECTOR, kHeads, 1>;
+  constexpr int kStages = W::kStages;
+  const W walk(p, smem_u32(copies));
   const int role = walk.role;
   const uint32_t rounds = walk.rounds();
 #pragma unroll
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
   // Angles one round ahead, positions two.
   Angles angles, next_angles;
   int64_t position = 0;
-  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io.first_pair, next_angles);
+  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io, next_angles);
   if (walk.live(1)) position = load_position(p, walk.token(1));
   float w[16];
   const bool norm = p.weight[role] != nullptr;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
     walk.issue(round + kStages - 1, 0, p.x[role], p.xs[role]);
     cp_async_commit();
     angles = next_angles;
-    if (walk.live(round + 1)) load_angles(p, position, walk.io.first_pair, next_angles);
+    if (walk.live(round + 1)) load_angles(p, position, walk.io, next_angles);
     if (walk.live(round + 2)) position = load_position(p, walk.token(round + 2));
     cp_async_wait<kStages - 1>();
     const bool live = walk.live(round);
@@ -350,11 +359,11 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
 // As the forward pass, over x and dy; a thread's 16 weight gradients stay in
 // registers for the whole launch, the block adds its groups' sums in a fixed
 // order and writes one partial per role.
-template <typename T, int LANES, bool INTERLEAVED, bool VECTOR>
+template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int kHeads>
 __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward(RotaryParams p) {
   extern __shared__ uint4 copies[];
-  constexpr int kHeads = kBackwardHeads<T>;
   using W = Walk<T, LANES, INTERLEAVED, VECTOR, kHeads, 2>;
+  constexpr int kStages = W::kStages;
   const W walk(p, smem_u32(copies));
   const int role = walk.role;
   const bool norm = p.weight[role] != nullptr;
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
   for (uint32_t round = 0; round < kStages - 1; ++round) issue(round);
   Angles angles, next_angles;
   int64_t position = 0;
-  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io.first_pair, next_angles);
+  if (walk.live(0)) load_angles(p, load_position(p, walk.token(0)), walk.io, next_angles);
   if (walk.live(1)) position = load_position(p, walk.token(1));
   float w[16], dw[16];
 #pragma unroll
@@ -378,7 +387,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
   for (uint32_t round = 0; round < rounds; ++round) {
     issue(round + kStages - 1);
     angles = next_angles;
-    if (walk.live(round + 1)) load_angles(p, position, walk.io.first_pair, next_angles);
+    if (walk.live(round + 1)) load_angles(p, position, walk.io, next_angles);
     if (walk.live(round + 2)) position = load_position(p, walk.token(round + 2));
     cp_async_wait<kStages - 1>();
     const bool live = walk.live(round);
@@ -422,32 +431,25 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
   }
   if (p.partials == nullptr) return;
 
-  // sums[group][16 * lane + i]: element order within a lane as in unpack().
-  // (The copies are all used: their place is free.)
+  // sums[group][element] (the copies are all used: their place is free).
   constexpr int kGroups = W::kGroups;
   float* sums = reinterpret_cast<float*>(copies);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sums[threadIdx.x * 16 + i] = walk.working ? dw[i] : 0.f;
+  for (int i = 0; i < 16; ++i) {
+    if (walk.io.active && walk.io.first_pair + i % 8 < walk.io.pairs) {
+      sums[threadIdx.x / LANES * LANES * 16 + walk.io.element(i % 8, i / 8)] = walk.working ? dw[i] : 0.f;
+    }
+  }
   __syncthreads();
   const uint32_t first_group = blockIdx.x * kGroups;
   for (int e = threadIdx.x; e < 2 * p.dim; e += kRotaryThreads) {
     const int r = e >= p.dim;
     const int at = e - r * p.dim;
-    // Lane and slot that hold element `at`.
-    int pair, member;
-    if (!INTERLEAVED && at < p.rotary) {
-      member = at >= p.rotary / 2;
-      pair = at - member * (p.rotary / 2);
-    } else {
-      pair = at / 2;
-      member = at & 1;
-    }
-    const int slot = (pair / 8) * 16 + member * 8 + pair % 8;
     float total = 0.f;
     for (int g = 0; g < kGroups; ++g) {
       const uint32_t c = (first_group + g) % p.chunks;
-      if (static_cast<int>(c >= p.q_chunks) == r) total += sums[g * LANES * 16 + slot];
+      if (static_cast<int>(c >= p.q_chunks) == r) total += sums[g * LANES * 16 + at];
     }
     p.partials[static_cast<int64_t>(blockIdx.x) * 2 * p.dim + e] = total;
   }
@@ -493,16 +495,30 @@ int rotary_blocks(int64_t tokens, uint32_t chunks, int dim) {
   return static_cast<int>(std::max(least, std::min<int64_t>(wanted, static_cast<int64_t>(sm_count()) * kRotaryBlocks)));
 }
 
-template <typename T, bool INTERLEAVED, bool VECTOR>
-int launch_rotary(const RotaryParams& p, bool backward, int blocks, cudaStream_t stream) {
+// Heads of a group: as many as keep the copies within the shared memory, half
+// of that where groups would be left short by more than a tenth (14 + 2 heads
+// are four groups of 4, 4, 4, 2 and one of 2, but eight of 2).
+int heads_per_group(int dtype, int heads_q, int heads_k, bool backward) {
+  const int most = (dtype == kF32 ? 2 : 4) / (backward ? 2 : 1);
+  const int64_t places = (ceil_div(heads_q, most) + ceil_div(heads_k, most)) * most;
+  return most > 1 && 10 * (heads_q + heads_k) < 9 * places ? most / 2 : most;
+}
+
+template <typename T, bool INTERLEAVED, bool VECTOR, int HEADS>
+int launch_heads(const RotaryParams& p, bool backward, int blocks, cudaStream_t stream) {
   auto run = [&](auto lanes) -> int {
     constexpr int L = decltype(lanes)::value;
-    void (*kernel)(RotaryParams) = backward ? rotary_backward<T, L, INTERLEAVED, VECTOR> : rotary_forward<T, L, INTERLEAVED, VECTOR>;
-    constexpr int kForward = Walk<T, L, INTERLEAVED, VECTOR, kForwardHeads<T>, 1>::kStageBytes;
-    constexpr int kBackward = Walk<T, L, INTERLEAVED, VECTOR, kBackwardHeads<T>, 2>::kStageBytes;
+    // HEADS counts forward; the backward pass copies twice as much a head.
+    constexpr int kBackHeads = HEADS > 1 ? HEADS / 2 : 1;
+    using Forward = Walk<T, L, INTERLEAVED, VECTOR, HEADS, 1>;
+    using Backward = Walk<T, L, INTERLEAVED, VECTOR, kBackHeads, 2>;
+    void (*kernel)(RotaryParams) =
+        backward ? rotary_backward<T, L, INTERLEAVED, VECTOR, kBackHeads> : rotary_forward<T, L, INTERLEAVED, VECTOR, HEADS>;
     constexpr int kSums = kRotaryThreads * 16 * 4;
     // Without the copies only the weight gradients' sums need shared memory.
-    const int shared = VECTOR ? kStages * (backward ? kBackward : kForward) : backward ? kSums : 0;
+    const int shared = VECTOR ? (backward ? std::max(Backward::kStages * Backward::kStageBytes, kSums)
+                                          : Forward::kStages * Forward::kStageBytes)
+                              : backward ? kSums : 0;
     if (shared > 48 * 1024) {
       SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
     }
@@ -518,6 +534,15 @@ int launch_rotary(const RotaryParams& p, bool backward, int blocks, cudaStream_t
     case 16: return run(std::integral_constant<int, 16>{});
     default: return run(std::integral_constant<int, 32>{});
   }
+}
+
+template <typename T, bool INTERLEAVED, bool VECTOR>
+int launch_rotary(const RotaryParams& p, bool backward, int blocks, cudaStream_t stream) {
+  constexpr int kMost = sizeof(T) == 2 ? 4 : 2;
+  if (p.group_heads * (backward ? 2 : 1) == kMost) {
+    return launch_heads<T, INTERLEAVED, VECTOR, kMost>(p, backward, blocks, stream);
+  }
+  return launch_heads<T, INTERLEAVED, VECTOR, kMost / 2>(p, backward, blocks, stream);
 }
 
 int dispatch_rotary(const RotaryParams& p, int dtype, bool interleaved, bool vector, bool backward, int blocks,
@@ -545,7 +570,7 @@ int fill_params(RotaryParams& p, int dtype, const void* q, const int64_t* q_stri
                 const int64_t* k_strides, int64_t batch, int64_t sequence, int heads_q, int heads_k, int dim,
                 const float* table, int64_t table_rows, int rotary, const void* positions, int positions_64,
                 const int64_t* position_strides, const void* q_weight, const void* k_weight, int weight_f32,
-                float eps, void* q_out, void* k_out, int heads_per_group) {
+                float eps, void* q_out, void* k_out, bool backward) {
   SDC_REQUIRE(dtype == kF32 || dtype == kBF16 || dtype == kF16,
               "head norm rotation takes FP32 (0), BF16 (1) or FP16 (2) heads");
   SDC_REQUIRE(batch >= 0 && sequence >= 0 && heads_q > 0 && heads_k >= 0, "head norm rotation sizes must not be negative and q needs a head");
@@ -573,6 +598,7 @@ int fill_params(RotaryParams& p, int dtype, const void* q, const int64_t* q_stri
   p.sequence = static_cast<uint32_t>(sequence);
   p.tokens = static_cast<uint32_t>(batch * sequence);
   p.heads[0] = heads_q, p.heads[1] = heads_k;
+  const int heads_per_group = p.group_heads = sdc::heads_per_group(dtype, heads_q, heads_k, backward);
   p.q_chunks = static_cast<uint32_t>(ceil_div(heads_q, heads_per_group));
   p.chunks = p.q_chunks + static_cast<uint32_t>(ceil_div(heads_k, heads_per_group));
   SDC_REQUIRE(static_cast<int64_t>(p.tokens) * p.chunks < INT_MAX - 512,
@@ -613,7 +639,7 @@ int sdc_head_norm_rotary(int dtype, const void* q, const int64_t* q_strides, con
   RotaryParams p{};
   int rc = fill_params(p, dtype, q, q_strides, k, k_strides, batch, sequence, heads_q, heads_k, dim, table,
                        table_rows, rotary, positions, positions_64, position_strides, q_weight, k_weight, weight_f32,
-                       eps, q_out, k_out, dtype == kF32 ? kForwardHeads<float> : kForwardHeads<__half>);
+                       eps, q_out, k_out, false);
   if (rc != SDC_OK || batch == 0 || sequence == 0) return rc;
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
@@ -641,7 +667,7 @@ int sdc_head_norm_rotary_backward(int dtype, const void* dq_out, const int64_t* 
   RotaryParams p{};
   int rc = fill_params(p, dtype, q, q_strides, k, k_strides, batch, sequence, heads_q, heads_k, dim, table,
                        table_rows, rotary, positions, positions_64, position_strides, q_weight, k_weight, weight_f32,
-                       eps, dq, dk, dtype == kF32 ? kBackwardHeads<float> : kBackwardHeads<__half>);
+                       eps, dq, dk, true);
   if (rc != SDC_OK) return rc;
   const bool norm = q_weight != nullptr;
   SDC_REQUIRE(!norm || (dq_weight != nullptr && (heads_k == 0 || dk_weight != nullptr)),
