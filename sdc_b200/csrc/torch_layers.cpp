@@ -6,6 +6,7 @@
 // derivatives are registered here as well: a training step's small layers
 // are bound by the host, and a C++ node costs a fraction of a Python one.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -41,7 +42,11 @@ void check_cuda(const Tensor& t, const Tensor& like, const char* what) {
               " must be a strided CUDA tensor on the operand device");
 }
 
-bool unit_rows(const Tensor& t) { return t.numel() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1; }
+// Rows of contiguous elements (any row stride).
+bool unit_rows(const Tensor& t) { return t.dim() == 0 || t.numel() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1; }
+// The tensorwise FP8 projections' outputs, and what is computed from them, are
+// column-major: copied to rows before a kernel that streams rows.
+Tensor as_rows(const Tensor& t) { return unit_rows(t) ? t : t.contiguous(); }
 const void* data_of(OptTensor t) { return t.has_value() ? t->const_data_ptr() : nullptr; }
 
 // ------------------------------------------------- head norm and rotation ----
@@ -55,7 +60,6 @@ struct Heads {
 // [tokens, heads, dim] or [batch, sequence, heads, dim] with a unit last stride.
 Heads heads_of(const Tensor& t, const char* what) {
   TORCH_CHECK(t.dim() == 3 || t.dim() == 4, what, " must be [tokens, heads, dim] or [batch, sequence, heads, dim]");
-  TORCH_CHECK(unit_rows(t), what, " must have contiguous heads (unit last stride)");
   const bool batched = t.dim() == 4;
   TORCH_CHECK(t.size(-1) <= 512 && t.size(-2) <= std::numeric_limits<int>::max() / 512, what,
               " has too large heads or too many of them");
@@ -111,9 +115,10 @@ RotaryArgs check_rotary(const Tensor& q, const Tensor& k, const Tensor& table, c
   return a;
 }
 
-std::tuple<Tensor, Tensor> head_norm_rotary(const Tensor& q, const Tensor& k, const Tensor& table,
+std::tuple<Tensor, Tensor> head_norm_rotary(const Tensor& q_in, const Tensor& k_in, const Tensor& table,
                                             const Tensor& positions, OptTensor q_weight, OptTensor k_weight,
                                             double eps, bool interleaved) {
+  const Tensor q = as_rows(q_in), k = as_rows(k_in);
   const RotaryArgs a = check_rotary(q, k, table, positions, q_weight, k_weight);
   const c10::cuda::CUDAGuard guard(q.device());
   auto q_out = at::empty(q.sizes(), q.options());
@@ -127,8 +132,9 @@ std::tuple<Tensor, Tensor> head_norm_rotary(const Tensor& q, const Tensor& k, co
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rotary_backward(
-    const Tensor& dq_out, const Tensor& dk_out, const Tensor& q, const Tensor& k, const Tensor& table,
+    const Tensor& dq_in, const Tensor& dk_in, const Tensor& q_in, const Tensor& k_in, const Tensor& table,
     const Tensor& positions, OptTensor q_weight, OptTensor k_weight, double eps, bool interleaved) {
+  const Tensor q = as_rows(q_in), k = as_rows(k_in), dq_out = as_rows(dq_in), dk_out = as_rows(dk_in);
   const RotaryArgs a = check_rotary(q, k, table, positions, q_weight, k_weight);
   check_cuda(dq_out, q, "gradients");
   check_cuda(dk_out, q, "gradients");
@@ -171,8 +177,7 @@ struct AdapterArgs {
 
 void check_matrix(const Tensor& t, const Tensor& like, int64_t rows, int64_t columns, const char* what) {
   check_cuda(t, like, what);
-  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == columns && unit_rows(t), what, " must be [", rows, ", ",
-              columns, "] with contiguous rows");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == columns, what, " must be [", rows, ", ", columns, "]");
   TORCH_CHECK(t.scalar_type() == like.scalar_type(), what, " must have the adapters' dtype");
 }
 
@@ -194,7 +199,6 @@ AdapterArgs check_adapters(const Tensor& x, const Tensor& a, const Tensor& b, Op
               "adapter weights must be [adapters, rank, in] and [adapters, out, rank]");
   TORCH_CHECK(a.size(0) >= 1 && a.size(0) <= 65535 && a.size(1) >= 1 && a.size(1) <= 256,
               "low-rank adapters take 1 to 65535 adapters of rank 1 to 256");
-  TORCH_CHECK(unit_rows(x), "adapter input must have contiguous rows");
   if (scale.has_value()) {
     check_cuda(*scale, x, "adapter scales");
     TORCH_CHECK(scale->scalar_type() == at::kFloat && scale->dim() == 1 && scale->size(0) == a.size(0) &&
@@ -239,12 +243,14 @@ void run_expand(const AdapterArgs& s, const void* base, int64_t base_stride, con
 }
 
 // The adapters' sum with base, and the low-rank rows that the backward pass reads.
-std::tuple<Tensor, Tensor> low_rank_adapters(const Tensor& base, const Tensor& x, const Tensor& a, const Tensor& b,
-                                             OptTensor scale, const Tensor& rows, const Tensor& groups,
-                                             const Tensor& tiles, int64_t slots, int64_t active, int64_t tile_rows) {
-  const AdapterArgs s = check_adapters(x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
-  check_matrix(base, x, s.tokens, s.n, "the projection's output");
-  const c10::cuda::CUDAGuard guard(x.device());
+std::tuple<Tensor, Tensor> low_rank_adapters(const Tensor& base_in, const Tensor& x_in, const Tensor& a,
+                                             const Tensor& b, OptTensor scale, const Tensor& rows,
+                                             const Tensor& groups, const Tensor& tiles, int64_t slots, int64_t active,
+                                             int64_t tile_rows) {
+  const AdapterArgs s = check_adapters(x_in, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+  check_matrix(base_in, x_in, s.tokens, s.n, "the projection's output");
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor base = as_rows(base_in), x = as_rows(x_in);
   Tensor low = low_rows(x, s);
   Tensor out = at::empty({s.tokens, s.n}, x.options());
   if (s.tokens == 0 || s.n == 0) return {out, low};
@@ -254,13 +260,20 @@ std::tuple<Tensor, Tensor> low_rank_adapters(const Tensor& base, const Tensor& x
 }
 
 // The same, added to the projection's output in place: rows without an adapter are not touched.
-Tensor low_rank_adapters_(Tensor& base, const Tensor& x, const Tensor& a, const Tensor& b, OptTensor scale,
+Tensor low_rank_adapters_(Tensor& base, const Tensor& x_in, const Tensor& a, const Tensor& b, OptTensor scale,
                           const Tensor& rows, const Tensor& groups, const Tensor& tiles, int64_t slots, int64_t active,
                           int64_t tile_rows) {
-  const AdapterArgs s = check_adapters(x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
-  check_matrix(base, x, s.tokens, s.n, "the projection's output");
+  const AdapterArgs s = check_adapters(x_in, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+  check_matrix(base, x_in, s.tokens, s.n, "the projection's output");
+  at::assert_no_internal_overlap(base);
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  if (!unit_rows(base)) {
+    auto [out, low] = low_rank_adapters(base, x_in, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+    base.copy_(out);
+    return low;
+  }
   TORCH_CHECK(s.tokens <= 1 || base.stride(0) >= s.n, "the projection's output must not overlap itself");
-  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor x = as_rows(x_in);
   Tensor low = low_rows(x, s);
   if (s.tokens == 0 || s.n == 0) return low;
   run_shrink(s, x, rows, tiles, a, s.k, false, scale, low);
@@ -269,17 +282,18 @@ Tensor low_rank_adapters_(Tensor& base, const Tensor& x, const Tensor& a, const 
 }
 
 std::tuple<Tensor, Tensor, Tensor> low_rank_adapters_backward(
-    const Tensor& grad, const Tensor& x, const Tensor& a, const Tensor& b, OptTensor scale, const Tensor& low,
+    const Tensor& grad_in, const Tensor& x_in, const Tensor& a, const Tensor& b, OptTensor scale, const Tensor& low,
     const Tensor& rows, const Tensor& groups, const Tensor& tiles, int64_t slots, int64_t active, int64_t tile_rows,
     bool need_x, bool need_a, bool need_b) {
-  const AdapterArgs s = check_adapters(x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
-  check_matrix(grad, x, s.tokens, s.n, "the output's gradient");
-  check_cuda(low, x, "the low-rank rows");
+  const AdapterArgs s = check_adapters(x_in, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+  check_matrix(grad_in, x_in, s.tokens, s.n, "the output's gradient");
+  check_cuda(low, x_in, "the low-rank rows");
   const int64_t padded = (s.rank + 15) / 16 * 16;
-  TORCH_CHECK(low.scalar_type() == x.scalar_type() && low.is_contiguous() && low.dim() == 3 && low.size(0) == 2 &&
+  TORCH_CHECK(low.scalar_type() == x_in.scalar_type() && low.is_contiguous() && low.dim() == 3 && low.size(0) == 2 &&
                   low.size(1) == s.slots && low.size(2) == padded,
               "the low-rank rows must be those of the forward pass");
-  const c10::cuda::CUDAGuard guard(x.device());
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor grad = as_rows(grad_in), x = as_rows(x_in);
   Tensor dx = at::empty({need_x ? s.tokens : 0, s.k}, x.options());
   Tensor da = need_a ? at::empty_like(a) : at::empty({0}, a.options());
   Tensor db = need_b ? at::empty_like(b) : at::empty({0}, b.options());
@@ -311,7 +325,7 @@ struct DistillArgs {
 DistillArgs check_distill(const Tensor& logits, const Tensor& indices, const Tensor& teacher) {
   TORCH_CHECK(logits.is_cuda() && logits.layout() == at::kStrided && logits.dim() == 2,
               "student logits must be a CUDA matrix [rows, vocabulary]");
-  TORCH_CHECK(logits.size(1) > 0 && unit_rows(logits), "student logits must have contiguous, nonempty rows");
+  TORCH_CHECK(logits.size(1) > 0, "student logits must have a vocabulary");
   check_cuda(indices, logits, "teacher indices");
   check_cuda(teacher, logits, "teacher logits");
   TORCH_CHECK(indices.scalar_type() == at::kInt || indices.scalar_type() == at::kLong,
@@ -319,15 +333,15 @@ DistillArgs check_distill(const Tensor& logits, const Tensor& indices, const Ten
   TORCH_CHECK(indices.dim() == 2 && indices.size(0) == logits.size(0) && indices.size(1) >= 1 &&
                   indices.size(1) <= 1024 && teacher.sizes() == indices.sizes(),
               "teacher indices and logits must be [rows, top] with top from 1 to 1024");
-  TORCH_CHECK(unit_rows(indices) && unit_rows(teacher), "teacher indices and logits must have contiguous rows");
   return {element_type(logits, "student logits"), element_type(teacher, "teacher logits"),
           static_cast<int>(indices.size(1)), logits.size(0), logits.size(1)};
 }
 
-std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits, const Tensor& indices, const Tensor& teacher,
+std::tuple<Tensor, Tensor> distill_loss(const Tensor& logits_in, const Tensor& indices_in, const Tensor& teacher_in,
                                         double temperature) {
-  const DistillArgs a = check_distill(logits, indices, teacher);
-  const c10::cuda::CUDAGuard guard(logits.device());
+  const DistillArgs a = check_distill(logits_in, indices_in, teacher_in);
+  const c10::cuda::CUDAGuard guard(logits_in.device());
+  const Tensor logits = as_rows(logits_in), indices = as_rows(indices_in), teacher = as_rows(teacher_in);
   auto loss = at::empty({a.rows}, logits.options().dtype(at::kFloat));
   auto stats = at::empty({a.rows, 4}, loss.options());
   check_status(sdc_distill_loss(a.dtype, logits.const_data_ptr(), a.rows, a.vocab, logits.stride(0),
@@ -362,9 +376,11 @@ int64_t upstream_stride(OptTensor grad_loss, const Tensor& logits) {
   return grad_loss->stride(0);
 }
 
-Tensor distill_backward(const Tensor& logits, const Tensor& indices, const Tensor& teacher, double temperature,
-                        const Tensor& stats, OptTensor grad_loss, OptTensor grad_scale) {
-  const DistillArgs a = check_distill(logits, indices, teacher);
+Tensor distill_backward(const Tensor& logits_in, const Tensor& indices_in, const Tensor& teacher_in,
+                        double temperature, const Tensor& stats, OptTensor grad_loss, OptTensor grad_scale) {
+  const DistillArgs a = check_distill(logits_in, indices_in, teacher_in);
+  const c10::cuda::CUDAGuard guard(logits_in.device());
+  const Tensor logits = as_rows(logits_in), indices = as_rows(indices_in), teacher = as_rows(teacher_in);
   check_cuda(stats, logits, "distillation statistics");
   TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == a.rows && stats.size(1) == 4 &&
                   stats.is_contiguous(),
@@ -374,7 +390,6 @@ Tensor distill_backward(const Tensor& logits, const Tensor& indices, const Tenso
     check_cuda(*grad_scale, logits, "the loss scale");
     TORCH_CHECK(grad_scale->scalar_type() == at::kFloat && grad_scale->numel() == 1, "the loss scale must be one FP32 value");
   }
-  const c10::cuda::CUDAGuard guard(logits.device());
   auto grad = at::empty({a.rows, a.vocab}, logits.options());
   check_status(sdc_distill_backward(
       a.dtype, logits.const_data_ptr(), a.rows, a.vocab, logits.stride(0), indices.const_data_ptr(),
@@ -385,9 +400,10 @@ Tensor distill_backward(const Tensor& logits, const Tensor& indices, const Tenso
   return grad;
 }
 
-Tensor loss_and_grad_into(const Tensor& logits, const Tensor& indices, const Tensor& teacher, double temperature,
+Tensor loss_and_grad_into(const Tensor& logits, const Tensor& indices_in, const Tensor& teacher_in, double temperature,
                           OptTensor grad_loss, Tensor& grad) {
-  const DistillArgs a = check_distill(logits, indices, teacher);
+  const DistillArgs a = check_distill(logits, indices_in, teacher_in);
+  const Tensor indices = as_rows(indices_in), teacher = as_rows(teacher_in);
   const int64_t stride = upstream_stride(grad_loss, logits);
   auto loss = at::empty({a.rows}, logits.options().dtype(at::kFloat));
   auto stats = at::empty({a.rows, 4}, loss.options());
@@ -404,7 +420,7 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
   check_distill(logits, indices, teacher);
   const c10::cuda::CUDAGuard guard(logits.device());
   auto grad = at::empty({logits.size(0), logits.size(1)}, logits.options());
-  auto loss = loss_and_grad_into(logits, indices, teacher, temperature, grad_loss, grad);
+  auto loss = loss_and_grad_into(as_rows(logits), indices, teacher, temperature, grad_loss, grad);
   return {loss, grad};
 }
 
@@ -412,6 +428,7 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
 Tensor distill_loss_and_grad_(Tensor& logits, const Tensor& indices, const Tensor& teacher, double temperature,
                               OptTensor grad_loss) {
   check_distill(logits, indices, teacher);
+  TORCH_CHECK(unit_rows(logits), "student logits must have contiguous rows to be replaced in place");
   TORCH_CHECK(logits.size(0) <= 1 || logits.stride(0) >= logits.size(1), "student logits must not overlap themselves");
   const c10::cuda::CUDAGuard guard(logits.device());
   return loss_and_grad_into(logits, indices, teacher, temperature, grad_loss, logits);
@@ -426,7 +443,6 @@ using torch::autograd::variable_list;
 std::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 Tensor tensor_of(OptTensor t) { return t.has_value() ? *t : Tensor(); }
 bool differentiates(OptTensor t) { return t.has_value() && t->requires_grad(); }
-Tensor unit_gradient(const Tensor& g) { return unit_rows(g) ? g : g.contiguous(); }
 
 // The backward kernels have no derivatives: a second differentiation raises.
 variable_list once_differentiable(variable_list grads) {
@@ -460,7 +476,7 @@ struct HeadNormRotary : torch::autograd::Function<HeadNormRotary> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       for (int i = 0; i < 2; ++i) {  // an output that was not used
-        grads[i] = grads[i].defined() ? unit_gradient(grads[i]) : at::zeros(saved[i].sizes(), saved[i].options());
+        grads[i] = grads[i].defined() ? grads[i] : at::zeros(saved[i].sizes(), saved[i].options());
       }
       auto [dq, dk, dq_weight, dk_weight] = head_norm_rotary_backward(
           grads[0], grads[1], saved[0], saved[1], saved[2], saved[3], optional_of(saved[4]), optional_of(saved[5]),
@@ -517,7 +533,7 @@ struct LowRankAdapters : torch::autograd::Function<LowRankAdapters> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       auto [dx, da, db] = low_rank_adapters_backward(
-          unit_gradient(grads[0]), saved[0], saved[1], saved[2], optional_of(saved[3]), saved[4], saved[5], saved[6],
+          grads[0], saved[0], saved[1], saved[2], optional_of(saved[3]), saved[4], saved[5], saved[6],
           saved[7], ctx->saved_data["slots"].toInt(), ctx->saved_data["active"].toInt(),
           ctx->saved_data["tile_rows"].toInt(), need_x, need_a, need_b);
       if (need_x) out[1] = dx;

@@ -84,7 +84,8 @@ def low_rank_adapters(base, x, a, b, batch, scale=None):
     """``base + scale[g] * (x a[g]^T) b[g]^T`` with each token's adapter ``g``.
 
     ``base`` ``[tokens, out]``: the shared projection's output; ``x``
-    ``[tokens, in]``: its input (bf16 or fp16, contiguous rows); ``a``
+    ``[tokens, in]``: its input (bf16 or fp16, any row stride; a column-major
+    tensor, like the FP8 projections' outputs, is copied to rows first); ``a``
     ``[count, rank, in]`` and ``b`` ``[count, out, rank]``: contiguous weights
     of the same dtype, rank up to 256 (adapters of lower rank are padded with
     zeros); ``scale`` fp32 ``[count]``, 1 when None; ``batch``: an

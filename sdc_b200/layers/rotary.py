@@ -25,7 +25,8 @@ def head_norm_rotary(q, k, table, positions, q_weight=None, k_weight=None, eps=1
     both with a leading batch dimension (fp32, bf16 or fp16; any strides with
     contiguous heads, so views of a fused QKV projection and
     ``[batch, heads, sequence, dim]`` tensors transposed to this order need no
-    copy); ``dim`` even and at most 512. ``positions`` int32 or int64
+    copy; others are copied first); ``dim`` even and at most 512.
+    ``positions`` int32 or int64
     ``[tokens]``, or ``[sequence]`` or ``[batch, sequence]``; ``table`` from
     ``rotary_table``, whose width is the rotated part of a head: pairs
     ``(i, i + rotary/2)``, or ``(2i, 2i + 1)`` when ``interleaved``. With

@@ -146,6 +146,10 @@ def test_head_norm_rotary_takes_any_strides_and_alignment():
         odd.copy_(q)
         for a, b in zip(head_norm_rotary(odd, k, table, positions), want):
             assert torch.equal(a, b)
+        # Heads whose elements are apart.
+        apart = q.transpose(2, 3).contiguous().transpose(2, 3)
+        for a, b in zip(head_norm_rotary(apart, k, table, positions), want):
+            assert torch.equal(a, b)
         # A broadcast gradient (zero strides), and an output that is not used.
         leaf = q.contiguous().requires_grad_()
         out = head_norm_rotary(leaf, k, table, positions)
@@ -323,6 +327,26 @@ def test_low_rank_adapters_take_strided_rows_and_no_scale():
             rest = torch.ones(192 + pad + shift, dtype=torch.bool, device=DEV)
             rest[shift:shift + 192] = False
             assert not wide_base[:, rest].any()
+
+
+def test_low_rank_adapters_take_column_major_operands():
+    """The FP8 projections' outputs are column-major, and so is what is computed from them."""
+    case = ([40, 9], [1, 0], 2, 16, 128, 192)
+    x, base, a, b, scale, batch = _adapter_inputs(case, torch.bfloat16)
+    grad = normal(rng(2), 49, 192, dtype=torch.bfloat16)
+
+    def results(x, base, grad):
+        leaves = [t.detach().requires_grad_() for t in (x, a, b)]
+        out = low_rank_adapters(base, *leaves, batch, scale)
+        return (out, *torch.autograd.grad(out, leaves, grad))
+
+    columns = [t.t().contiguous().t() for t in (x, base, grad)]
+    for got, want in zip(results(*columns), results(x, base, grad)):
+        assert torch.equal(got, want)
+    in_place = columns[1].clone(memory_format=torch.preserve_format)
+    assert in_place.stride() == columns[1].stride()
+    low_rank_adapters_(in_place, columns[0], a, b, batch, scale)
+    assert torch.equal(in_place, low_rank_adapters(base, x, a, b, batch, scale))
 
 
 def test_low_rank_adapters_keep_foreign_values_out():
@@ -577,6 +601,13 @@ def test_distillation_of_rows_masked_throughout(dtype):
 def test_distillation_shapes_types_and_no_rows():
     logits, indices, teacher = _distill_inputs(6, 500, 8, torch.bfloat16)
     flat = distillation_loss_and_grad(logits, indices, teacher)
+    columns = [t.t().contiguous().t() for t in (logits, indices, teacher)]
+    for got, want in zip(distillation_loss_and_grad(*columns), flat):
+        assert torch.equal(got, want)
+    leaf = columns[0].requires_grad_()
+    (grad,) = torch.autograd.grad(distillation_loss(leaf, *columns[1:], reduction="sum"), leaf)
+    _, _, grad64, q, p = distill64(logits, indices, teacher, 1.0)
+    close(grad, grad64, q + p, 2.0 ** -17)
     loss, grad = distillation_loss_and_grad(logits.view(2, 3, 500), indices.view(2, 3, 8), teacher.view(2, 3, 8),
                                             grad_loss=torch.ones(2, 3, device=DEV))
     assert torch.equal(loss.view(-1), flat[0]) and torch.equal(grad.view(6, 500), flat[1])
@@ -686,8 +717,6 @@ def test_refusals():
         head_norm_rotary(q, k, table, positions.float())
     with pytest.raises(RuntimeError, match="agree in tokens"):
         head_norm_rotary(q, k[:3], table, positions)
-    with pytest.raises(RuntimeError, match="contiguous heads"):
-        head_norm_rotary(q.transpose(1, 2).contiguous().transpose(1, 2), k, table, positions)
     with pytest.raises(RuntimeError, match="both q and k"):
         head_norm_rotary(q, k, table, positions, w)
     with pytest.raises(RuntimeError, match=r"\[dim\]"):
@@ -714,7 +743,7 @@ def test_refusals():
         low_rank_adapters(base, x, a, b, batch, scale.half())
     with pytest.raises(RuntimeError, match="projection's output"):
         low_rank_adapters(base[:, 1:], x, a, b, batch, scale)
-    with pytest.raises(RuntimeError, match="overlap"):
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
         low_rank_adapters_(base[:1].expand(5, -1), x, a, b, batch, scale)
     with pytest.raises(ValueError, match="AdapterBatch"):
         low_rank_adapters(base, x, a, b, None, scale)
@@ -735,7 +764,7 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="FP32, BF16 or FP16"):
         distillation_loss(logits.double(), indices, teacher)
     with pytest.raises(RuntimeError, match="contiguous"):
-        distillation_loss(logits.t().contiguous().t(), indices, teacher)
+        distillation_loss_and_grad(logits.t().contiguous().t(), indices, teacher, in_place=True)
     with pytest.raises(RuntimeError, match="overlap"):
         distillation_loss_and_grad(logits[:1].expand(3, -1), indices, teacher, in_place=True)
     with pytest.raises(RuntimeError, match="loss gradient"):
