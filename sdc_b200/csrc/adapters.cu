@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "mma.cuh"
 
@@ -65,6 +66,7 @@ struct AdapterParams {
   int64_t out_stride;        // expand: row; outer: column
   int64_t out_rank_stride;   // outer
   int chunks_per_split;
+  int32_t* watchdog;
   int tile_count, tiles_per_block;  // expand
   int piece_bits;            // expand: 2^piece_bits >= rank_pad / 8 threads copy a row
 };
@@ -76,25 +78,53 @@ __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot
 
 // ------------------------------------------------------------------ shrink ----
 
-// ROWS kWide: eight warps of 16 rows; ROWS kNarrow: four warps share the rows and take
-// a quarter of each chunk of the width. RANK: columns of `low` per block.
-template <int ROWS, int RANK, bool TRANS>
-struct ShrinkShape {
-  static constexpr int kThreads = ROWS == kWide ? 256 : 128;
-  static constexpr int kChunk = ROWS == kWide ? 64 : 256;
+// A sum's two planes: hi = round(v), lo = round(v - hi).
+template <typename T>
+__device__ __forceinline__ void store_planes(const AdapterParams& p, int64_t slot, int rank, float v) {
+  T* high = static_cast<T*>(p.low) + slot * p.rank_pad + rank;
+  const T hi = from_float<T>(v);
+  const float rest = v - to_float(hi);
+  high[0] = hi;
+  high[p.slots * p.rank_pad] = from_float<T>(isfinite(rest) ? rest : 0.f);  // an infinite sum stays one
+}
+
+template <typename T>
+__device__ __forceinline__ void store_planes4(const AdapterParams& p, int64_t slot, int rank, float4 v) {
+  const float e[4] = {v.x, v.y, v.z, v.w};
+  float hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = to_float(from_float<T>(e[i]));
+    const float rest = e[i] - hi[i];
+    lo[i] = isfinite(rest) ? rest : 0.f;
+  }
+  T* to = static_cast<T*>(p.low) + slot * p.rank_pad + rank;  // rank and rank_pad are multiples of 4: 8-byte words
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]));
+  *reinterpret_cast<uint2*>(to + p.slots * p.rank_pad) = make_uint2(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]));
+}
+
+// Tiles of 16 rows (decoding): the weight is the traffic, and the tensor
+// memory's 128 rows would be empty. Four warps share the rows and take a
+// quarter of each chunk of the width. RANK: columns of `low` per block.
+template <int RANK, bool TRANS>
+struct NarrowShape {
+  static constexpr int ROWS = kNarrow;
+  static constexpr int kThreads = 128;
+  static constexpr int kChunk = 256;
   static constexpr int kStages = 4;
   static constexpr int kRowBytes = (kChunk + 8) * 2;  // 8 elements of padding: fragment rows on different banks
   static constexpr int kWeightRows = TRANS ? kChunk : RANK;
   static constexpr int kWeightBytes = ((TRANS ? RANK : kChunk) + 8) * 2;
   static constexpr int kStageBytes = ROWS * kRowBytes + kWeightRows * kWeightBytes;
-  static constexpr int kPartRows = ROWS == kWide ? ROWS : 4 * ROWS;
+  static constexpr int kPartRows = 4 * ROWS;
   static constexpr int kPartBytes = kPartRows * RANK * 4;
   static constexpr int kBytes = kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes;
 };
 
-template <typename T, int ROWS, int RANK, bool TRANS, bool FAST>
-__global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adapter_shrink(AdapterParams p) {
-  using S = ShrinkShape<ROWS, RANK, TRANS>;
+template <typename T, int RANK, bool TRANS, bool FAST>
+__global__ void __launch_bounds__(NarrowShape<RANK, TRANS>::kThreads) adapter_shrink(AdapterParams p) {
+  using S = NarrowShape<RANK, TRANS>;
+  constexpr int ROWS = kNarrow;
   extern __shared__ __align__(16) uint8_t shared[];
   const uint32_t stages = smem_u32(shared);
   griddep_launch_dependents();
@@ -162,8 +192,8 @@ __global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adap
     if (first + i < last) load(first + i);
     cp_async_commit();
   }
-  const int k_of = ROWS == kWide ? 0 : warp * (S::kChunk / 4);
-  const uint32_t a_from = stages + ((ROWS == kWide ? warp * 16 : 0) + (lane & 15)) * S::kRowBytes + (k_of + (lane >> 4) * 8) * 2;
+  const int k_of = warp * (S::kChunk / 4);
+  const uint32_t a_from = stages + (lane & 15) * S::kRowBytes + (k_of + (lane >> 4) * 8) * 2;
   const uint32_t b_from =
       stages + ROWS * S::kRowBytes +
       (TRANS ? (k_of + ((lane >> 3) & 1) * 8 + (lane & 7)) * S::kWeightBytes + (lane >> 4) * 16
@@ -174,7 +204,7 @@ __global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adap
     if (chunk + S::kStages - 1 < last) load(chunk + S::kStages - 1);
     cp_async_commit();
     const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
-    constexpr int kSteps = ROWS == kWide ? S::kChunk / 16 : S::kChunk / 64;
+    constexpr int kSteps = S::kChunk / 64;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
       uint32_t a[4];
@@ -205,8 +235,6 @@ __global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adap
   }
   cluster_sync();
   const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
-  T* high = static_cast<T*>(p.low);
-  T* low = high + p.slots * p.rank_pad;
   for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * RANK; e += static_cast<int>(splits) * S::kThreads) {
     const int row = e / RANK, c = e % RANK;
     if (rank0 + c >= p.rank_pad) continue;
@@ -214,18 +242,235 @@ __global__ void __launch_bounds__(ShrinkShape<ROWS, RANK, TRANS>::kThreads) adap
 #pragma unroll 4
     for (uint32_t s = 0; s < splits; ++s) {
       const uint32_t from = mapa_shared(part, s) + e * 4;
-      v += load_cluster_f32(from);
-      if constexpr (ROWS == kNarrow) {
 #pragma unroll
-        for (int other = 1; other < 4; ++other) v += load_cluster_f32(from + other * 16 * RANK * 4);
-      }
+      for (int other = 0; other < 4; ++other) v += load_cluster_f32(from + other * ROWS * RANK * 4);
     }
-    v *= scale;
-    const T hi = from_float<T>(v);
-    const float rest = v - to_float(hi);
-    const int64_t at = (tile.start + row) * static_cast<int64_t>(p.rank_pad) + rank0 + c;
-    high[at] = hi;
-    low[at] = from_float<T>(isfinite(rest) ? rest : 0.f);  // an infinite sum stays one
+    store_planes<T>(p, tile.start + row, rank0 + c, v * scale);
+  }
+  cluster_sync();  // the others may still be reading this block's sums
+}
+
+// ---- tensor memory: shrink of wide tiles, and outer ----
+
+// kind::f16 instruction: fp32 accumulators, both operands T; *_mn: the
+// operand's rows (A) or columns (B) are contiguous in memory, not its K.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b_mn) {
+  const uint32_t type = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Layouts of the operands in shared memory.
+//   swizzled  rows of 128 bytes in groups of 8 (1024 bytes); the 16-byte
+//             pieces of row r are permuted by r % 8 (128-byte swizzle). K-major
+//             when a row holds K, MN-major when it holds 64 rows of A.
+//   panels    (MN-major, no swizzle) the 8 columns n of a panel for 8 values
+//             of K are 8 consecutive 16-byte pieces; K groups are 128 bytes
+//             apart, panels `stride`.
+__device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint32_t paneled(int k, int panel, int stride) { return panel * stride + k * 16; }
+
+// A ring of stages that all threads fill and one thread multiplies from. A
+// stage is refilled when the products that read it have completed. Waits are
+// bounded: after one has run out (recorded in the watchdog word) the block
+// goes on without waiting, on whatever is there.
+template <int STAGES>
+struct TensorRing {
+  uint64_t used[STAGES];
+  uint32_t tensor_memory;
+  int32_t abort;
+
+  // One warp; everyone else sees it after the block's next barrier.
+  __device__ __forceinline__ void start(int columns) {
+    if ((threadIdx.x & 31) == 0) {
+      for (int i = 0; i < STAGES; ++i) mbar_init(&used[i], 1);
+      fence_barrier_init();
+      abort = 0;
+    }
+    __syncwarp();
+    tmem_alloc(&tensor_memory, static_cast<uint32_t>(columns));
+    tmem_relinquish();
+  }
+  // The products of the index-th filling of the ring have completed.
+  __device__ __forceinline__ void wait(int index, int32_t* watchdog) {
+    volatile int32_t* flag = &abort;
+    if (*flag == 0) mbar_wait(&used[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1, kWaitAccum, flag, watchdog);
+  }
+  __device__ __forceinline__ void drain(int index) {
+    mbar_drain(&used[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1);
+  }
+};
+
+// Sums in shared memory: rows of RANK floats and 16 bytes of padding (the
+// lanes of a tensor-memory load write their rows' words to different banks).
+// Four neighbouring ones over the blocks of a cluster, in their order.
+__device__ __forceinline__ float4 sum_cluster(const float* part, int at, uint32_t splits) {
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (uint32_t s = 0; s < splits; ++s) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(mapa_shared(part, s) + at * 4)
+                 : "memory");
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  return sum;
+}
+// This thread's row of an accumulator (zeros where nothing was multiplied).
+template <int RANK>
+__device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any) {
+#pragma unroll
+  for (int c0 = 0; c0 < RANK; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(accumulator + c0, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < (RANK < 32 ? RANK : 32); c += 4) {
+      float4 w = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
+                             __uint_as_float(v[c + 3]));
+      *reinterpret_cast<float4*>(row + c0 + c) = any ? w : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
+template <int RANK, bool TRANS>
+struct WideShape {
+  static constexpr int kThreads = 256;
+  static constexpr int kChunk = 64;  // of the width: one swizzled row of 128 bytes
+  static constexpr int kStages = 4;
+  static constexpr int kAhead = 3;   // chunks on their way; the others' products may still run
+  static constexpr int kRowBytes = kWide * 128;
+  static constexpr int kStageBytes = kRowBytes + kChunk * RANK * 2;
+  static constexpr int kTensorColumns = RANK < 32 ? 32 : RANK;
+  static constexpr int kPartPitch = RANK + 4;
+  static constexpr int kPartBytes = kWide * kPartPitch * 4;
+  static constexpr int kBytes = 1024 + (kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes);
+};
+
+// Tiles of 128 rows: D [128, RANK] in tensor memory. The rows are A (K-major,
+// swizzled); the weight chunk is B, K-major and swizzled ([rank, width]) or in
+// panels ([width, rank]).
+template <typename T, int RANK, bool TRANS, bool FAST>
+__global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_shrink_wide(AdapterParams p) {
+  using S = WideShape<RANK, TRANS>;
+  extern __shared__ uint8_t shared_raw[];
+  __shared__ TensorRing<S::kStages> ring;
+  uint8_t* shared = shared_raw + (-smem_u32(shared_raw) & 1023u);  // the swizzle goes by address bits
+  const uint32_t stages = smem_u32(shared);
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const uint32_t split = cluster_ctarank();
+  const Tile tile = p.tiles[blockIdx.x / splits];
+  const int rank0 = blockIdx.y * RANK;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) ring.start(S::kTensorColumns);
+  const bool valid = tile.adapter >= 0 && tile.adapter < p.adapters;
+  const int count = valid ? tile.count : 0;
+  const int width = static_cast<int>(p.width);
+  const int chunks = (width + S::kChunk - 1) / S::kChunk;
+  const int first = min(static_cast<int>(split) * p.chunks_per_split, chunks);
+  const int last = min(first + p.chunks_per_split, chunks);
+
+  constexpr int kPieces = 8, kRowStep = S::kThreads / kPieces, kRowCopies = kWide / kRowStep;
+  constexpr int kWeightPieces = TRANS ? RANK / 8 : kPieces, kWeightRows = TRANS ? S::kChunk : RANK;
+  constexpr int kWeightStep = S::kThreads / kWeightPieces;
+  constexpr int kWeightCopies = (kWeightRows + kWeightStep - 1) / kWeightStep;
+  const int piece = tid % kPieces, row_of = tid / kPieces;
+  const int weight_piece = tid % kWeightPieces, weight_row = tid / kWeightPieces;
+  const T* source[kRowCopies];
+  uint32_t present = 0;
+#pragma unroll
+  for (int i = 0; i < kRowCopies; ++i) {
+    const int row = row_of + i * kRowStep;
+    const int64_t token = row < count ? token_of(p, tile.start + row) : -1;
+    if (token >= 0) present |= 1u << i;
+    source[i] = static_cast<const T*>(p.rows_in) + (token >= 0 ? token * p.row_stride : 0) + piece * 8;
+  }
+  const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(valid ? tile.adapter : 0) * p.rank * p.width;
+  weight += TRANS ? static_cast<int64_t>(weight_row) * p.rank + rank0 + weight_piece * 8
+                  : static_cast<int64_t>(rank0 + weight_row) * width + weight_piece * 8;
+  // Row and weight steps are multiples of 8: the swizzle is the same for all of a thread's copies.
+  const uint32_t row_to = stages + swizzled(row_of, piece);
+  const uint32_t weight_to = stages + S::kRowBytes +
+                             (TRANS ? paneled(weight_row, weight_piece, S::kChunk * 16) : swizzled(weight_row, weight_piece));
+  constexpr int kWeightStride = kWeightStep * (TRANS ? 16 : 128);
+
+  auto load = [&](int chunk) {
+    const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
+    const int k0 = chunk * S::kChunk, left = width - k0 - piece * 8;
+#pragma unroll
+    for (int i = 0; i < kRowCopies; ++i) {
+      copy8<T, FAST>(row_to + stage + i * kRowStep * 128, left > 0 ? source[i] + k0 : source[i],
+                     (present >> i & 1) ? left : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kWeightCopies; ++i) {
+      const int at = weight_row + i * kWeightStep;
+      if (kWeightRows % kWeightStep != 0 && at >= kWeightRows) continue;
+      const int in = TRANS ? (k0 + at < width ? p.rank - (rank0 + weight_piece * 8) : 0) : (rank0 + at < p.rank ? left : 0);
+      const T* from = weight + (TRANS ? static_cast<int64_t>(k0 + i * kWeightStep) * p.rank
+                                      : static_cast<int64_t>(i * kWeightStep) * width + k0);
+      copy8<T, FAST>(weight_to + stage + i * kWeightStride, in > 0 ? from : static_cast<const T*>(p.weight), in);
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < S::kAhead; ++i) {
+    if (first + i < last) load(first + i);
+    cp_async_commit();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t accumulator = ring.tensor_memory;
+  constexpr uint32_t kInstruction = idesc_f16<T>(kWide, RANK, false, TRANS);
+  for (int chunk = first; chunk < last; ++chunk) {
+    cp_async_wait<S::kAhead - 1>();
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      const uint32_t rows = stages + static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
+      const uint32_t w = rows + S::kRowBytes;
+#pragma unroll
+      for (int k = 0; k < S::kChunk / 16; ++k) {
+        const uint64_t b = TRANS ? smem_desc(w + k * 256, 128, S::kChunk * 16, 0) : sw128_desc(w + k * 32);
+        mma_bf16(accumulator, sw128_desc(rows + k * 32), b, kInstruction, chunk > first || k > 0);
+      }
+      tc_commit(&ring.used[(chunk - first) % S::kStages]);
+    }
+    __syncwarp();
+    if (chunk + S::kAhead < last) {
+      constexpr int kBehind = S::kStages - S::kAhead;
+      if (chunk - first >= kBehind) ring.wait(chunk - first - kBehind, p.watchdog);
+      load(chunk + S::kAhead);
+    }
+    cp_async_commit();
+  }
+  cp_async_wait<0>();
+  float* part = reinterpret_cast<float*>(shared);
+  if (first < last) {
+    ring.wait(last - 1 - first, p.watchdog);
+    if (ring.abort != 0 && tid == 0) ring.drain(last - 1 - first);
+  }
+  tc_fence_after();
+  __syncthreads();
+  if (warp < 4) {
+    store_part<RANK>(part + (warp * 32 + lane) * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp) << 21), first < last);
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(accumulator, S::kTensorColumns);
+  const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
+  constexpr int kQuads = RANK / 4;
+  for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * kQuads; e += static_cast<int>(splits) * S::kThreads) {
+    const int row = e / kQuads, c = e % kQuads * 4;
+    if (rank0 + c >= p.rank_pad) continue;
+    const float4 v = sum_cluster(part, row * S::kPartPitch + c, splits);
+    store_planes4<T>(p, tile.start + row, rank0 + c, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
   }
   cluster_sync();  // the others may still be reading this block's sums
 }
@@ -486,29 +731,36 @@ __global__ void __launch_bounds__(ExpandShape<ROWS>::kThreads, ExpandShape<ROWS>
 
 // ------------------------------------------------------------------- outer ----
 
-// dW[column, r] = sum over the adapter's slots of row[column] * low[r]. A
-// block takes 128 columns and RANK ranks; the blocks of a cluster share the
-// adapter's tokens.
+// dW[column, r] = sum over the adapter's slots of row[column] * low[r]: D
+// [128 columns, RANK] twice in tensor memory, K the slots. The rows are A
+// (MN-major: 64 columns are a swizzled row of 128 bytes), both planes of `low`
+// B (in panels). A block takes 256 columns and RANK ranks; the blocks of a
+// cluster share the adapter's tokens.
 template <int RANK>
 struct OuterShape {
   static constexpr int kThreads = 256;
   static constexpr int kColumns = 256;
   static constexpr int kTokens = 32;
   static constexpr int kStages = 4;
-  static constexpr int kLook = 2 * kStages;  // token lists in flight
-  static constexpr int kRowBytes = (kColumns + 8) * 2;
-  static constexpr int kLowBytes = (RANK + 8) * 2;
-  static constexpr int kStageBytes = kTokens * (kRowBytes + 2 * kLowBytes);
-  static constexpr int kPartPitch = RANK + 1;
-  static constexpr int kPartBytes = kColumns * kPartPitch * 4;
-  static constexpr int kBytes = kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes;
+  static constexpr int kAhead = 3;   // tiles on their way; the others' products may still run
+  static constexpr int kLook = 8;    // token lists in flight
+  static constexpr int kSubBytes = kTokens * 128;  // 64 columns
+  static constexpr int kRowBytes = kColumns / 64 * kSubBytes;
+  static constexpr int kPlaneBytes = kTokens * RANK * 2;
+  static constexpr int kStageBytes = kRowBytes + 2 * kPlaneBytes;
+  static constexpr int kTensorColumns = RANK < 32 ? 64 : 2 * RANK;  // a load reads 32 columns
+  static constexpr int kPartPitch = RANK + 4;
+  static constexpr int kPartBytes = kColumns * kPartPitch * 4 * 3 / 2;  // and a cluster's share, at most half
+  static constexpr int kBytes = 1024 + (kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes);
 };
 
 template <typename T, int RANK, bool FAST>
 __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(AdapterParams p) {
   using S = OuterShape<RANK>;
-  extern __shared__ __align__(16) uint8_t shared[];
+  extern __shared__ uint8_t shared_raw[];
+  __shared__ TensorRing<S::kStages> ring;
   __shared__ int32_t tokens[S::kLook][S::kTokens];
+  uint8_t* shared = shared_raw + (-smem_u32(shared_raw) & 1023u);  // the swizzle goes by address bits
   const uint32_t stages = smem_u32(shared);
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
@@ -517,6 +769,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   const int adapter = blockIdx.y;
   const int rank0 = blockIdx.z * RANK;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) ring.start(S::kTensorColumns);
   const int32_t begin = p.group_offsets[adapter], end = p.group_offsets[adapter + 1];
   const int tiles = (end - begin + S::kTokens - 1) / S::kTokens;
   const int per_split = (tiles + static_cast<int>(splits) - 1) / static_cast<int>(splits);
@@ -524,6 +777,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   const int last = min(first + per_split, tiles);
 
   constexpr int kPieces = S::kColumns / 8, kRowStep = S::kThreads / kPieces, kRowCopies = S::kTokens / kRowStep;
+  static_assert(kRowStep == 8, "a thread's rows share their swizzle");
   constexpr int kLowPieces = RANK / 8, kLowStep = S::kThreads / kLowPieces;
   constexpr int kLowCopies = (2 * S::kTokens + kLowStep - 1) / kLowStep;
   const int piece = tid % kPieces, row_of = tid / kPieces;
@@ -532,10 +786,9 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   const int columns_left = static_cast<int>(p.width - column0) - piece * 8;
   const bool low_in = rank0 + low_piece * 8 < p.rank_pad;
   const T* low = static_cast<const T*>(p.low) + (low_in ? rank0 + low_piece * 8 : 0);
-  const uint32_t row_to = stages + row_of * S::kRowBytes + piece * 16;
-  const uint32_t low_to = stages + S::kTokens * S::kRowBytes + low_row * S::kLowBytes + low_piece * 16;
+  const uint32_t row_to = stages + piece / 8 * S::kSubBytes + swizzled(row_of, piece % 8);
 
-  // The tokens of a tile are copied kStages - 1 tiles before its rows.
+  // The tokens of a tile are copied kAhead tiles before its rows.
   auto look = [&](int tile) {
     const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + tid;
     if (tid >= S::kTokens || tile >= last) return;
@@ -548,96 +801,105 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
     for (int i = 0; i < kRowCopies; ++i) {
       const int32_t token = tokens[tile % S::kLook][row_of + i * kRowStep];
       const bool in = token >= 0 && token < p.tokens && columns_left > 0;
-      copy8<T, FAST>(row_to + stage + i * kRowStep * S::kRowBytes,
+      copy8<T, FAST>(row_to + stage + i * kRowStep * 128,
                      in ? x + token * p.row_stride : static_cast<const T*>(p.rows_in), in ? columns_left : 0);
     }
     const int slot0 = begin + tile * S::kTokens;
 #pragma unroll
     for (int i = 0; i < kLowCopies; ++i) {
-      const int at = low_row + i * kLowStep, row = at % S::kTokens;
+      const int at = low_row + i * kLowStep, plane = at / S::kTokens, row = at % S::kTokens;
       if (2 * S::kTokens % kLowStep != 0 && at >= 2 * S::kTokens) continue;
       const bool in = low_in && slot0 + row < end;
-      cp_async16(low_to + stage + i * kLowStep * S::kLowBytes,
-                 in ? low + (at / S::kTokens * p.slots + slot0 + row) * p.rank_pad : low, in);
+      cp_async16(stages + stage + S::kRowBytes + plane * S::kPlaneBytes + paneled(row, low_piece, S::kTokens * 16),
+                 in ? low + (plane * p.slots + slot0 + row) * p.rank_pad : low, in);
     }
   };
 
-  float acc[2][RANK / 8][4];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-#pragma unroll
-    for (int i = 0; i < RANK / 8; ++i) acc[m][i][0] = acc[m][i][1] = acc[m][i][2] = acc[m][i][3] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < 2 * (S::kStages - 1); ++i) look(first + i);
+  for (int i = 0; i < 2 * S::kAhead; ++i) look(first + i);
   cp_async_commit();
   cp_async_wait<0>();
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) {
+  for (int i = 0; i < S::kAhead; ++i) {
     if (first + i < last) load(first + i);
     cp_async_commit();
   }
-  const uint32_t a_from = stages + ((lane >> 4) * 8 + (lane & 7)) * S::kRowBytes + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
-  const uint32_t b_from = stages + S::kTokens * S::kRowBytes + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::kLowBytes +
-                          (lane >> 4) * 16;
+  const uint32_t accumulator = ring.tensor_memory;
+  constexpr uint32_t kInstruction = idesc_f16<T>(128, RANK, true, true);
   for (int tile = first; tile < last; ++tile) {
-    cp_async_wait<S::kStages - 2>();
+    cp_async_wait<S::kAhead - 1>();
+    fence_proxy_async_smem();
     __syncthreads();
-    if (tile + S::kStages - 1 < last) load(tile + S::kStages - 1);
-    look(tile + 2 * (S::kStages - 1));
-    cp_async_commit();
-    const uint32_t stage = static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
+    if (tid == 0) {
+      const uint32_t rows = stages + static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
 #pragma unroll
-    for (int k = 0; k < S::kTokens; k += 16) {
-      uint32_t a[2][4];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) ldmatrix_x4_trans(a[m], a_from + stage + k * S::kRowBytes + m * 32);
-#pragma unroll
-      for (int n = 0; n < RANK / 16; ++n) {
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
-          uint32_t b[4];
-          ldmatrix_x4_trans(b, b_from + stage + (plane * S::kTokens + k) * S::kLowBytes + n * 32);
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            mma_16816<T>(acc[m][2 * n], a[m], b);
-            mma_16816<T>(acc[m][2 * n + 1], a[m], b + 2);
+          for (int k = 0; k < S::kTokens / 16; ++k) {
+            // Groups of 8 slots are 1024 bytes apart, the two runs of 64 columns kSubBytes.
+            const uint64_t a = smem_desc(rows + half * 2 * S::kSubBytes + k * 2048, S::kSubBytes, 1024, 2);
+            const uint64_t b = smem_desc(rows + S::kRowBytes + plane * S::kPlaneBytes + k * 256, 128, S::kTokens * 16, 0);
+            mma_bf16(accumulator + half * RANK, a, b, kInstruction, tile > first || plane > 0 || k > 0);
           }
         }
       }
+      tc_commit(&ring.used[(tile - first) % S::kStages]);
     }
+    __syncwarp();
+    if (tile + S::kAhead < last) {
+      constexpr int kBehind = S::kStages - S::kAhead;
+      if (tile - first >= kBehind) ring.wait(tile - first - kBehind, p.watchdog);
+      load(tile + S::kAhead);
+    }
+    look(tile + 2 * S::kAhead);
+    cp_async_commit();
   }
 
   cp_async_wait<0>();
-  __syncthreads();
   float* part = reinterpret_cast<float*>(shared);
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int c = warp * 32 + m * 16 + (lane >> 2);
-#pragma unroll
-    for (int i = 0; i < RANK / 8; ++i) {
-      const int r = i * 8 + (lane & 3) * 2;
-      part[c * S::kPartPitch + r] = acc[m][i][0];
-      part[c * S::kPartPitch + r + 1] = acc[m][i][1];
-      part[(c + 8) * S::kPartPitch + r] = acc[m][i][2];
-      part[(c + 8) * S::kPartPitch + r + 1] = acc[m][i][3];
+  if (first < last) {
+    ring.wait(last - 1 - first, p.watchdog);
+    if (ring.abort != 0 && tid == 0) ring.drain(last - 1 - first);
+  }
+  tc_fence_after();
+  __syncthreads();
+  {
+    const int half = warp / 4, c = half * 128 + warp % 4 * 32 + lane;
+    store_part<RANK>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * RANK,
+                     first < last);
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(accumulator, S::kTensorColumns);
+  // Each block adds up its share of the columns, beside its own sums (which
+  // the others may still be reading), then writes it in memory order.
+  const int share = (S::kColumns + static_cast<int>(splits) - 1) / static_cast<int>(splits);
+  const int c_first = static_cast<int>(split) * share, c_count = max(0, min(share, S::kColumns - c_first));
+  float* mine = part;
+  if (splits > 1) {
+    mine = part + S::kColumns * S::kPartPitch;
+    constexpr int kQuads = RANK / 4;
+    for (int e = tid; e < c_count * kQuads; e += S::kThreads) {
+      const int c = e / kQuads, q = e % kQuads * 4;
+      *reinterpret_cast<float4*>(mine + c * S::kPartPitch + q) = sum_cluster(part, (c_first + c) * S::kPartPitch + q, splits);
     }
+    cluster_sync();
   }
-  cluster_sync();
   T* out = static_cast<T*>(p.out) + static_cast<int64_t>(adapter) * p.rank * p.width;
-  const bool columns_fast = p.out_stride == 1;  // neighbouring threads write neighbouring elements
-  for (int e = static_cast<int>(split) * S::kThreads + tid; e < S::kColumns * RANK;
-       e += static_cast<int>(splits) * S::kThreads) {
-    const int c = columns_fast ? e % S::kColumns : e / RANK;
-    const int r = columns_fast ? e / S::kColumns : e % RANK;
-    if (column0 + c >= p.width || rank0 + r >= p.rank) continue;
-    float v = 0.f;
-#pragma unroll 4
-    for (uint32_t s = 0; s < splits; ++s) v += load_cluster_f32(mapa_shared(part, s) + (c * S::kPartPitch + r) * 4);
-    out[(column0 + c) * p.out_stride + (rank0 + r) * p.out_rank_stride] = from_float<T>(v);
+  const bool columns_fast = p.out_stride == 1;
+  for (int e = tid; e < c_count * RANK; e += S::kThreads) {
+    const int c = columns_fast ? e % c_count : e / RANK;
+    const int r = columns_fast ? e / c_count : e % RANK;
+    const int64_t column = column0 + c_first + c;
+    if (column >= p.width || rank0 + r >= p.rank) continue;
+    out[column * p.out_stride + (rank0 + r) * p.out_rank_stride] = from_float<T>(mine[c * S::kPartPitch + r]);
   }
-  cluster_sync();
 }
 
 // -------------------------------------------------------------------- host ----
@@ -696,15 +958,19 @@ int split_count(int64_t blocks, int64_t chunks, int resident) {
 
 template <typename T, int ROWS, int RANK, bool TRANS>
 int launch_shrink(AdapterParams p, int64_t tiles, cudaStream_t stream) {
-  using S = ShrinkShape<ROWS, RANK, TRANS>;
+  using S = std::conditional_t<ROWS == kWide, WideShape<RANK, TRANS>, NarrowShape<RANK, TRANS>>;
   const int64_t chunks = ceil_div(p.width, S::kChunk);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int split = split_count(tiles * rank_blocks, chunks, ROWS == kWide ? 2 : 4);
   p.chunks_per_split = static_cast<int>(ceil_div(chunks, split));
   const dim3 grid(static_cast<unsigned>(tiles * split), rank_blocks);
   const bool fast = p.vector_rows && p.vector_weight && p.width % 8 == 0 && (!TRANS || p.rank % 8 == 0);
-  return fast ? launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, true>, p, grid, S::kThreads, split, S::kBytes, false, stream)
-              : launch_clustered(adapter_shrink<T, ROWS, RANK, TRANS, false>, p, grid, S::kThreads, split, S::kBytes, false, stream);
+  auto launch = [&](auto kernel) { return launch_clustered(kernel, p, grid, S::kThreads, split, S::kBytes, false, stream); };
+  if constexpr (ROWS == kWide) {
+    return fast ? launch(adapter_shrink_wide<T, RANK, TRANS, true>) : launch(adapter_shrink_wide<T, RANK, TRANS, false>);
+  } else {
+    return fast ? launch(adapter_shrink<T, RANK, TRANS, true>) : launch(adapter_shrink<T, RANK, TRANS, false>);
+  }
 }
 
 template <typename T, int ROWS, bool TRANS>
@@ -806,6 +1072,8 @@ int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride, int64_t token
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
+  p.watchdog = watchdog_ptr();
+  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
   p.rows_in = x;
   p.row_stride = x_stride;
   p.tokens = tokens;
@@ -877,6 +1145,8 @@ int sdc_adapter_outer(int dtype, const void* x, int64_t x_stride, int64_t tokens
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
+  p.watchdog = watchdog_ptr();
+  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
   p.rows_in = x;
   p.row_stride = x_stride;
   p.tokens = tokens;
