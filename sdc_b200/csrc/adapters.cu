@@ -272,20 +272,26 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 __device__ __forceinline__ uint32_t paneled(int k, int panel, int stride) { return panel * stride + k * 16; }
 
-// A ring of stages that all threads fill and one thread multiplies from. A
-// stage is refilled when the products that read it have completed. Waits are
-// bounded: after one has run out (recorded in the watchdog word) the block
-// goes on without waiting, on whatever is there.
+// A ring of stages that eight warps fill and a ninth multiplies from. A
+// filling is full when every filling thread's copies have arrived, and its
+// stage is free again when the products that read it have completed. Waits
+// are bounded: one that runs out is recorded in the watchdog word, the warps
+// leave their loops one after the other and meet at the block's next barrier.
+constexpr int kFillThreads = 256, kTensorThreads = kFillThreads + 32;
+
 template <int STAGES>
 struct TensorRing {
-  uint64_t used[STAGES];
+  uint64_t full[STAGES], used[STAGES];
   uint32_t tensor_memory;
   int32_t abort;
 
   // One warp; everyone else sees it after the block's next barrier.
   __device__ __forceinline__ void start(int columns) {
     if ((threadIdx.x & 31) == 0) {
-      for (int i = 0; i < STAGES; ++i) mbar_init(&used[i], 1);
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(&full[i], kFillThreads);
+        mbar_init(&used[i], 1);
+      }
       fence_barrier_init();
       abort = 0;
     }
@@ -293,13 +299,44 @@ struct TensorRing {
     tmem_alloc(&tensor_memory, static_cast<uint32_t>(columns));
     tmem_relinquish();
   }
-  // The products of the index-th filling of the ring have completed.
-  __device__ __forceinline__ void wait(int index, int32_t* watchdog) {
-    volatile int32_t* flag = &abort;
-    if (*flag == 0) mbar_wait(&used[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1, kWaitAccum, flag, watchdog);
+  // Until the index-th filling is full, or its products have completed. The
+  // same for a whole warp.
+  __device__ __forceinline__ bool wait(uint64_t* bars, int index, int32_t* watchdog) {
+    const uint32_t parity = static_cast<uint32_t>(index / STAGES) & 1;
+    return __all_sync(0xffffffffu, mbar_wait(&bars[index % STAGES], parity, kWaitAccum, &abort, watchdog)) != 0;
+  }
+  // A filling thread's copies of a filling have been issued (FAST: the
+  // barrier counts it when they arrive) or made.
+  template <bool FAST>
+  __device__ __forceinline__ void filled(int index) {
+    if constexpr (FAST) {
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[index % STAGES]))
+                   : "memory");
+    } else {
+      cp_async_commit();
+      cp_async_wait<0>();
+      mbar_arrive(&full[index % STAGES]);
+    }
   }
   __device__ __forceinline__ void drain(int index) {
     mbar_drain(&used[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1);
+  }
+  // The ninth warp: products of `count` fillings, issued by one lane.
+  template <typename Products>
+  __device__ __forceinline__ void multiply(int count, int32_t* watchdog, const Products& products) {
+    int done = 0;
+    for (; done < count; ++done) {
+      if (!wait(full, done, watchdog)) break;
+      fence_proxy_async_smem();  // the copies were made by ordinary writes
+      tc_fence_after();
+      if ((threadIdx.x & 31) == 0) {
+        products(done);
+        tc_commit(&used[done % STAGES]);
+      }
+      __syncwarp();
+    }
+    if (abort != 0 && done > 0 && (threadIdx.x & 31) == 0) drain(done - 1);  // nothing may stay in flight
+    __syncwarp();
   }
 };
 
@@ -338,10 +375,9 @@ __device__ __forceinline__ void store_part(float* row, uint32_t accumulator, boo
 
 template <int RANK, bool TRANS>
 struct WideShape {
-  static constexpr int kThreads = 256;
+  static constexpr int kThreads = kTensorThreads;
   static constexpr int kChunk = 64;  // of the width: one swizzled row of 128 bytes
   static constexpr int kStages = 4;
-  static constexpr int kAhead = 3;   // chunks on their way; the others' products may still run
   static constexpr int kRowBytes = kWide * 128;
   static constexpr int kStageBytes = kRowBytes + kChunk * RANK * 2;
   static constexpr int kTensorColumns = RANK < 32 ? 32 : RANK;
@@ -366,95 +402,85 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
   const Tile tile = p.tiles[blockIdx.x / splits];
   const int rank0 = blockIdx.y * RANK;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) ring.start(S::kTensorColumns);
+  if (warp == 8) ring.start(S::kTensorColumns);
   const bool valid = tile.adapter >= 0 && tile.adapter < p.adapters;
   const int count = valid ? tile.count : 0;
   const int width = static_cast<int>(p.width);
   const int chunks = (width + S::kChunk - 1) / S::kChunk;
   const int first = min(static_cast<int>(split) * p.chunks_per_split, chunks);
   const int last = min(first + p.chunks_per_split, chunks);
-
-  constexpr int kPieces = 8, kRowStep = S::kThreads / kPieces, kRowCopies = kWide / kRowStep;
-  constexpr int kWeightPieces = TRANS ? RANK / 8 : kPieces, kWeightRows = TRANS ? S::kChunk : RANK;
-  constexpr int kWeightStep = S::kThreads / kWeightPieces;
-  constexpr int kWeightCopies = (kWeightRows + kWeightStep - 1) / kWeightStep;
-  const int piece = tid % kPieces, row_of = tid / kPieces;
-  const int weight_piece = tid % kWeightPieces, weight_row = tid / kWeightPieces;
-  const T* source[kRowCopies];
-  uint32_t present = 0;
-#pragma unroll
-  for (int i = 0; i < kRowCopies; ++i) {
-    const int row = row_of + i * kRowStep;
-    const int64_t token = row < count ? token_of(p, tile.start + row) : -1;
-    if (token >= 0) present |= 1u << i;
-    source[i] = static_cast<const T*>(p.rows_in) + (token >= 0 ? token * p.row_stride : 0) + piece * 8;
-  }
-  const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(valid ? tile.adapter : 0) * p.rank * p.width;
-  weight += TRANS ? static_cast<int64_t>(weight_row) * p.rank + rank0 + weight_piece * 8
-                  : static_cast<int64_t>(rank0 + weight_row) * width + weight_piece * 8;
-  // Row and weight steps are multiples of 8: the swizzle is the same for all of a thread's copies.
-  const uint32_t row_to = stages + swizzled(row_of, piece);
-  const uint32_t weight_to = stages + S::kRowBytes +
-                             (TRANS ? paneled(weight_row, weight_piece, S::kChunk * 16) : swizzled(weight_row, weight_piece));
-  constexpr int kWeightStride = kWeightStep * (TRANS ? 16 : 128);
-
-  auto load = [&](int chunk) {
-    const uint32_t stage = static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
-    const int k0 = chunk * S::kChunk, left = width - k0 - piece * 8;
-#pragma unroll
-    for (int i = 0; i < kRowCopies; ++i) {
-      copy8<T, FAST>(row_to + stage + i * kRowStep * 128, left > 0 ? source[i] + k0 : source[i],
-                     (present >> i & 1) ? left : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < kWeightCopies; ++i) {
-      const int at = weight_row + i * kWeightStep;
-      if (kWeightRows % kWeightStep != 0 && at >= kWeightRows) continue;
-      const int in = TRANS ? (k0 + at < width ? p.rank - (rank0 + weight_piece * 8) : 0) : (rank0 + at < p.rank ? left : 0);
-      const T* from = weight + (TRANS ? static_cast<int64_t>(k0 + i * kWeightStep) * p.rank
-                                      : static_cast<int64_t>(i * kWeightStep) * width + k0);
-      copy8<T, FAST>(weight_to + stage + i * kWeightStride, in > 0 ? from : static_cast<const T*>(p.weight), in);
-    }
-  };
-
-#pragma unroll
-  for (int i = 0; i < S::kAhead; ++i) {
-    if (first + i < last) load(first + i);
-    cp_async_commit();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t accumulator = ring.tensor_memory;
-  constexpr uint32_t kInstruction = idesc_f16<T>(kWide, RANK, false, TRANS);
-  for (int chunk = first; chunk < last; ++chunk) {
-    cp_async_wait<S::kAhead - 1>();
-    fence_proxy_async_smem();
-    __syncthreads();
-    if (tid == 0) {
-      const uint32_t rows = stages + static_cast<uint32_t>((chunk - first) % S::kStages) * S::kStageBytes;
-      const uint32_t w = rows + S::kRowBytes;
+
+  if (warp < 8) {
+    constexpr int kPieces = 8, kRowStep = kFillThreads / kPieces, kRowCopies = kWide / kRowStep;
+    constexpr int kWeightPieces = TRANS ? RANK / 8 : kPieces, kWeightRows = TRANS ? S::kChunk : RANK;
+    constexpr int kWeightStep = kFillThreads / kWeightPieces;
+    constexpr int kWeightCopies = (kWeightRows + kWeightStep - 1) / kWeightStep;
+    const int piece = tid % kPieces, row_of = tid / kPieces;
+    const int weight_piece = tid % kWeightPieces, weight_row = tid / kWeightPieces;
+    // Sources of the next chunk, and where they may no longer be read from:
+    // columns left from this thread's piece on (0 for rows that are not there).
+    const T* source[kRowCopies];
+    int left[kRowCopies];
+    const int skipped = first * S::kChunk;
 #pragma unroll
-      for (int k = 0; k < S::kChunk / 16; ++k) {
-        const uint64_t b = TRANS ? smem_desc(w + k * 256, 128, S::kChunk * 16, 0) : sw128_desc(w + k * 32);
-        mma_bf16(accumulator, sw128_desc(rows + k * 32), b, kInstruction, chunk > first || k > 0);
-      }
-      tc_commit(&ring.used[(chunk - first) % S::kStages]);
+    for (int i = 0; i < kRowCopies; ++i) {
+      const int row = row_of + i * kRowStep;
+      const int64_t token = row < count ? token_of(p, tile.start + row) : -1;
+      source[i] = static_cast<const T*>(p.rows_in) + (token >= 0 ? token * p.row_stride : 0) + piece * 8 + skipped;
+      left[i] = token >= 0 ? width - piece * 8 - skipped : 0;
     }
-    __syncwarp();
-    if (chunk + S::kAhead < last) {
-      constexpr int kBehind = S::kStages - S::kAhead;
-      if (chunk - first >= kBehind) ring.wait(chunk - first - kBehind, p.watchdog);
-      load(chunk + S::kAhead);
+    const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(valid ? tile.adapter : 0) * p.rank * p.width;
+    weight += TRANS ? static_cast<int64_t>(skipped + weight_row) * p.rank + rank0 + weight_piece * 8
+                    : static_cast<int64_t>(rank0 + weight_row) * width + weight_piece * 8 + skipped;
+    const int64_t weight_step = TRANS ? static_cast<int64_t>(kWeightStep) * p.rank : static_cast<int64_t>(kWeightStep) * width;
+    const int64_t weight_chunk = TRANS ? static_cast<int64_t>(S::kChunk) * p.rank : S::kChunk;
+    const int ranks_left = p.rank - rank0 - (TRANS ? weight_piece * 8 : weight_row);
+    int weight_left = TRANS ? width - skipped - weight_row : width - skipped - weight_piece * 8;
+    // Row and weight steps are multiples of 8: the swizzle is the same for all of a thread's copies.
+    const uint32_t row_to = stages + swizzled(row_of, piece);
+    const uint32_t weight_to = stages + S::kRowBytes +
+                               (TRANS ? paneled(weight_row, weight_piece, S::kChunk * 16) : swizzled(weight_row, weight_piece));
+    constexpr int kWeightStride = kWeightStep * (TRANS ? 16 : 128);
+    for (int fill = 0; fill < last - first; ++fill) {
+      if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+      const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < kRowCopies; ++i) {
+        copy8<T, FAST>(row_to + stage + i * kRowStep * 128, source[i], left[i]);
+        source[i] += S::kChunk;
+        left[i] -= S::kChunk;
+      }
+#pragma unroll
+      for (int i = 0; i < kWeightCopies; ++i) {
+        if (kWeightRows % kWeightStep != 0 && weight_row + i * kWeightStep >= kWeightRows) continue;
+        const int in = TRANS ? (weight_left > i * kWeightStep ? ranks_left : 0) : (ranks_left > i * kWeightStep ? weight_left : 0);
+        copy8<T, FAST>(weight_to + stage + i * kWeightStride, weight + i * weight_step, in);
+      }
+      weight += weight_chunk;
+      weight_left -= S::kChunk;
+      ring.filled<FAST>(fill);
     }
     cp_async_commit();
+    cp_async_wait<0>();
+  } else {
+    constexpr uint32_t kInstruction = idesc_f16<T>(kWide, RANK, false, TRANS);
+    const uint64_t a = sw128_desc(stages);
+    const uint64_t b = TRANS ? smem_desc(stages + S::kRowBytes, 128, S::kChunk * 16, 0) : sw128_desc(stages + S::kRowBytes);
+    ring.multiply(last - first, p.watchdog, [&](int fill) {
+      // Addresses advance in the descriptors' units of 16 bytes.
+      const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
+#pragma unroll
+      for (int k = 0; k < S::kChunk / 16; ++k) {
+        mma_bf16(accumulator, a + stage + k * 2, b + stage + k * (TRANS ? 16 : 2), kInstruction, fill > 0 || k > 0);
+      }
+    });
   }
-  cp_async_wait<0>();
   float* part = reinterpret_cast<float*>(shared);
-  if (first < last) {
-    ring.wait(last - 1 - first, p.watchdog);
-    if (ring.abort != 0 && tid == 0) ring.drain(last - 1 - first);
-  }
+  if (first < last) ring.wait(ring.used, last - 1 - first, p.watchdog);
   tc_fence_after();
   __syncthreads();
   if (warp < 4) {
@@ -463,7 +489,7 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  if (warp == 0) tmem_dealloc(accumulator, S::kTensorColumns);
+  if (warp == 8) tmem_dealloc(accumulator, S::kTensorColumns);
   const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
   constexpr int kQuads = RANK / 4;
   for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * kQuads; e += static_cast<int>(splits) * S::kThreads) {
@@ -738,12 +764,10 @@ __global__ void __launch_bounds__(ExpandShape<ROWS>::kThreads, ExpandShape<ROWS>
 // cluster share the adapter's tokens.
 template <int RANK>
 struct OuterShape {
-  static constexpr int kThreads = 256;
+  static constexpr int kThreads = kTensorThreads;
   static constexpr int kColumns = 256;
   static constexpr int kTokens = 32;
   static constexpr int kStages = 4;
-  static constexpr int kAhead = 3;   // tiles on their way; the others' products may still run
-  static constexpr int kLook = 8;    // token lists in flight
   static constexpr int kSubBytes = kTokens * 128;  // 64 columns
   static constexpr int kRowBytes = kColumns / 64 * kSubBytes;
   static constexpr int kPlaneBytes = kTokens * RANK * 2;
@@ -759,7 +783,6 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   using S = OuterShape<RANK>;
   extern __shared__ uint8_t shared_raw[];
   __shared__ TensorRing<S::kStages> ring;
-  __shared__ int32_t tokens[S::kLook][S::kTokens];
   uint8_t* shared = shared_raw + (-smem_u32(shared_raw) & 1023u);  // the swizzle goes by address bits
   const uint32_t stages = smem_u32(shared);
   uint32_t splits;
@@ -769,106 +792,92 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   const int adapter = blockIdx.y;
   const int rank0 = blockIdx.z * RANK;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) ring.start(S::kTensorColumns);
+  if (warp == 8) ring.start(S::kTensorColumns);
   const int32_t begin = p.group_offsets[adapter], end = p.group_offsets[adapter + 1];
   const int tiles = (end - begin + S::kTokens - 1) / S::kTokens;
   const int per_split = (tiles + static_cast<int>(splits) - 1) / static_cast<int>(splits);
   const int first = min(static_cast<int>(split) * per_split, tiles);
   const int last = min(first + per_split, tiles);
-
-  constexpr int kPieces = S::kColumns / 8, kRowStep = S::kThreads / kPieces, kRowCopies = S::kTokens / kRowStep;
-  static_assert(kRowStep == 8, "a thread's rows share their swizzle");
-  constexpr int kLowPieces = RANK / 8, kLowStep = S::kThreads / kLowPieces;
-  constexpr int kLowCopies = (2 * S::kTokens + kLowStep - 1) / kLowStep;
-  const int piece = tid % kPieces, row_of = tid / kPieces;
-  const int low_piece = tid % kLowPieces, low_row = tid / kLowPieces;
-  const T* x = static_cast<const T*>(p.rows_in) + column0 + piece * 8;
-  const int columns_left = static_cast<int>(p.width - column0) - piece * 8;
-  const bool low_in = rank0 + low_piece * 8 < p.rank_pad;
-  const T* low = static_cast<const T*>(p.low) + (low_in ? rank0 + low_piece * 8 : 0);
-  const uint32_t row_to = stages + piece / 8 * S::kSubBytes + swizzled(row_of, piece % 8);
-
-  // The tokens of a tile are copied kAhead tiles before its rows.
-  auto look = [&](int tile) {
-    const int64_t slot = begin + static_cast<int64_t>(tile) * S::kTokens + tid;
-    if (tid >= S::kTokens || tile >= last) return;
-    if (slot < end) cp_async4(smem_u32(&tokens[tile % S::kLook][tid]), p.rows + slot);
-    else tokens[tile % S::kLook][tid] = -1;
-  };
-  auto load = [&](int tile) {
-    const uint32_t stage = static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
-#pragma unroll
-    for (int i = 0; i < kRowCopies; ++i) {
-      const int32_t token = tokens[tile % S::kLook][row_of + i * kRowStep];
-      const bool in = token >= 0 && token < p.tokens && columns_left > 0;
-      copy8<T, FAST>(row_to + stage + i * kRowStep * 128,
-                     in ? x + token * p.row_stride : static_cast<const T*>(p.rows_in), in ? columns_left : 0);
-    }
-    const int slot0 = begin + tile * S::kTokens;
-#pragma unroll
-    for (int i = 0; i < kLowCopies; ++i) {
-      const int at = low_row + i * kLowStep, plane = at / S::kTokens, row = at % S::kTokens;
-      if (2 * S::kTokens % kLowStep != 0 && at >= 2 * S::kTokens) continue;
-      const bool in = low_in && slot0 + row < end;
-      cp_async16(stages + stage + S::kRowBytes + plane * S::kPlaneBytes + paneled(row, low_piece, S::kTokens * 16),
-                 in ? low + (plane * p.slots + slot0 + row) * p.rank_pad : low, in);
-    }
-  };
-
-#pragma unroll
-  for (int i = 0; i < 2 * S::kAhead; ++i) look(first + i);
-  cp_async_commit();
-  cp_async_wait<0>();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-#pragma unroll
-  for (int i = 0; i < S::kAhead; ++i) {
-    if (first + i < last) load(first + i);
-    cp_async_commit();
-  }
   const uint32_t accumulator = ring.tensor_memory;
-  constexpr uint32_t kInstruction = idesc_f16<T>(128, RANK, true, true);
-  for (int tile = first; tile < last; ++tile) {
-    cp_async_wait<S::kAhead - 1>();
-    fence_proxy_async_smem();
-    __syncthreads();
-    if (tid == 0) {
-      const uint32_t rows = stages + static_cast<uint32_t>((tile - first) % S::kStages) * S::kStageBytes;
+
+  if (warp < 8) {
+    constexpr int kRowCopies = S::kTokens / 8;  // a warp copies rows warp, warp + 8, ...: whole lines
+    static_assert(S::kColumns == 32 * 8, "a lane copies one piece of a row");
+    constexpr int kLowPieces = RANK / 8, kLowStep = kFillThreads / kLowPieces;
+    constexpr int kLowCopies = (2 * S::kTokens + kLowStep - 1) / kLowStep;
+    const int columns_left = static_cast<int>(min(p.width - column0, static_cast<int64_t>(S::kColumns))) - lane * 8;
+    const T* x = static_cast<const T*>(p.rows_in) + (columns_left > 0 ? column0 + lane * 8 : 0);
+    const uint32_t row_to = stages + lane / 8 * S::kSubBytes + swizzled(warp, lane % 8);
+    const int low_piece = tid % kLowPieces, low_row = tid / kLowPieces;
+    const bool low_in = rank0 + low_piece * 8 < p.rank_pad;
+    const T* low = static_cast<const T*>(p.low) + (low_in ? rank0 + low_piece * 8 : 0);
+    const uint32_t low_to = stages + S::kRowBytes;
+
+    // Tokens of the warp's rows of 8 tiles, one a lane, read 8 tiles ahead.
+    auto look = [&](int tile) {
+      const int slot = begin + (tile + lane / kRowCopies) * S::kTokens + warp + lane % kRowCopies * 8;
+      if (slot >= end) return -1;
+      const int32_t token = p.rows[slot];
+      return token < p.tokens ? token : -1;
+    };
+    constexpr int kBatch = 32 / kRowCopies;
+    int32_t tokens = look(first), next_tokens = look(first + kBatch);
+    for (int tile = first; tile < last; ++tile) {
+      const int fill = tile - first;
+      if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+      const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
+      if (fill > 0 && fill % kBatch == 0) {
+        tokens = next_tokens;
+        next_tokens = look(tile + kBatch);
+      }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int i = 0; i < kRowCopies; ++i) {
+        const int32_t token = __shfl_sync(0xffffffffu, tokens, fill % kBatch * kRowCopies + i);
+        copy8<T, FAST>(row_to + stage + i * 8 * 128, x + static_cast<int64_t>(max(token, 0)) * p.row_stride,
+                       token >= 0 ? columns_left : 0);
+      }
+      const int slot0 = begin + tile * S::kTokens;
 #pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
+      for (int i = 0; i < kLowCopies; ++i) {
+        const int at = low_row + i * kLowStep, plane = at / S::kTokens, row = at % S::kTokens;
+        if (2 * S::kTokens % kLowStep != 0 && at >= 2 * S::kTokens) continue;
+        const bool in = low_in && slot0 + row < end;
+        cp_async16(low_to + stage + plane * S::kPlaneBytes + paneled(row, low_piece, S::kTokens * 16),
+                   low + (in ? (plane * p.slots + slot0 + row) * p.rank_pad : 0), in);
+      }
+      ring.filled<FAST>(fill);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+  } else {
+    constexpr uint32_t kInstruction = idesc_f16<T>(128, RANK, true, true);
+    // Groups of 8 slots are 1024 bytes apart, runs of 64 columns kSubBytes.
+    const uint64_t a = smem_desc(stages, S::kSubBytes, 1024, 2);
+    const uint64_t b = smem_desc(stages + S::kRowBytes, 128, S::kTokens * 16, 0);
+    ring.multiply(last - first, p.watchdog, [&](int fill) {
+      // Addresses advance in the descriptors' units of 16 bytes.
+      const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
 #pragma unroll
-          for (int k = 0; k < S::kTokens / 16; ++k) {
-            // Groups of 8 slots are 1024 bytes apart, the two runs of 64 columns kSubBytes.
-            const uint64_t a = smem_desc(rows + half * 2 * S::kSubBytes + k * 2048, S::kSubBytes, 1024, 2);
-            const uint64_t b = smem_desc(rows + S::kRowBytes + plane * S::kPlaneBytes + k * 256, 128, S::kTokens * 16, 0);
-            mma_bf16(accumulator + half * RANK, a, b, kInstruction, tile > first || plane > 0 || k > 0);
+      for (int plane = 0; plane < 2; ++plane) {
+#pragma unroll
+        for (int k = 0; k < S::kTokens / 16; ++k) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            mma_bf16(accumulator + half * RANK, a + stage + half * (2 * S::kSubBytes / 16) + k * 128,
+                     b + stage + plane * (S::kPlaneBytes / 16) + k * 16, kInstruction, fill > 0 || plane > 0 || k > 0);
           }
         }
       }
-      tc_commit(&ring.used[(tile - first) % S::kStages]);
-    }
-    __syncwarp();
-    if (tile + S::kAhead < last) {
-      constexpr int kBehind = S::kStages - S::kAhead;
-      if (tile - first >= kBehind) ring.wait(tile - first - kBehind, p.watchdog);
-      load(tile + S::kAhead);
-    }
-    look(tile + 2 * S::kAhead);
-    cp_async_commit();
+    });
   }
-
-  cp_async_wait<0>();
   float* part = reinterpret_cast<float*>(shared);
-  if (first < last) {
-    ring.wait(last - 1 - first, p.watchdog);
-    if (ring.abort != 0 && tid == 0) ring.drain(last - 1 - first);
-  }
+  if (first < last) ring.wait(ring.used, last - 1 - first, p.watchdog);
   tc_fence_after();
   __syncthreads();
-  {
+  if (warp < 8) {
     const int half = warp / 4, c = half * 128 + warp % 4 * 32 + lane;
     store_part<RANK>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * RANK,
                      first < last);
@@ -876,7 +885,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  if (warp == 0) tmem_dealloc(accumulator, S::kTensorColumns);
+  if (warp == 8) tmem_dealloc(accumulator, S::kTensorColumns);
   // Each block adds up its share of the columns, beside its own sums (which
   // the others may still be reading), then writes it in memory order.
   const int share = (S::kColumns + static_cast<int>(splits) - 1) / static_cast<int>(splits);
