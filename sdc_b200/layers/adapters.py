@@ -8,11 +8,15 @@ from .. import ops
 
 _OP, _OP_IN_PLACE = ops.low_rank_adapters.default, ops.low_rank_adapters_.default
 
-# Rows of a tile. With at least this many tokens an adapter on average, tiles
-# of 128 rows share one read of the adapter's weights; below, most of their rows
-# would be empty and tiles of 16 do less for the same traffic. Ranks beyond
-# _WIDE_RANK leave no room for wide tiles beside the weight.
-_WIDE_TILE, _NARROW_TILE, _WIDE_FROM, _WIDE_RANK = 128, 16, 32, 128
+# Rows of a tile: 16 (warp-level products, a short start) or 128 (tensor
+# memory, one read of the adapter's weights for all rows). Measured forward
+# passes, narrow against wide: 4 adapters of 128 tokens each at 3584 -> 3584
+# rank 16 15.4 against 19.4 us, of 256 21.5 against 19.4; 32 of 64 27.6 against
+# 27.6, of 128 42.0 against 33.8, of 256 74.8 against 50.2; at 896 -> 4864 rank
+# 64 4 of 256 23.6 against 29.7, 32 of 64 40.0 against 46.1, of 128 74.8
+# against 56.3. Ranks beyond _WIDE_RANK leave no room for wide tiles beside
+# the weight.
+_WIDE_TILE, _NARROW_TILE, _WIDE_FROM, _WIDE_SLOTS, _WIDE_RANK = 128, 16, 96, 1536, 128
 
 
 def _tiles(offsets, tokens, rows):
@@ -60,7 +64,7 @@ class AdapterBatch:
         rows = np.argsort(of_token, kind="stable").astype(np.int32)
         narrow, narrow_active = _tiles(offsets, tokens, _NARROW_TILE)
         wide, wide_active = narrow[:0], 0
-        if used and slots >= _WIDE_FROM * used:
+        if slots >= max(_WIDE_SLOTS, _WIDE_FROM * used):
             wide, wide_active = _tiles(offsets, tokens, _WIDE_TILE)
         packed = torch.from_numpy(np.concatenate((rows, offsets.astype(np.int32), narrow.reshape(-1),
                                                   wide.reshape(-1)))).to(device)

@@ -13,7 +13,7 @@ from sdc_b200.layers import (AdapterBatch, distillation_loss, head_norm_rotary, 
 
 @pytest.mark.parametrize("lengths,adapters,count", [
     ([], [], 1), ([0, 0], [0, -1], 2), ([1], [0], 1), ([5], [-1], 3), ([1] * 30, [i % 7 - 1 for i in range(30)], 8),
-    ([100, 3, 0, 250, 64], [1, 0, 1, 1, -1], 2), ([63, 64, 65, 128], [0, 1, 2, 3], 4)])
+    ([100, 3, 0, 250, 64], [1, 0, 1, 1, -1], 2), ([1000, 3, 0, 2500, 64], [1, 0, 1, 1, -1], 2), ([63, 64, 65, 128], [0, 1, 2, 3], 4)])
 def test_adapter_batch_lists_every_token_once_under_its_adapter(lengths, adapters, count):
     batch = AdapterBatch(lengths, adapters, count, device="cpu")
     of_token = np.repeat(np.asarray(adapters, dtype=np.int64), lengths)

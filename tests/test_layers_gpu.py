@@ -225,6 +225,13 @@ ADAPTER_CASES = [
     ([130], [0], 1, 256, 264, 136),
     ([12], [-1], 2, 16, 64, 64),                  # nothing adapted
     ([1000, 500], [0, 1], 2, 32, 896, 520),
+    # Tiles of 128 rows: ranks of each kind, odd widths, unused adapters, tokens without one between.
+    ([1000, 37, 700, 0], [0, -1, 1, 1], 3, 16, 320, 264),
+    ([2000], [0], 1, 64, 136, 72),
+    ([901, 800, 13], [1, 0, 1], 2, 5, 104, 1000),
+    ([1700], [0], 1, 24, 37, 53),
+    ([1024, 640], [0, 1], 2, 100, 200, 136),
+    ([1600], [0], 1, 256, 264, 136),
     ([2] * 40, list(range(40)), 40, 16, 1032, 904),
 ]
 
