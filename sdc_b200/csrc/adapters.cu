@@ -503,66 +503,55 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
 
 // ------------------------------------------------------------------ expand ----
 
-// ROWS kWide: a warp takes 16 rows of 256 columns; ROWS kNarrow: all 16 rows of 32 of
-// 128 columns. A thread's accumulators over four 8-column tiles are made 8
+// Tiles of 16 rows: bound by the weight, of which each block reads 128 columns
+// (with base, before it waits for `low`). Four warps, each all 16 rows of 32
+// columns. A thread's accumulators over four 8-column tiles are made 8
 // neighbouring columns by assigning column 8 q + 2 j + b of 32 to element
 // 2 q + b of tile j: base and out then move in 16-byte words straight between
 // registers and memory.
-template <int ROWS>
-struct ExpandShape {
-  static constexpr int kThreads = ROWS == kWide ? 256 : 128;
-  static constexpr int kBlocks = ROWS == kWide ? 2 : 4;  // at least, on an SM
-  static constexpr int kColumns = ROWS == kWide ? 256 : 128;
-  static constexpr int kGroups = ROWS == kWide ? 8 : 1;  // 32-column groups per warp
+//
+// Shared layout of the weight: !TRANS (weight [width, rank]): rows of a column's
+// ranks and 8 elements of padding, each run of 8 columns skewed by 32 bytes so
+// that the 8 rows of a fragment (columns 0, 1, 8, 9, 16, ... of a group) hit
+// different banks. TRANS (weight [rank, width]): rows of permuted columns.
+struct NarrowExpand {
+  static constexpr int kThreads = 128;
+  static constexpr int kColumns = 128;
+  static constexpr int kTransPitch = (kColumns + 8) * 2;
+  static __host__ __device__ constexpr int group_bytes(int pad) { return 32 * (pad + 8) * 2 + 96; }
+  static __host__ __device__ constexpr int weight_bytes(int pad, bool trans) {
+    return trans ? pad * kTransPitch : kColumns / 32 * group_bytes(pad);
+  }
+  static __host__ __device__ constexpr int bytes(int pad, bool trans) {
+    return weight_bytes(pad, trans) + 2 * kNarrow * (pad + 8) * 2;
+  }
 };
 
-// Shared layout of the weight: !TRANS (weight [width, rank]): column-major
-// rows of rank_pad + 8 elements, each run of 8 columns skewed by 32 bytes so
-// that the 8 rows of a fragment (columns 0, 1, 8, 9, 16, ... of a group) hit
-// different banks. TRANS (weight [rank, width]): rank_pad rows of permuted
-// columns.
-__host__ __device__ constexpr int expand_group_bytes(int rank_pad) { return 32 * (rank_pad + 8) * 2 + 96; }
-__host__ __device__ constexpr int expand_weight_bytes(int columns, int rank_pad, bool trans) {
-  return trans ? rank_pad * (columns + 8) * 2 : columns / 32 * expand_group_bytes(rank_pad);
-}
-// Two tiles' low rows, or one where two do not fit.
-__host__ __device__ constexpr int low_buffers(int rank_pad) { return rank_pad <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int expand_bytes(int rows, int columns, int rank_pad, bool trans) {
-  return expand_weight_bytes(columns, rank_pad, trans) + low_buffers(rank_pad) * 2 * rows * (rank_pad + 8) * 2;
-}
-
-// A block keeps 256 columns of one adapter's weight in shared memory and walks
-// a run of tiles: the next tile's low rows are copied and its part of base is
-// loaded into registers as soon as the current one's has been used, so loads
-// never stop. FAST: widths, strides and addresses allow 16-byte accesses
-// throughout. PAD: rank_pad, or 0 where it is read from the parameters.
-template <typename T, int ROWS, bool TRANS, bool FAST, int PAD>
-__global__ void __launch_bounds__(ExpandShape<ROWS>::kThreads, ExpandShape<ROWS>::kBlocks) adapter_expand(AdapterParams p) {
-  using S = ExpandShape<ROWS>;
+// FAST: widths, strides and addresses allow 16-byte accesses throughout. PAD:
+// rank_pad, or 0 where it is read from the parameters.
+template <typename T, bool TRANS, bool FAST, int PAD>
+__global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(AdapterParams p) {
+  using S = NarrowExpand;
   extern __shared__ __align__(16) uint8_t shared[];
   const int pad = PAD > 0 ? PAD : p.rank_pad;
   const int width = static_cast<int>(p.width);
   const int column_blocks = (width + S::kColumns - 1) / S::kColumns;
-  const int run = static_cast<int>(blockIdx.x) / column_blocks;
-  const int column0 = (static_cast<int>(blockIdx.x) - run * column_blocks) * S::kColumns;
-  const int first = run * p.tiles_per_block, last = min(first + p.tiles_per_block, p.tile_count);
+  const Tile tile = p.tiles[blockIdx.x / column_blocks];
+  const int column0 = static_cast<int>(blockIdx.x % column_blocks) * S::kColumns;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pitch = (pad + 8) * 2;  // bytes of a low row, and of a weight row when !TRANS
-  const int group_bytes = expand_group_bytes(pad);
-  constexpr int kTransPitch = (S::kColumns + 8) * 2;
+  const int group_bytes = S::group_bytes(pad);
   const uint32_t weight_shared = smem_u32(shared);
-  const uint32_t low_shared = weight_shared + expand_weight_bytes(S::kColumns, pad, TRANS);
-  const uint32_t low_bytes = 2 * ROWS * pitch;  // of one tile
-  const bool two_buffers = low_buffers(pad) == 2;
+  const uint32_t low_shared = weight_shared + S::weight_bytes(pad, TRANS);
   const int piece_bits = PAD > 0 ? (PAD <= 16 ? 1 : PAD <= 32 ? 2 : 3) : p.piece_bits;
   const int piece = tid & ((1 << piece_bits) - 1), piece_row = tid >> piece_bits;
   const int piece_step = S::kThreads >> piece_bits;
+  const bool adapted = tile.adapter >= 0 && tile.adapter < p.adapters;
 
-  auto load_weight = [&](int adapter) {
-    const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
+  if (adapted) {
+    const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(tile.adapter) * p.rank * p.width;
     if constexpr (!TRANS) {
-      if (piece * 8 >= pad) return;
-      for (int c = piece_row; c < S::kColumns; c += piece_step) {
+      for (int c = piece_row; c < S::kColumns && piece * 8 < pad; c += piece_step) {
         const uint32_t to = weight_shared + (c >> 5) * group_bytes + (c & 31) * pitch + ((c >> 3) & 3) * 32 + piece * 16;
         const int in = column0 + c < width ? p.rank - piece * 8 : 0;
         copy8<T, FAST>(to, in > 0 ? weight + static_cast<int64_t>(column0 + c) * p.rank + piece * 8 : weight, in);
@@ -583,176 +572,361 @@ __global__ void __launch_bounds__(ExpandShape<ROWS>::kThreads, ExpandShape<ROWS>
             if (j < left) e[j] = from[j];
           }
         }
-        const uint32_t to = weight_shared + r * kTransPitch + (c & ~31) * 2 + ((c >> 3) & 3) * 4;
+        const uint32_t to = weight_shared + r * S::kTransPitch + (c & ~31) * 2 + ((c >> 3) & 3) * 4;
         asm volatile("st.shared.b32 [%0], %1;\n\tst.shared.b32 [%0 + 16], %2;\n\t"
                      "st.shared.b32 [%0 + 32], %3;\n\tst.shared.b32 [%0 + 48], %4;" ::"r"(to), "r"(w.x), "r"(w.y),
                      "r"(w.z), "r"(w.w)
                      : "memory");
       }
     }
-  };
-  auto load_low = [&](const Tile& tile, int buffer) {
-    if (piece * 8 >= pad) return;
-    const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * pad + piece * 8;
-    const uint32_t to = low_shared + buffer * low_bytes + piece * 16;
-    for (int i = piece_row; i < 2 * ROWS; i += piece_step) {
-      const int row = i % ROWS;
-      const bool in = row < tile.count;
-      cp_async16(to + i * pitch, in ? from + (i >= ROWS ? p.slots * pad : 0) + row * pad : from, in);
-    }
-  };
-  auto adapted = [&](const Tile& tile) { return tile.adapter >= 0 && tile.adapter < p.adapters; };
+  }
 
-  // This thread's part of base and out: rows lane / 4 and lane / 4 + 8 of its
-  // 16, 8 columns of each 32.
-  const int row0 = (ROWS == kWide ? warp * 16 : 0) + (lane >> 2);
-  const int column = column0 + (ROWS == kWide ? 0 : warp * 32) + (lane & 3) * 8;
-  const int columns_left = width - column;  // column + 32 g + j lies in the matrix when 32 g + j is less
-  struct Rows {
-    const T* base[2];
-    T* out[2];
-    int base_limit[2], out_limit[2];  // columns_left where there is a base and a row, else 0
-  };
-  auto look = [&](const Tile& tile) {
-    Rows r;
+  // This thread's part of base and out: rows lane / 4 and lane / 4 + 8, 8
+  // columns of the warp's 32. The accumulators start from it.
+  const int column = column0 + warp * 32 + (lane & 3) * 8;
+  float acc[4][4];
+  T* out[2];
+  int limit[2];  // columns of out; 0 where there is no row
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t token = row0 + 8 * h < tile.count ? token_of(p, tile.start + row0 + 8 * h) : -1;
-      r.base[h] = static_cast<const T*>(p.base) + token * p.base_stride + column;
-      r.out[h] = static_cast<T*>(p.out) + token * p.out_stride + column;
-      r.out_limit[h] = token >= 0 ? columns_left : 0;
-      r.base_limit[h] = p.base != nullptr ? r.out_limit[h] : 0;
+  for (int h = 0; h < 2; ++h) {
+    const int row = (lane >> 2) + 8 * h;
+    const int64_t token = row < tile.count ? token_of(p, tile.start + row) : -1;
+    limit[h] = token >= 0 ? width - column : 0;
+    out[h] = static_cast<T*>(p.out) + token * p.out_stride + column;
+    Raw8<T> base;
+    base.w[0] = make_uint4(0, 0, 0, 0);
+    const T* from = static_cast<const T*>(p.base) + token * p.base_stride + column;
+    if (p.base != nullptr) {
+      if constexpr (FAST) {
+        if (limit[h] > 0) base = load8(from);
+      } else {
+        T* e = reinterpret_cast<T*>(&base);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < limit[h]) e[j] = from[j];
+        }
+      }
     }
-    return r;
-  };
-  auto load_base = [&](const Rows& rows, int h, int g) {
-    Raw8<T> r;
-    r.w[0] = make_uint4(0, 0, 0, 0);
-    if constexpr (FAST) {
-      if (32 * g < rows.base_limit[h]) r = load8(rows.base[h] + 32 * g);
+    float v[8];
+    unpack8(base, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j][2 * h] = v[2 * j], acc[j][2 * h + 1] = v[2 * j + 1];
+  }
+
+  griddep_wait();  // `low` from here on
+  if (adapted) {
+    const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * pad + piece * 8;
+    for (int i = piece_row; i < 2 * kNarrow && piece * 8 < pad; i += piece_step) {
+      const int row = i % kNarrow;
+      const bool in = row < tile.count;
+      cp_async16(low_shared + i * pitch + piece * 16, in ? from + (i >= kNarrow ? p.slots * pad : 0) + row * pad : from, in);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    const uint32_t low = low_shared + (lane & 15) * pitch + (lane >> 4) * 16;
+    auto step = [&](int k) {
+      uint32_t hi[4], lo[4];
+      ldmatrix_x4(hi, low + k * 2);
+      ldmatrix_x4(lo, low + kNarrow * pitch + k * 2);
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair) {
+        uint32_t b[4];
+        const int i = lane & 7, j = 2 * pair + (lane >> 4), c = (i >> 1) * 8 + j * 2 + (i & 1);
+        if constexpr (!TRANS) {
+          ldmatrix_x4(b, weight_shared + warp * group_bytes + c * pitch + (c >> 3) * 32 + ((lane >> 3) & 1) * 16 + k * 2);
+        } else {
+          ldmatrix_x4_trans(b, weight_shared + (((lane >> 3) & 1) * 8 + i + k) * S::kTransPitch + warp * 64 + j * 16);
+        }
+        mma_16816<T>(acc[2 * pair], hi, b);
+        mma_16816<T>(acc[2 * pair + 1], hi, b + 2);
+        mma_16816<T>(acc[2 * pair], lo, b);
+        mma_16816<T>(acc[2 * pair + 1], lo, b + 2);
+      }
+    };
+    if constexpr (PAD > 0) {
+#pragma unroll
+      for (int k = 0; k < PAD; k += 16) step(k);
     } else {
-      T* e = reinterpret_cast<T*>(&r);
+      for (int k = 0; k < pad; k += 16) step(k);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[2 * j] = acc[j][2 * h], v[2 * j + 1] = acc[j][2 * h + 1];
+    if constexpr (FAST) {
+      if (limit[h] > 0) store8(out[h], pack8<T>(v));
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (32 * g + j < rows.base_limit[h]) e[j] = rows.base[h][32 * g + j];
+        if (j < limit[h]) out[h][j] = from_float<T>(v[j]);
       }
     }
-    return r;
-  };
+  }
+}
 
-  Tile tile = p.tiles[first];
-  Rows rows = look(tile), next_rows{};
-  Raw8<T> part[S::kGroups][2];
-#pragma unroll
-  for (int g = 0; g < S::kGroups; ++g) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) part[g][h] = load_base(rows, h, g);
-  }
-  int adapter = -1;  // whose weight is in shared memory
-  if (adapted(tile)) load_weight(adapter = tile.adapter);
-  griddep_wait();  // `low` from here on
-  if (adapted(tile)) load_low(tile, 0);
-  cp_async_commit();
-  Tile next = first + 1 < last ? p.tiles[first + 1] : Tile{0, 0, -1};
-  // Fragment addresses: low rows, and the weight's columns in the order above.
-  const uint32_t low_from = low_shared + ((ROWS == kWide ? warp * 16 : 0) + (lane & 15)) * pitch + (lane >> 4) * 16;
-  uint32_t weight_from[2];
-#pragma unroll
-  for (int pair = 0; pair < 2; ++pair) {
-    const int i = lane & 7, j = 2 * pair + (lane >> 4), c = (i >> 1) * 8 + j * 2 + (i & 1);
-    weight_from[pair] = weight_shared + (TRANS ? (((lane >> 3) & 1) * 8 + i) * kTransPitch + pair * 32 + (lane >> 4) * 16
-                                               : c * pitch + (c >> 3) * 32 + ((lane >> 3) & 1) * 16);
-    if (ROWS == kNarrow) weight_from[pair] += warp * (TRANS ? 64 : group_bytes);
-  }
-  for (int t = first; t < last; ++t) {
-    const int buffer = two_buffers ? (t - first) & 1 : 0;
-    const bool more = t + 1 < last;
-    const Tile after = t + 2 < last ? p.tiles[t + 2] : Tile{0, 0, -1};
-    next_rows = look(next);
-    if (two_buffers && more && adapted(next)) load_low(next, buffer ^ 1);
-    cp_async_commit();
-    if (adapted(tile) && tile.adapter != adapter) {
-      __syncthreads();  // the last tile's products are done with the old weight
-      load_weight(adapter = tile.adapter);
-      cp_async_commit();
-      cp_async_wait<0>();
-    } else {
-      cp_async_wait<1>();
+// ---- expand of wide tiles ----
+
+// A block keeps 256 columns of one adapter's weight in shared memory and walks
+// a run of tiles. D [128 rows, 256 columns] in tensor memory is the product of
+// a tile's two low planes (A, K-major panels) with the weight (B); eight warps
+// add it to base, 32 columns of 16 rows at a time: a 16x256b load gives a
+// thread rows lane / 4 and lane / 4 + 8 and two columns of each 8. The weight's
+// columns are permuted within 32 (column 8 q + 2 j + b stands at 8 j + 2 q + b)
+// so that these are 8 neighbours, and base and out move in 16-byte words. The
+// next tile's part of base is loaded as soon as the current one's has been
+// used, its low rows while the current tile is worked on.
+struct ExpandWide {
+  static constexpr int kThreads = kFillThreads;
+  static constexpr int kColumns = 256;
+  static constexpr int kWarps = 8, kHalves = 2, kGroups = 4;  // a warp: 32 rows of 128 columns
+  static constexpr int kWeightStep = kColumns * 16, kLowStep = kWide * 16;  // bytes of 8 ranks
+  static __host__ __device__ constexpr int weight_bytes(int pad) { return pad / 8 * kWeightStep; }
+  static __host__ __device__ constexpr int low_bytes(int pad) { return 2 * (pad / 8) * kLowStep; }  // of one tile
+  static __host__ __device__ constexpr int bytes(int pad) { return weight_bytes(pad) + 2 * low_bytes(pad); }
+};
+
+// 16 rows of 32 columns: v[4 j ..] are tile j's (row lane / 4: two columns;
+// row lane / 4 + 8: the same).
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t address, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(address));
+}
+
+template <typename T, bool TRANS, bool FAST>
+__global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(AdapterParams p) {
+  using S = ExpandWide;
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ uint64_t loaded[2], ready, drained;
+  __shared__ uint32_t tensor_memory;
+  __shared__ int32_t abort;
+  const int width = static_cast<int>(p.width), pad = p.rank_pad, pieces = pad / 8;
+  const int column_blocks = (width + S::kColumns - 1) / S::kColumns;
+  const int run = static_cast<int>(blockIdx.x) / column_blocks;
+  const int column0 = (static_cast<int>(blockIdx.x) - run * column_blocks) * S::kColumns;
+  const int first = run * p.tiles_per_block, last = min(first + p.tiles_per_block, p.tile_count);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t weight_shared = smem_u32(shared), low_shared = weight_shared + S::weight_bytes(pad);
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(&loaded[0], kFillThreads);
+      mbar_init(&loaded[1], kFillThreads);
+      mbar_init(&ready, 1);
+      mbar_init(&drained, S::kWarps);
+      fence_barrier_init();
+      abort = 0;
     }
-    __syncthreads();
-    const uint32_t low = low_from + buffer * low_bytes;
-    auto group = [&](int g, bool mine) {
-      float acc[4][4];  // base, to which the products are added
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-        unpack8(part[g][h], v);
-        part[g][h] = load_base(next_rows, h, g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[j][2 * h] = v[2 * j];
-          acc[j][2 * h + 1] = v[2 * j + 1];
+    __syncwarp();
+    tmem_alloc(&tensor_memory, S::kColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t accumulator = tensor_memory;
+  // False for the whole warp once a wait of the block has run out: the warps
+  // then leave their loops one after the other and meet at the last barrier.
+  auto wait = [&](uint64_t* bar, int index) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, static_cast<uint32_t>(index) & 1, kWaitAccum, &abort, p.watchdog)) != 0;
+  };
+  auto adapted = [&](const Tile& tile) { return tile.adapter >= 0 && tile.adapter < p.adapters; };
+  constexpr Tile kNone{0, 0, -1};
+
+  // Warp 0, one lane: a tile's product, once its operands are there and the
+  // last one has been read.
+  auto multiply = [&](int product) {
+    if (!wait(&loaded[product & 1], product >> 1) || (product > 0 && !wait(&drained, product - 1))) return;
+    fence_proxy_async_smem();  // the copies were made by ordinary writes
+    tc_fence_after();
+    if (lane == 0) {
+      constexpr uint32_t kInstruction = idesc_f16<T>(kWide, S::kColumns, false, TRANS);
+      // K-major panels: rows of 8 ranks, groups of 8 rows 128 bytes apart; the weight [rank, width] by columns.
+      const uint64_t a = smem_desc(low_shared + (product & 1) * S::low_bytes(pad), S::kLowStep, 128, 0);
+      const uint64_t b = TRANS ? smem_desc(weight_shared, 128, pad * 16, 0) : smem_desc(weight_shared, S::kWeightStep, 128, 0);
+      constexpr int kStep = (TRANS ? 256 : 2 * S::kWeightStep) / 16;
+      for (int plane = 0; plane < 2; ++plane) {
+        for (int k = 0; k < pad / 16; ++k) {
+          mma_bf16(accumulator, a + (plane * pieces + 2 * k) * (S::kLowStep / 16), b + k * kStep, kInstruction,
+                   plane > 0 || k > 0);
         }
       }
-      if (mine) {
-        auto step = [&](int k) {
-          uint32_t hi[4], lo[4];
-          ldmatrix_x4(hi, low + k * 2);
-          ldmatrix_x4(lo, low + ROWS * pitch + k * 2);
+      tc_commit(&ready);
+    }
+    __syncwarp();
+  };
+  int products = 0;
+  {
+    // Copies by these 256 threads; each arrives once for every product.
+    auto load_low = [&](const Tile& tile, int product) {
+      const T* from = static_cast<const T*>(p.low) + static_cast<int64_t>(tile.start) * pad;
+      const uint32_t to = low_shared + (product & 1) * S::low_bytes(pad);
+      const int row = tid & 127, plane = tid >> 7;
+      const bool in = row < tile.count;
+      const T* source = from + (in ? (plane * p.slots + row) * pad : 0);
+      for (int i = 0; i < pieces; ++i) {
+        cp_async16(to + (plane * pieces + i) * S::kLowStep + row * 16, source + i * 8, in);
+      }
+    };
+    auto load_weight = [&](int adapter) {
+      const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
+      if constexpr (!TRANS) {
+        const int c = tid;  // one column a thread
+        const int at = (c & ~31) + c % 8 / 2 * 8 + c / 8 % 4 * 2 + (c & 1);
+        for (int i = 0; i < pieces; ++i) {
+          const int in = column0 + c < width ? p.rank - i * 8 : 0;
+          copy8<T, FAST>(weight_shared + i * S::kWeightStep + at * 16,
+                         in > 0 ? weight + static_cast<int64_t>(column0 + c) * p.rank + i * 8 : weight, in);
+        }
+      } else {
+        for (int i = tid; i < pad * (S::kColumns / 8); i += kFillThreads) {
+          const int r = i / (S::kColumns / 8), c = i % (S::kColumns / 8) * 8;
+          const T* from = weight + r * p.width + column0 + c;
+          const int left = r < p.rank ? width - (column0 + c) : 0;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if constexpr (FAST) {
+            if (left > 0) w = *reinterpret_cast<const uint4*>(from);
+          } else {
+            T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-          for (int pair = 0; pair < 2; ++pair) {
-            uint32_t b[4];
-            if constexpr (!TRANS) ldmatrix_x4(b, weight_from[pair] + g * group_bytes + k * 2);
-            else ldmatrix_x4_trans(b, weight_from[pair] + g * 64 + k * kTransPitch);
-            mma_16816<T>(acc[2 * pair], hi, b);
-            mma_16816<T>(acc[2 * pair + 1], hi, b + 2);
-            mma_16816<T>(acc[2 * pair], lo, b);
-            mma_16816<T>(acc[2 * pair + 1], lo, b + 2);
+            for (int j = 0; j < 8; ++j) {
+              if (j < left) e[j] = from[j];
+            }
           }
-        };
-        if constexpr (PAD > 0) {
+          // Panels of 8 columns: pair j of these 8 goes to panel j of its 32 columns, at 2 (c / 8 % 4).
+          const uint32_t to = weight_shared + (c / 32 * 4) * (pad * 16) + r * 16 + c / 8 % 4 * 4;
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int k = 0; k < PAD; k += 16) step(k);
-        } else {
-          for (int k = 0; k < pad; k += 16) step(k);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] = acc[j][2 * h];
-          v[2 * j + 1] = acc[j][2 * h + 1];
-        }
-        T* to = rows.out[h] + 32 * g;
-        if constexpr (FAST) {
-          if (32 * g < rows.out_limit[h]) store8(to, pack8<T>(v));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (32 * g + j < rows.out_limit[h]) to[j] = from_float<T>(v[j]);
+          for (int j = 0; j < 4; ++j) {
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + j * (pad * 16)), "r"(words[j]) : "memory");
           }
         }
       }
     };
-    if (adapted(tile)) {
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) group(g, true);
-    } else {
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) group(g, false);
-    }
-    if (!two_buffers) {
-      __syncthreads();
-      if (more && adapted(next)) load_low(next, 0);
+    int adapter = -1;  // whose weight is in shared memory
+    auto load = [&](const Tile& tile, int product) {
+      if (!adapted(tile)) return;
+      load_low(tile, product);
+      if (tile.adapter == adapter) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&loaded[product & 1])) : "memory");
+        return;
+      }
+      load_weight(adapter = tile.adapter);
       cp_async_commit();
       cp_async_wait<0>();
+      mbar_arrive(&loaded[product & 1]);
+    };
+
+    // This thread's rows of a tile, two of each half of its warp's 32, and columns.
+    const int quarter = warp % 4, row0 = quarter * 32 + (lane >> 2);
+    const int column = column0 + warp / 4 * 128 + (lane & 3) * 8, columns_left = width - column;
+    auto look = [&](const Tile& tile, int32_t (&token)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        token[i] = row0 + 8 * i < tile.count ? static_cast<int32_t>(token_of(p, tile.start + row0 + 8 * i)) : -1;
+      }
+    };
+    auto load_base = [&](int32_t token, int g) {
+      Raw8<T> r;
+      r.w[0] = make_uint4(0, 0, 0, 0);
+      const T* from = static_cast<const T*>(p.base) + static_cast<int64_t>(token) * p.base_stride + column + 32 * g;
+      const int limit = p.base != nullptr && token >= 0 ? columns_left - 32 * g : 0;
+      if constexpr (FAST) {
+        if (limit > 0) r = load8(from);
+      } else {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < limit) e[j] = from[j];
+        }
+      }
+      return r;
+    };
+    Tile tile = p.tiles[first], next = first + 1 < last ? p.tiles[first + 1] : kNone;
+    int32_t token[4], next_token[4];
+    look(tile, token);
+    Raw8<T> part[S::kHalves][S::kGroups][2];
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+#pragma unroll
+      for (int g = 0; g < S::kGroups; ++g) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) part[half][g][h] = load_base(token[2 * half + h], g);
+      }
     }
-    tile = next;
-    next = after;
-    rows = next_rows;
+    load(tile, 0);
+    int product = 0;  // of the current tile, if it has one
+    for (int t = first; t < last; ++t) {
+      const bool mine = adapted(tile);
+      const int next_product = product + mine;
+      // The next tile's low rows go where those of the product before this
+      // one were (it has completed); a new weight waits for this product.
+      const bool early = !mine || next.adapter == adapter;
+      if (early) load(next, next_product);
+      look(next, next_token);
+      if (mine && warp == 0) multiply(product);
+      if (mine && !wait(&ready, product)) break;
+      products = next_product;
+      if (!early) load(next, next_product);
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < S::kHalves; ++half) {
+#pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+          uint32_t d[16];
+          if (mine) {
+            tmem_ld_16x256b_x4(accumulator + (static_cast<uint32_t>(quarter * 32 + half * 16) << 16) + warp / 4 * 128 + g * 32, d);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[8];
+            unpack8(part[half][g][h], v);
+            part[half][g][h] = load_base(next_token[2 * half + h], g);
+            if (mine) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[2 * j] += __uint_as_float(d[4 * j + 2 * h]);
+                v[2 * j + 1] += __uint_as_float(d[4 * j + 2 * h + 1]);
+              }
+            }
+            const int32_t row = token[2 * half + h];
+            T* to = static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_stride + column + 32 * g;
+            const int limit = row >= 0 ? columns_left - 32 * g : 0;
+            if constexpr (FAST) {
+              if (limit > 0) store8(to, pack8<T>(v));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                if (j < limit) to[j] = from_float<T>(v[j]);
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (mine && lane == 0) mbar_arrive(&drained);
+      tile = next;
+      next = t + 2 < last ? p.tiles[t + 2] : kNone;
+      product = next_product;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) token[i] = next_token[i];
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
   }
+  if (abort != 0 && tid == 0 && products > 0) mbar_drain(&ready, static_cast<uint32_t>(products - 1) & 1);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(accumulator, S::kColumns);
 }
 
 // ------------------------------------------------------------------- outer ----
@@ -916,9 +1090,8 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
 template <typename Kernel>
 int launch_clustered(Kernel kernel, const AdapterParams& p, dim3 grid, int threads, int cluster, int shared,
                      bool dependent, cudaStream_t stream) {
-  if (shared > 48 * 1024) {
-    SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-  }
+  const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared);
+  if (rc != SDC_OK) return rc;
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(static_cast<unsigned>(threads));
@@ -997,40 +1170,49 @@ int shrink_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tile
   return trans ? shrink_by_rank<T, kNarrow, true>(p, tiles, stream) : shrink_by_rank<T, kNarrow, false>(p, tiles, stream);
 }
 
-template <typename T, int ROWS, bool TRANS>
-int launch_expand(AdapterParams p, int64_t tiles, bool dependent, cudaStream_t stream) {
-  using S = ExpandShape<ROWS>;
-  constexpr int kColumns = S::kColumns;
-  const int64_t column_blocks = ceil_div(p.width, kColumns);
-  // Runs of tiles that fill the SMs' blocks once; tiles of few rows
-  // are bound by the weight, of which each then wants its own.
-  p.tile_count = static_cast<int>(tiles);
-  const int64_t runs = std::max<int64_t>(1, S::kBlocks * sm_count() / column_blocks);
-  p.tiles_per_block = ROWS == kWide ? static_cast<int>(ceil_div(tiles, runs)) : 1;
-  const int64_t blocks = column_blocks * ceil_div(tiles, p.tiles_per_block);
+bool expand_fast(const AdapterParams& p, bool trans) {
+  return p.vector_rows && p.vector_out && p.vector_weight && p.width % 8 == 0 && (trans || p.rank % 8 == 0);
+}
+
+template <typename T, bool TRANS>
+int launch_expand_narrow(AdapterParams p, int64_t tiles, bool dependent, cudaStream_t stream) {
+  using S = NarrowExpand;
+  const int64_t blocks = ceil_div(p.width, S::kColumns) * tiles;
   SDC_REQUIRE(blocks <= INT_MAX, "low-rank adapters have too many tiles for one launch");
   while ((8 << p.piece_bits) < p.rank_pad) ++p.piece_bits;
-  dependent = dependent && ROWS == kNarrow;  // blocks of long runs that start early, where there is room, end late
-  const int shared = expand_bytes(ROWS, kColumns, p.rank_pad, TRANS);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  const bool fast = p.vector_rows && p.vector_out && p.vector_weight && p.width % 8 == 0 && (TRANS || p.rank % 8 == 0);
-  if (!fast) return launch_clustered(adapter_expand<T, ROWS, TRANS, false, 0>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
+  auto launch = [&](auto kernel) {
+    return launch_clustered(kernel, p, dim3(static_cast<unsigned>(blocks)), S::kThreads, 0, S::bytes(p.rank_pad, TRANS),
+                            dependent, stream);
+  };
+  if (!expand_fast(p, TRANS)) return launch(adapter_expand<T, TRANS, false, 0>);
   switch (p.rank_pad) {
-    case 16: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 16>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
-    case 32: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 32>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
-    case 64: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 64>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
-    default: return launch_clustered(adapter_expand<T, ROWS, TRANS, true, 0>, p, grid, ExpandShape<ROWS>::kThreads, 0, shared, dependent, stream);
+    case 16: return launch(adapter_expand<T, TRANS, true, 16>);
+    case 32: return launch(adapter_expand<T, TRANS, true, 32>);
+    case 64: return launch(adapter_expand<T, TRANS, true, 64>);
+    default: return launch(adapter_expand<T, TRANS, true, 0>);
   }
+}
+
+template <typename T, bool TRANS>
+int launch_expand_wide(AdapterParams p, int64_t tiles, cudaStream_t stream) {
+  const int64_t column_blocks = ceil_div(p.width, ExpandWide::kColumns);
+  // Runs of tiles that fill the SMs' two blocks once.
+  const int64_t runs = std::max<int64_t>(1, 2 * sm_count() / column_blocks);
+  p.tile_count = static_cast<int>(tiles);
+  p.tiles_per_block = static_cast<int>(ceil_div(tiles, runs));
+  const int64_t blocks = column_blocks * ceil_div(tiles, p.tiles_per_block);
+  SDC_REQUIRE(blocks <= INT_MAX, "low-rank adapters have too many tiles for one launch");
+  auto launch = [&](auto kernel) {
+    return launch_clustered(kernel, p, dim3(static_cast<unsigned>(blocks)), ExpandWide::kThreads, 0, ExpandWide::bytes(p.rank_pad), false, stream);
+  };
+  return expand_fast(p, TRANS) ? launch(adapter_expand_wide<T, TRANS, true>) : launch(adapter_expand_wide<T, TRANS, false>);
 }
 
 template <typename T>
 int expand_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tiles, bool dependent, cudaStream_t stream) {
-  if (tile_rows == kWide) {
-    return trans ? launch_expand<T, kWide, true>(p, tiles, dependent, stream)
-                 : launch_expand<T, kWide, false>(p, tiles, dependent, stream);
-  }
-  return trans ? launch_expand<T, kNarrow, true>(p, tiles, dependent, stream)
-               : launch_expand<T, kNarrow, false>(p, tiles, dependent, stream);
+  if (tile_rows == kWide) return trans ? launch_expand_wide<T, true>(p, tiles, stream) : launch_expand_wide<T, false>(p, tiles, stream);
+  return trans ? launch_expand_narrow<T, true>(p, tiles, dependent, stream)
+               : launch_expand_narrow<T, false>(p, tiles, dependent, stream);
 }
 
 template <typename T, int RANK>
@@ -1119,6 +1301,8 @@ int sdc_adapter_expand(int dtype, const void* base, int64_t base_stride, int64_t
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
+  p.watchdog = watchdog_ptr();
+  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
   p.tokens = tokens;
   p.rows = rows;
   p.tiles = reinterpret_cast<const Tile*>(tiles);

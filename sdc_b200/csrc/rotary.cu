@@ -519,9 +519,8 @@ int launch_heads(const RotaryParams& p, bool backward, int blocks, cudaStream_t 
     const int shared = VECTOR ? (backward ? std::max(Backward::kStages * Backward::kStageBytes, kSums)
                                           : Forward::kStages * Forward::kStageBytes)
                               : backward ? kSums : 0;
-    if (shared > 48 * 1024) {
-      SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-    }
+    const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared);
+    if (rc != SDC_OK) return rc;
     kernel<<<blocks, kRotaryThreads, shared, stream>>>(p);
     SDC_CUDA_CHECK(cudaGetLastError());
     return SDC_OK;

@@ -80,6 +80,24 @@ int sm_count() {
   return count;
 }
 
+int allow_shared(const void* kernel, int bytes) {
+  if (bytes <= 40 * 1024) return SDC_OK;  // 48 KB, static shared memory included, need no asking
+  // Nothing here allocates (or throws): a kernel that finds its place taken asks again.
+  struct Allowed {
+    const void* kernel = nullptr;
+    int device = -1, bytes = 0;
+  };
+  constexpr int kPlaces = 64;
+  static thread_local Allowed places[kPlaces];
+  int device = 0;
+  SDC_CUDA_CHECK(cudaGetDevice(&device));
+  Allowed& place = places[reinterpret_cast<uintptr_t>(kernel) / 16 % kPlaces];
+  if (place.kernel == kernel && place.device == device && place.bytes >= bytes) return SDC_OK;
+  SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  place = Allowed{kernel, device, bytes};
+  return SDC_OK;
+}
+
 namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
