@@ -68,6 +68,7 @@ struct AdapterParams {
   int chunks_per_split;
   int32_t* watchdog;
   int tile_count, tiles_per_block;  // expand
+  int weights;               // expand of wide tiles: buffers of weights, 1 or 2
   int piece_bits;            // expand: 2^piece_bits >= rank_pad / 8 threads copy a row
 };
 
@@ -685,7 +686,8 @@ struct ExpandWide {
   static constexpr int kWeightStep = kColumns * 16, kLowStep = kWide * 16;  // bytes of 8 ranks
   static __host__ __device__ constexpr int weight_bytes(int pad) { return pad / 8 * kWeightStep; }
   static __host__ __device__ constexpr int low_bytes(int pad) { return 2 * (pad / 8) * kLowStep; }  // of one tile
-  static __host__ __device__ constexpr int bytes(int pad) { return weight_bytes(pad) + 2 * low_bytes(pad); }
+  static __host__ __device__ constexpr int bytes(int pad, int weights) { return weights * weight_bytes(pad) + 2 * low_bytes(pad); }
+  static constexpr int kBlockBytes = 110 * 1024;  // of two blocks on an SM
 };
 
 // 16 rows of 32 columns: v[4 j ..] are tile j's (row lane / 4: two columns;
@@ -712,7 +714,8 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
   const int column0 = (static_cast<int>(blockIdx.x) - run * column_blocks) * S::kColumns;
   const int first = run * p.tiles_per_block, last = min(first + p.tiles_per_block, p.tile_count);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t weight_shared = smem_u32(shared), low_shared = weight_shared + S::weight_bytes(pad);
+  const uint32_t weights_shared = smem_u32(shared), low_shared = weights_shared + p.weights * S::weight_bytes(pad);
+  uint32_t weight_shared = weights_shared;  // the current tile's
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(&loaded[0], kFillThreads);
@@ -773,7 +776,7 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
         cp_async16(to + (plane * pieces + i) * S::kLowStep + row * 16, source + i * 8, in);
       }
     };
-    auto load_weight = [&](int adapter) {
+    auto load_weight = [&](int adapter, uint32_t weight_shared) {
       const T* weight = static_cast<const T*>(p.weight) + static_cast<int64_t>(adapter) * p.rank * p.width;
       if constexpr (!TRANS) {
         const int c = tid;  // one column a thread
@@ -808,7 +811,8 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
         }
       }
     };
-    int adapter = -1;  // whose weight is in shared memory
+    int adapter = -1;  // whose weight was loaded last, and to where
+    uint32_t newest = weights_shared;
     auto load = [&](const Tile& tile, int product) {
       if (!adapted(tile)) return;
       load_low(tile, product);
@@ -816,10 +820,15 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&loaded[product & 1])) : "memory");
         return;
       }
-      load_weight(adapter = tile.adapter);
-      cp_async_commit();
-      cp_async_wait<0>();
-      mbar_arrive(&loaded[product & 1]);
+      if (p.weights == 2 && adapter >= 0) newest = 2 * weights_shared + S::weight_bytes(pad) - newest;  // the other one
+      load_weight(adapter = tile.adapter, newest);
+      if constexpr (FAST && !TRANS) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&loaded[product & 1])) : "memory");
+      } else {  // written by ordinary stores
+        cp_async_commit();
+        cp_async_wait<0>();
+        mbar_arrive(&loaded[product & 1]);
+      }
     };
 
     // This thread's rows of a tile, two of each half of its warp's 32, and columns.
@@ -865,8 +874,10 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       const bool mine = adapted(tile);
       const int next_product = product + mine;
       // The next tile's low rows go where those of the product before this
-      // one were (it has completed); a new weight waits for this product.
-      const bool early = !mine || next.adapter == adapter;
+      // one were (it has completed), a new weight where the one before this
+      // was; with room for one only it waits for this product.
+      weight_shared = newest;
+      const bool early = !mine || next.adapter == adapter || p.weights == 2;
       if (early) load(next, next_product);
       look(next, next_token);
       if (mine && warp == 0) multiply(product);
@@ -1202,8 +1213,11 @@ int launch_expand_wide(AdapterParams p, int64_t tiles, cudaStream_t stream) {
   p.tiles_per_block = static_cast<int>(ceil_div(tiles, runs));
   const int64_t blocks = column_blocks * ceil_div(tiles, p.tiles_per_block);
   SDC_REQUIRE(blocks <= INT_MAX, "low-rank adapters have too many tiles for one launch");
+  // Two buffers of weights where two blocks of an SM have the room (ranks up to 48).
+  p.weights = ExpandWide::bytes(p.rank_pad, 2) <= ExpandWide::kBlockBytes ? 2 : 1;
   auto launch = [&](auto kernel) {
-    return launch_clustered(kernel, p, dim3(static_cast<unsigned>(blocks)), ExpandWide::kThreads, 0, ExpandWide::bytes(p.rank_pad), false, stream);
+    return launch_clustered(kernel, p, dim3(static_cast<unsigned>(blocks)), ExpandWide::kThreads, 0,
+                            ExpandWide::bytes(p.rank_pad, p.weights), false, stream);
   };
   return expand_fast(p, TRANS) ? launch(adapter_expand_wide<T, TRANS, true>) : launch(adapter_expand_wide<T, TRANS, false>);
 }
