@@ -357,19 +357,32 @@ __device__ __forceinline__ float4 sum_cluster(const float* part, int at, uint32_
   }
   return sum;
 }
-// This thread's row of an accumulator (zeros where nothing was multiplied).
-template <int RANK>
+// This thread's row of an accumulator (zeros where nothing was multiplied);
+// PLANES: 2 where RANK further columns hold the second plane's sums.
+template <int RANK, int PLANES>
 __device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any) {
+  constexpr int kStep = RANK < 32 ? RANK : 32;
 #pragma unroll
-  for (int c0 = 0; c0 < RANK; c0 += 32) {
+  for (int c0 = 0; c0 < RANK; c0 += kStep) {
     uint32_t v[32];
     tmem_ld_32x32b_x32(accumulator + c0, v);
     tmem_ld_wait();
+    float f[kStep];
 #pragma unroll
-    for (int c = 0; c < (RANK < 32 ? RANK : 32); c += 4) {
-      float4 w = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
-                             __uint_as_float(v[c + 3]));
-      *reinterpret_cast<float4*>(row + c0 + c) = any ? w : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < kStep; ++c) f[c] = __uint_as_float(v[c]);
+    if constexpr (PLANES == 2 && 2 * RANK <= 32) {
+#pragma unroll
+      for (int c = 0; c < kStep; ++c) f[c] += __uint_as_float(v[RANK + c]);
+    } else if constexpr (PLANES == 2) {
+      tmem_ld_32x32b_x32(accumulator + RANK + c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < kStep; ++c) f[c] += __uint_as_float(v[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kStep; c += 4) {
+      *reinterpret_cast<float4*>(row + c0 + c) =
+          any ? make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
 }
@@ -485,7 +498,7 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
   tc_fence_after();
   __syncthreads();
   if (warp < 4) {
-    store_part<RANK>(part + (warp * 32 + lane) * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp) << 21), first < last);
+    store_part<RANK, 1>(part + (warp * 32 + lane) * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp) << 21), first < last);
   }
   tc_fence_before();
   cluster_sync();
@@ -943,9 +956,10 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
 // ------------------------------------------------------------------- outer ----
 
 // dW[column, r] = sum over the adapter's slots of row[column] * low[r]: D
-// [128 columns, RANK] twice in tensor memory, K the slots. The rows are A
+// [128 columns, 2 RANK] twice in tensor memory, K the slots. The rows are A
 // (MN-major: 64 columns are a swizzled row of 128 bytes), both planes of `low`
-// B (in panels). A block takes 256 columns and RANK ranks; the blocks of a
+// side by side are B (in panels), so that A, whose reading takes longer than
+// the product, is read once; the planes' sums are added at the end. A block takes 256 columns and RANK ranks; the blocks of a
 // cluster share the adapter's tokens.
 template <int RANK>
 struct OuterShape {
@@ -957,7 +971,7 @@ struct OuterShape {
   static constexpr int kRowBytes = kColumns / 64 * kSubBytes;
   static constexpr int kPlaneBytes = kTokens * RANK * 2;
   static constexpr int kStageBytes = kRowBytes + 2 * kPlaneBytes;
-  static constexpr int kTensorColumns = RANK < 32 ? 64 : 2 * RANK;  // a load reads 32 columns
+  static constexpr int kTensorColumns = 4 * RANK;
   static constexpr int kPartPitch = RANK + 4;
   static constexpr int kPartBytes = kColumns * kPartPitch * 4 * 3 / 2;  // and a cluster's share, at most half
   static constexpr int kBytes = 1024 + (kStages * kStageBytes > kPartBytes ? kStages * kStageBytes : kPartBytes);
@@ -1038,7 +1052,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
     cp_async_commit();
     cp_async_wait<0>();
   } else {
-    constexpr uint32_t kInstruction = idesc_f16<T>(128, RANK, true, true);
+    constexpr uint32_t kInstruction = idesc_f16<T>(128, 2 * RANK, true, true);
     // Groups of 8 slots are 1024 bytes apart, runs of 64 columns kSubBytes.
     const uint64_t a = smem_desc(stages, S::kSubBytes, 1024, 2);
     const uint64_t b = smem_desc(stages + S::kRowBytes, 128, S::kTokens * 16, 0);
@@ -1046,14 +1060,11 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
       // Addresses advance in the descriptors' units of 16 bytes.
       const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
 #pragma unroll
-      for (int plane = 0; plane < 2; ++plane) {
+      for (int k = 0; k < S::kTokens / 16; ++k) {
 #pragma unroll
-        for (int k = 0; k < S::kTokens / 16; ++k) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            mma_bf16(accumulator + half * RANK, a + stage + half * (2 * S::kSubBytes / 16) + k * 128,
-                     b + stage + plane * (S::kPlaneBytes / 16) + k * 16, kInstruction, fill > 0 || plane > 0 || k > 0);
-          }
+        for (int half = 0; half < 2; ++half) {
+          mma_bf16(accumulator + half * 2 * RANK, a + stage + half * (2 * S::kSubBytes / 16) + k * 128, b + stage + k * 16,
+                   kInstruction, fill > 0 || k > 0);
         }
       }
     });
@@ -1064,8 +1075,8 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   __syncthreads();
   if (warp < 8) {
     const int half = warp / 4, c = half * 128 + warp % 4 * 32 + lane;
-    store_part<RANK>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * RANK,
-                     first < last);
+    store_part<RANK, 2>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * 2 * RANK,
+                        first < last);
   }
   tc_fence_before();
   cluster_sync();
