@@ -850,8 +850,13 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
     auto look = [&](const Tile& tile, int32_t (&token)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        token[i] = row0 + 8 * i < tile.count ? static_cast<int32_t>(token_of(p, tile.start + row0 + 8 * i)) : -1;
+        token[i] = row0 + 8 * i < tile.count ? p.rows[tile.start + row0 + 8 * i] : -1;
       }
+    };
+    // Apart from the look, so that its loads stay under way.
+    auto check = [&](int32_t (&token)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) token[i] = static_cast<uint32_t>(token[i]) < static_cast<uint32_t>(p.tokens) ? token[i] : -1;
     };
     auto load_base = [&](int32_t token, int g) {
       Raw8<T> r;
@@ -872,6 +877,7 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
     Tile tile = p.tiles[first], next = first + 1 < last ? p.tiles[first + 1] : kNone;
     int32_t token[4], next_token[4];
     look(tile, token);
+    check(token);
     Raw8<T> part[S::kHalves][S::kGroups][2];
 #pragma unroll
     for (int half = 0; half < S::kHalves; ++half) {
@@ -897,6 +903,7 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       if (mine && !wait(&ready, product)) break;
       products = next_product;
       if (!early) load(next, next_product);
+      check(next_token);
       tc_fence_after();
 #pragma unroll
       for (int half = 0; half < S::kHalves; ++half) {
