@@ -17,10 +17,14 @@
 // A rank r of a few dozen against widths of thousands leaves about r flops a
 // byte of the streamed matrix: all three are bound by reading x, base and dy
 // and writing y and dx once, not by the tensor cores. Tokens of one adapter
-// are gathered into tiles of 128 rows (16 when adapters have few tokens, as in
-// decoding, where the weights are the traffic); low ranks are summed over the
-// width in fp32, across the blocks of a cluster through distributed shared
-// memory, so nothing is added in an order that changes.
+// are gathered into tiles of 128 rows, whose products accumulate in tensor
+// memory, or of 16 when adapters have few tokens, as in decoding, where the
+// weights are the traffic. Sums over the width or over the tokens are fp32,
+// across the blocks of a cluster through distributed shared memory in a fixed
+// order, so nothing is added in an order that changes.
+//
+// Copies are each thread's own (16 bytes, zeros where there is nothing): the
+// rows of a tile lie anywhere, and any stride and alignment is taken.
 //
 // `low` is kept as two 16-bit planes, hi = round(v) and lo = round(v - hi):
 // the tensor cores take 16-bit operands, and the second product then loses
@@ -106,7 +110,11 @@ __device__ __forceinline__ void store_planes4(const AdapterParams& p, int64_t sl
 
 // Tiles of 16 rows (decoding): the weight is the traffic, and the tensor
 // memory's 128 rows would be empty. Four warps share the rows and take a
-// quarter of each chunk of the width. RANK: columns of `low` per block.
+// quarter of each chunk of the width. RANK: columns of `low` per block. The
+// width is split over a cluster of up to 8 blocks until they fill the SMs,
+// and the expand kernel may start behind it (its weight and base do not wait).
+// One row, width 3584, rank 16: 5.0 us, the time of a launch with a cluster's
+// exchange; 192 rows of 48 adapters: 6.7 us.
 template <int RANK, bool TRANS>
 struct NarrowShape {
   static constexpr int ROWS = kNarrow;
@@ -402,7 +410,11 @@ struct WideShape {
 
 // Tiles of 128 rows: D [128, RANK] in tensor memory. The rows are A (K-major,
 // swizzled); the weight chunk is B, K-major and swizzled ([rank, width]) or in
-// panels ([width, rank]).
+// panels ([width, rank]). Two blocks an SM keep 128 KB of copies under way.
+// 16384 x 3584 bf16, rank 32: 25.7 us (4.6 TB/s), of which about 10 start and
+// end the launch: each further 16384 rows take 19.3 (6.1 TB/s, bound by
+// memory). Register accumulators and mma.sync took 35. Chunks of 128 columns
+// and 3 to 6 stages measured the same.
 template <typename T, int RANK, bool TRANS, bool FAST>
 __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_shrink_wide(AdapterParams p) {
   using S = WideShape<RANK, TRANS>;
@@ -518,7 +530,8 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
 // ------------------------------------------------------------------ expand ----
 
 // Tiles of 16 rows: bound by the weight, of which each block reads 128 columns
-// (with base, before it waits for `low`). Four warps, each all 16 rows of 32
+// (with base, before it waits for `low`), and by the launch: one row of 3584
+// columns takes 4.9 us, 192 rows of 48 adapters, width 4608, 9.6. Four warps, each all 16 rows of 32
 // columns. A thread's accumulators over four 8-column tiles are made 8
 // neighbouring columns by assigning column 8 q + 2 j + b of 32 to element
 // 2 q + b of tile j: base and out then move in 16-byte words straight between
@@ -691,7 +704,13 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
 // columns are permuted within 32 (column 8 q + 2 j + b stands at 8 j + 2 q + b)
 // so that these are 8 neighbours, and base and out move in 16-byte words. The
 // next tile's part of base is loaded as soon as the current one's has been
-// used, its low rows while the current tile is worked on.
+// used, its low rows (and weight, if another) while the current tile is worked
+// on. Bound by base and out: 16384 x 3584 bf16, rank 32, 49 us (4.8 TB/s; each
+// further 16384 rows take 40, 5.8 TB/s), rank 64 63 us (register accumulators
+// and mma.sync: 80); 8191 x 18944 fp16 of 23 ragged adapters 123 us (5.0 TB/s).
+// Blocks of 128 columns, two or three to an SM, took 58 and 66 us for the
+// first; runs half as long, in two waves, 57, though 4 % less where ragged
+// adapters leave the runs uneven.
 struct ExpandWide {
   static constexpr int kThreads = kFillThreads;
   static constexpr int kColumns = 256;
@@ -966,7 +985,11 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
 // [128 columns, 2 RANK] twice in tensor memory, K the slots. The rows are A
 // (MN-major: 64 columns are a swizzled row of 128 bytes), both planes of `low`
 // side by side are B (in panels), so that A, whose reading takes longer than
-// the product, is read once; the planes' sums are added at the end. A block takes 256 columns and RANK ranks; the blocks of a
+// the product, is read once; the planes' sums are added at the end. Each block
+// takes about 0.43 us for a stage of 16 KB, with one or two blocks on the SM
+// and 4 or 5 stages. 16384 x 3584 bf16, rank 32, 4 adapters: 34 us (3.5 TB/s),
+// 40 in a backward pass, where earlier writes are still leaving L2; each
+// further 16384 rows take 24 (4.9 TB/s). Register accumulators took 68. A block takes 256 columns and RANK ranks; the blocks of a
 // cluster share the adapter's tokens.
 template <int RANK>
 struct OuterShape {

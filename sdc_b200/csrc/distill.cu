@@ -40,9 +40,9 @@ constexpr int kMaxCluster = 8;
 constexpr int kGradBlocks = 3;
 constexpr size_t kSharedLimit = 227 * 1024;
 // Three blocks of loss with gradient on an SM: some compute while others
-// exchange. At 4096 x 151936 bf16 this took 520 us; two blocks of 80 KB 560,
-// four of 50 KB 550 (the exchange costs each block about a microsecond a row),
-// one of 152 KB 550.
+// exchange. At 4096 x 151936 bf16, compared in one run before the last steps,
+// this took 520 us; two blocks of 80 KB 560, four of 50 KB 550 (the exchange
+// costs each block about a microsecond a row), one of 152 KB 550.
 constexpr size_t kSliceTarget = 74 * 1024;
 constexpr int kBackThreads = 256;
 constexpr int kBackWords = 4;                  // 16-byte words per thread of the backward pass
@@ -416,6 +416,9 @@ __device__ __forceinline__ void write_empty(const DistillParams& p, int64_t row)
 }
 
 // The losses alone: a cluster of blocks per row streams it through registers.
+// Bound by memory: 4096 rows of 151936 bf16 take 191 us (1245 MB, 6.5 TB/s),
+// 509 rows 33.7 us (4.6 TB/s: the start and the last, partly filled wave cost
+// more of so few rows); one row 6.1 us.
 template <typename T>
 __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams p) {
   extern __shared__ uint4 shared[];
@@ -487,7 +490,11 @@ __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams 
 // chunk by chunk; a chunk they have read for the last time is refilled with
 // the next row's at once. The list warp looks ahead for rows without entries
 // (which are not read at all), issues the copies, and after the streaming
-// warps writes the list's columns again with the teacher's part.
+// warps writes the list's columns again with the teacher's part. 4096 rows of
+// 151936 bf16 take 504 us (2489 MB, 4.9 TB/s): two exponentials an element
+// keep their unit 56 % busy, and a row's exchange costs about a microsecond in
+// which its block reads but does not write. Loss and backward pass one after
+// the other take 566 us.
 struct GradBarriers {
   uint64_t full[kChunks];   // the chunk's copy has arrived
   uint64_t empty[kChunks];  // every streaming warp has read the chunk for the last time
@@ -781,7 +788,8 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
 // The gradient from the row statistics: one read, one write, blocks of a row
 // independent of each other. A warp of its own collects the block's entries of
 // the list meanwhile (their logits before they are overwritten: the gradient
-// may replace them) and writes their columns last.
+// may replace them) and writes their columns last. Bound by memory: 4096 rows
+// of 151936 bf16 take 375 us (2489 MB, 6.6 TB/s).
 struct BackEntry {
   float s, p;
   int at;
@@ -874,7 +882,7 @@ __global__ void __launch_bounds__(kBackThreads + 32, 6) distill_backward(Distill
 
 // out[0] = sum or mean of the losses over the rows that have entries (0 when
 // none has), out[1] = what a row's loss was multiplied with. One block, fixed
-// order.
+// order: 2.4 us for 333 rows.
 __global__ void __launch_bounds__(1024) distill_reduce(const float* loss, const float4* stats, int64_t rows, bool mean,
                                                        float* out) {
   __shared__ float sums[32];

@@ -1,9 +1,8 @@
-// Warp-level matrix instructions for the skinny products of the low-rank
-// adapters: 16-bit operands from shared memory, fp32 accumulators in
-// registers. Those products are bound by the streamed operand's bytes (a rank
-// of at most a few dozen against rows of thousands), so they need neither
-// tensor memory nor descriptors, and the fragments can be formed from any
-// row stride.
+// Copies into shared memory that every thread can make on its own, and
+// warp-level matrix instructions for products of 16 rows (16-bit operands from
+// shared memory, fp32 accumulators in registers): the tensor memory's
+// instructions take 64 rows at least, and so few rows wait for their weights
+// whatever multiplies them.
 #pragma once
 
 #include "layers.cuh"
@@ -47,9 +46,6 @@ __device__ __forceinline__ void mma_16816<__half>(float* d, const uint32_t* a, c
 __device__ __forceinline__ void cp_async16(uint32_t shared, const void* global, bool copied = true) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(global), "r"(copied ? 16 : 0)
                : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t shared, const void* global) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared), "l"(global) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

@@ -33,9 +33,10 @@ def distillation_loss(student_logits, teacher_indices, teacher_logits, temperatu
     student's over the whole vocabulary, times ``temperature^2``.
 
     ``student_logits`` ``[..., vocabulary]`` (fp32, bf16 or fp16, any row
-    stride; column-major ones are copied to rows first); ``teacher_indices`` (int32 or int64) and ``teacher_logits`` ``[...,
-    top]`` with ``top`` up to 1024. Both distributions are softmaxes at the
-    temperature, the teacher's over its list alone. Negative indices are no
+    stride; column-major ones are copied to rows first); ``teacher_indices``
+    (int32 or int64) and ``teacher_logits`` ``[..., top]`` with ``top`` up to
+    1024. Both distributions are softmaxes at the temperature, the teacher's
+    over its list alone. Negative indices are no
     entries; entries that name a token twice add up; a row without entries (or
     with teacher logits of -inf alone) has loss 0 and gradient 0 whatever its
     student logits; an index beyond the vocabulary makes the row NaN.
@@ -58,8 +59,9 @@ def distillation_loss_and_grad(student_logits, teacher_indices, teacher_logits, 
     """The losses of every row (as ``reduction="none"``) and the gradient of
     ``sum(grad_loss * losses)`` with respect to the logits, in one pass over
     them. ``grad_loss``: fp32 scalar tensor or one value a row; None: 1. With
-    ``in_place`` the gradient replaces the logits (contiguous rows). Not recorded by autograd:
-    hand the gradient to ``torch.autograd.backward(logits, grad)``."""
+    ``in_place`` the gradient replaces the logits (contiguous rows). Not
+    recorded by autograd: hand the gradient to
+    ``torch.autograd.backward(logits, grad)``."""
     shape = student_logits.shape
     student, indices, teacher, temperature = _arguments(student_logits, teacher_indices, teacher_logits, temperature)
     if grad_loss is not None and grad_loss.dim() > 1:
