@@ -43,7 +43,8 @@ namespace {
 constexpr int kWide = 128, kNarrow = 16;  // rows of a tile
 constexpr int kMaxWideRank = 128;         // beyond, a wide tile's low rows and weight do not fit together
 constexpr int kMaxRank = 256;
-constexpr int kMaxSplit = 8;
+constexpr int kMaxSplit = 16;  // blocks of a cluster
+constexpr int kPortableSplit = 8;
 
 struct Tile {
   int32_t start, count, adapter;
@@ -1144,6 +1145,7 @@ int launch_clustered(Kernel kernel, const AdapterParams& p, dim3 grid, int threa
                      bool dependent, cudaStream_t stream) {
   const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared);
   if (rc != SDC_OK) return rc;
+  if (cluster > kPortableSplit) SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(static_cast<unsigned>(threads));
@@ -1183,11 +1185,25 @@ int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
 bool vector_rows(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
+// Clusters of 1, 2, ... 16 blocks that run at once when an SM holds two blocks
+// (the driver's occupancy figures on a B200 of 148 SMs; another layout of the
+// SMs costs time, not results).
+constexpr int kClusterRoom[kMaxSplit + 1] = {0, 296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14};
+
 // Blocks that share a tile's sum: as many as fill the SMs' `resident` blocks
-// each once, as long as each keeps two chunks.
-int split_count(int64_t blocks, int64_t chunks, int resident) {
-  const int64_t wanted = std::min<int64_t>(static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(blocks, 1), chunks / 2);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, kMaxSplit)));
+// each once, as long as each keeps two chunks (four of more than eight blocks),
+// and no more than let all clusters run at once: a few that waited for a second
+// turn would double the time. Outer products of 16384 rows and one adapter:
+// 3584 columns, rank 32, in 14 clusters of 16 blocks 29 us, of 8 35; 1024
+// columns, rank 16, 21 and 33. 37 tiles of shrink (3584 columns, rank 32) in
+// clusters of 7 take 14 us, of 8 19; 42 clusters of outer products are the other
+// way round, 6 blocks 36 us and 7 33.
+int split_count(int64_t clusters, int64_t chunks, int resident, int most) {
+  const int64_t wanted = std::min<int64_t>(static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(clusters, 1), chunks / 2);
+  int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, most)));
+  if (split > kPortableSplit && chunks / split < 4) split = kPortableSplit;
+  while (split > 1 && clusters > kClusterRoom[split] * resident / 2) --split;
+  return split;
 }
 
 template <typename T, int ROWS, int RANK, bool TRANS>
@@ -1195,7 +1211,7 @@ int launch_shrink(AdapterParams p, int64_t tiles, cudaStream_t stream) {
   using S = std::conditional_t<ROWS == kWide, WideShape<RANK, TRANS>, NarrowShape<RANK, TRANS>>;
   const int64_t chunks = ceil_div(p.width, S::kChunk);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
-  const int split = split_count(tiles * rank_blocks, chunks, ROWS == kWide ? 2 : 4);
+  const int split = split_count(tiles * rank_blocks, chunks, ROWS == kWide ? 2 : 4, kPortableSplit);
   p.chunks_per_split = static_cast<int>(ceil_div(chunks, split));
   const dim3 grid(static_cast<unsigned>(tiles * split), rank_blocks);
   const bool fast = p.vector_rows && p.vector_weight && p.width % 8 == 0 && (!TRANS || p.rank % 8 == 0);
@@ -1276,7 +1292,7 @@ int launch_outer(const AdapterParams& p, cudaStream_t stream) {
   const int64_t columns = ceil_div(p.width, S::kColumns);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int64_t tiles = ceil_div(ceil_div(p.slots, p.adapters), S::kTokens);
-  const int split = split_count(columns * p.adapters * rank_blocks, tiles, 2);
+  const int split = split_count(columns * p.adapters * rank_blocks, tiles, 2, kMaxSplit);
   const dim3 grid(static_cast<unsigned>(columns * split), static_cast<unsigned>(p.adapters), rank_blocks);
   return p.vector_rows && p.width % 8 == 0
              ? launch_clustered(adapter_outer<T, RANK, true>, p, grid, S::kThreads, split, S::kBytes, false, stream)
@@ -1311,7 +1327,7 @@ int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride, int64_t token
   if (rc != SDC_OK) return rc;
   SDC_REQUIRE(tile_rows == kNarrow || (tile_rows == kWide && rank <= kMaxWideRank),
               "low-rank adapter tiles have 16 rows, or 128 for ranks of up to 128");
-  SDC_REQUIRE(tile_count >= 0 && tile_count <= INT_MAX / kMaxSplit, "low-rank adapters have too many tiles for one launch");
+  SDC_REQUIRE(tile_count >= 0 && tile_count <= INT_MAX / kPortableSplit, "low-rank adapters have too many tiles for one launch");
   if (tile_count == 0) return SDC_OK;
   SDC_REQUIRE(x != nullptr && rows != nullptr && tiles != nullptr && weight != nullptr && low != nullptr && aligned16(low),
               "low-rank adapter pointers must not be null and the low-rank rows must be 16-byte aligned");
