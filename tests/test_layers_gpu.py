@@ -305,6 +305,14 @@ def test_low_rank_adapters_forward_and_backward(case, dtype):
         assert torch.equal(first, second)
 
 
+# Token sums long enough for clusters of 9 to 16 blocks: few column blocks, both forms of a row, blocks of ranks, empty adapters.
+@pytest.mark.parametrize("case", [([2100], [0], 1, 16, 37, 53), ([5000, 3], [0, 2], 3, 64, 136, 520),
+                                  ([2500, 0, 2400], [0, 2, 1], 3, 100, 200, 136), ([4096], [0], 1, 32, 896, 2056),
+                                  ([3001], [0], 1, 5, 1032, 264)])
+def test_low_rank_adapters_sum_long_batches(case):
+    test_low_rank_adapters_forward_and_backward(case, torch.bfloat16)
+
+
 @pytest.mark.parametrize("requests", [1, 5, 60])
 def test_low_rank_adapters_tiles_do_not_change_a_token(requests):
     """A token's output has the same exact value whatever shares its batch."""
