@@ -22,8 +22,8 @@ int cuda_fail(cudaError_t error, const char* what);
 int check_current_device();
 // Streaming multiprocessors of the current device (cached per device).
 int sm_count();
-// Lets `kernel` use `bytes` of dynamic shared memory on the current device
-// (asked of the runtime once for each kernel, device and larger amount).
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device, from
+// any thread (each asks the runtime once for each kernel and device).
 int allow_shared(const void* kernel, int bytes);
 // Encodes a tiled TMA descriptor through the driver entry point (no -lcuda).
 int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank,

@@ -997,7 +997,7 @@ int launch_rows(DistillParams p, int64_t rows, int cluster, size_t shared, cudaS
     int device = 0;
     SDC_CUDA_CHECK(cudaGetDevice(&device));
     if (last.device != device || last.cluster != cluster || last.shared != shared) {
-      const int rc = allow_shared(reinterpret_cast<const void*>(kernel), static_cast<int>(kSharedLimit - 2048));
+      const int rc = allow_shared(reinterpret_cast<const void*>(kernel), static_cast<int>(shared));
       if (rc != SDC_OK) return rc;
       config.gridDim = dim3(static_cast<unsigned>(cluster));
       SDC_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&last.clusters, kernel, &config));

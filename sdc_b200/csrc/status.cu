@@ -82,7 +82,11 @@ int sm_count() {
 
 int allow_shared(const void* kernel, int bytes) {
   if (bytes <= 40 * 1024) return SDC_OK;  // 48 KB, static shared memory included, need no asking
-  // Nothing here allocates (or throws): a kernel that finds its place taken asks again.
+  // The limit belongs to the kernel and the device, not to a thread: every
+  // thread sets the same one, the most that fits, so that none lowers what
+  // another's launch relies on. What a thread remembers is only that it was
+  // set. Nothing here allocates (or throws): a kernel that finds its place
+  // taken asks again.
   struct Allowed {
     const void* kernel = nullptr;
     int device = -1, bytes = 0;
@@ -92,9 +96,16 @@ int allow_shared(const void* kernel, int bytes) {
   int device = 0;
   SDC_CUDA_CHECK(cudaGetDevice(&device));
   Allowed& place = places[reinterpret_cast<uintptr_t>(kernel) / 16 % kPlaces];
-  if (place.kernel == kernel && place.device == device && place.bytes >= bytes) return SDC_OK;
-  SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  place = Allowed{kernel, device, bytes};
+  if (place.kernel != kernel || place.device != device) {
+    int most = 0;
+    cudaFuncAttributes attributes{};
+    SDC_CUDA_CHECK(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+    SDC_CUDA_CHECK(cudaFuncGetAttributes(&attributes, kernel));
+    most -= static_cast<int>(attributes.sharedSizeBytes);
+    SDC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    place = Allowed{kernel, device, most};
+  }
+  SDC_REQUIRE(bytes <= place.bytes, "the kernel's shared memory does not fit this device");
   return SDC_OK;
 }
 
