@@ -6,7 +6,7 @@
 //
 // Rot turns pair p < rotary/2 of a head by the position's angle p: elements
 // (p, p + rotary/2), or (2p, 2p+1) when interleaved; elements from `rotary`
-// on pass. Without weights the heads are only turned.
+// on pass, each by itself. Without weights the heads are only turned.
 //
 // Both directions move bytes and little else (about 10 flops an element), so
 // the layout serves the loads: a thread owns 8 pairs of a head, both members
@@ -76,6 +76,7 @@ __device__ __forceinline__ int element_of(int pair, int member, int rotary) {
 // first half of their part of the head, their second runs in the other.
 template <typename T, bool INTERLEAVED, bool VECTOR>
 struct HeadIO {
+  static constexpr bool kTogether = VECTOR && !INTERLEAVED;  // a lane's pairs turn (split) or pass together
   int first_pair, rotary, pairs, low_run, high_run;
   bool active, split;
 
@@ -91,7 +92,7 @@ struct HeadIO {
     if (split) return (member ? high_run : low_run) + i;
     return (i < 4 ? low_run + 2 * i : high_run + 2 * (i - 4)) + member;
   }
-  // Index of pair i's angle (rotary / 2 or more: none).
+  // Index of pair i's angle (rotary / 2 or more: none, the pair passes).
   __device__ __forceinline__ int angle(int i) const {
     if (!VECTOR || !INTERLEAVED) return first_pair + i;
     return element(i, 0) / 2;
@@ -209,8 +210,10 @@ struct HeadIO {
   }
 };
 
-// The position's cosine and sine for this lane's 8 pairs; identity beyond the
-// rotary pairs. A position outside the table gives NaN, not a stray read.
+// The position's cosine and sine for this lane's 8 pairs; beyond the rotary
+// pairs 1 and -0 (an angle of 0 whose sign marks a pair that passes). A
+// position outside the table gives NaN, not a stray read.
+constexpr uint32_t kPasses = 0x80000000u;
 struct Angles {
   float cosine[8], sine[8];
 };
@@ -235,8 +238,24 @@ __device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t posit
       const int pair = io.angle(i);
       const bool turned = pair < half;
       a.cosine[i] = turned ? (inside ? row[pair] : nan) : 1.f;
-      a.sine[i] = turned ? (inside ? row[half + pair] : nan) : 0.f;
+      a.sine[i] = turned ? (inside ? row[half + pair] : nan) : __uint_as_float(kPasses);
     }
+  }
+}
+
+// Turns the lane's pairs by their angles, or (BACK) by their opposites. Pairs
+// that pass are kept apart: a product with a sine of 0 would carry an infinity
+// or a NaN of one element over to the other.
+template <bool BACK, typename IO>
+__device__ __forceinline__ void turn(const IO& io, const Angles& a, float* v) {
+  if (IO::kTogether && !io.split) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool passes = !IO::kTogether && __float_as_uint(a.sine[i]) == kPasses;
+    const float sine = BACK ? -a.sine[i] : a.sine[i];
+    const float x = v[i], y = v[8 + i];
+    v[i] = x * a.cosine[i] - (passes ? 0.f : y) * sine;
+    v[8 + i] = y * a.cosine[i] + (passes ? 0.f : x) * sine;
   }
 }
 
@@ -349,13 +368,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
         for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
       }
       if (!mine) continue;
-      float out[16];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        out[i] = v[i] * angles.cosine[i] - v[8 + i] * angles.sine[i];
-        out[8 + i] = v[8 + i] * angles.cosine[i] + v[i] * angles.sine[i];
-      }
-      walk.io.store(y + h * p.dim, out);
+      turn<false>(walk.io, angles, v);
+      walk.io.store(y + h * p.dim, v);
     }
   }
 }
@@ -405,13 +419,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
       const bool mine = live && h < walk.heads;
       float v[16], g[16];
       if (mine) {
-        float dv[16];
-        walk.io.unpack(walk.head(round, 1, p.dy[role], p.dys[role], h), dv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          g[i] = dv[i] * angles.cosine[i] + dv[8 + i] * angles.sine[i];
-          g[8 + i] = dv[8 + i] * angles.cosine[i] - dv[i] * angles.sine[i];
-        }
+        walk.io.unpack(walk.head(round, 1, p.dy[role], p.dys[role], h), g);
+        turn<true>(walk.io, angles, g);
       }
       if (norm) {
         float squares = 0.f, products = 0.f;
