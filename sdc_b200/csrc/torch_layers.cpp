@@ -444,6 +444,14 @@ std::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? std::o
 Tensor tensor_of(OptTensor t) { return t.has_value() ? *t : Tensor(); }
 bool differentiates(OptTensor t) { return t.has_value() && t->requires_grad(); }
 
+// The derivatives here are those of backward passes. A dual tensor's tangent
+// would be lost where nothing else asks for a gradient.
+template <typename... Tensors>
+void refuse_tangents(const Tensors&... inputs) {
+  auto dual = [](OptTensor t) { return t.has_value() && t->defined() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!(dual(inputs) || ...), "the layer operators have no forward-mode derivatives");
+}
+
 // The backward kernels have no derivatives: a second differentiation raises.
 variable_list once_differentiable(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -495,6 +503,7 @@ struct HeadNormRotary : torch::autograd::Function<HeadNormRotary> {
 std::tuple<Tensor, Tensor> head_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& table,
                                                      const Tensor& positions, OptTensor q_weight, OptTensor k_weight,
                                                      double eps, bool interleaved) {
+  refuse_tangents(q, k, table, q_weight, k_weight);
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || differentiates(q_weight) || differentiates(k_weight))) {
     variable_list out = HeadNormRotary::apply(q, k, table, positions, q_weight, k_weight, eps, interleaved);
@@ -547,6 +556,7 @@ struct LowRankAdapters : torch::autograd::Function<LowRankAdapters> {
 };
 
 bool adapters_differentiate(const Tensor& base, const Tensor& x, const Tensor& a, const Tensor& b, OptTensor scale) {
+  refuse_tangents(base, x, a, b, scale);
   if (!at::GradMode::is_enabled()) return false;
   TORCH_CHECK(!differentiates(scale), "adapter scales are not differentiable");
   return base.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad();
@@ -621,6 +631,7 @@ Tensor distillation_loss_cuda(const Tensor& logits, const Tensor& indices, const
 Tensor distillation_loss_autograd(const Tensor& logits, const Tensor& indices, const Tensor& teacher,
                                   double temperature, int64_t reduction) {
   TORCH_CHECK(reduction >= kNone && reduction <= kMean, "distillation reduction must be 0 (none), 1 (sum) or 2 (mean)");
+  refuse_tangents(logits, teacher);
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     return DistillationLoss::apply(logits, indices, teacher, temperature, reduction);
   }
@@ -628,11 +639,21 @@ Tensor distillation_loss_autograd(const Tensor& logits, const Tensor& indices, c
   return distillation_loss_cuda(logits, indices, teacher, temperature, reduction);
 }
 
+// Losses and gradients as values, not recorded.
+std::tuple<Tensor, Tensor> distill_loss_and_grad_autograd(const Tensor& logits, const Tensor& indices,
+                                                          const Tensor& teacher, double temperature,
+                                                          OptTensor grad_loss) {
+  refuse_tangents(logits, teacher, grad_loss);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return distill_loss_and_grad(logits, indices, teacher, temperature, grad_loss);
+}
+
 // No derivative: the logits become their gradient, which anything that saved them has to notice.
 Tensor distill_loss_and_grad_autograd_(Tensor& logits, const Tensor& indices, const Tensor& teacher,
                                        double temperature, OptTensor grad_loss) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && logits.requires_grad()),
               "in-place distillation replaces the logits and is not differentiable");
+  refuse_tangents(logits, teacher, grad_loss);
   at::AutoDispatchBelowADInplaceOrView below;
   Tensor loss = distill_loss_and_grad_(logits, indices, teacher, temperature, grad_loss);
   if (!logits.is_inference()) torch::autograd::impl::bump_version(logits);
@@ -674,5 +695,6 @@ TORCH_LIBRARY_IMPL(sdc_cutlass, AutogradCUDA, lib) {
   lib.impl("low_rank_adapters", &low_rank_adapters_autograd);
   lib.impl("low_rank_adapters_", &low_rank_adapters_autograd_);
   lib.impl("distillation_loss", &distillation_loss_autograd);
+  lib.impl("distill_loss_and_grad", &distill_loss_and_grad_autograd);
   lib.impl("distill_loss_and_grad_", &distill_loss_and_grad_autograd_);
 }

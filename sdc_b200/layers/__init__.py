@@ -3,7 +3,8 @@
 ``head_norm_rotary`` (between the query/key projections and attention),
 ``low_rank_adapters`` (beside a shared, possibly quantised and protected,
 projection) and ``distillation_loss`` (after the last one), each with its
-backward pass, on hand-written sm_100a kernels. Extensions: the reference has
+backward pass, on hand-written sm_100a kernels (first derivatives, reverse
+mode; others raise). Extensions: the reference has
 no counterpart. Like the rest of the package they run on the current CUDA
 stream, never synchronise with the host and have no CPU fallback.
 """

@@ -10,8 +10,10 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from sdc_b200.layers import AdapterBatch, head_norm_rotary, low_rank_adapters, rotary_table
+from sdc_b200.layers import (AdapterBatch, distillation_loss, distillation_loss_and_grad, head_norm_rotary,
+                             low_rank_adapters, low_rank_adapters_, rotary_table)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -106,3 +108,40 @@ def test_passing_elements_of_a_head_stay_apart(case, dtype):
     normed = head_norm_rotary(q, k, table, positions, ones, ones, interleaved=interleaved)[0][:, :dim - rotary]
     bad = expected_bad[:, :dim - rotary]
     assert normed[bad].isnan().all() and not normed[~bad].any()
+
+
+# -------------------------------------------------------------- derivatives ----
+
+def _small():
+    g = rng(7)
+    q, table, positions, w = normal(g, 3, 2, 64), rotary_table(8, 64), torch.arange(3, device=DEV), normal(g, 64)
+    base, x = normal(g, 8, 48, dtype=torch.bfloat16), normal(g, 8, 64, dtype=torch.bfloat16)
+    a, b = normal(g, 2, 8, 64, dtype=torch.bfloat16), normal(g, 2, 48, 8, dtype=torch.bfloat16)
+    logits, teacher = normal(g, 3, 50), normal(g, 3, 4)
+    return q, table, positions, w, base, x, a, b, torch.ones(2, device=DEV), AdapterBatch([5, 3], [0, 1], 2), logits, teacher
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor that asks for no gradient must not lose its tangent."""
+    q, table, positions, w, base, x, a, b, scale, batch, logits, teacher = _small()
+    indices = torch.tensor([[0, 7, 49, -1]] * 3, device=DEV)
+    calls = [
+        (q, lambda t: head_norm_rotary(t, q, table, positions)), (q, lambda t: head_norm_rotary(q, t, table, positions)),
+        (table, lambda t: head_norm_rotary(q, q, t, positions)), (w, lambda t: head_norm_rotary(q, q, table, positions, t, w)),
+        (w, lambda t: head_norm_rotary(q, q, table, positions, w, t)),
+        (base, lambda t: low_rank_adapters(t, x, a, b, batch)), (x, lambda t: low_rank_adapters(base, t, a, b, batch)),
+        (a, lambda t: low_rank_adapters(base, x, t, b, batch)), (b, lambda t: low_rank_adapters(base, x, a, t, batch)),
+        (scale, lambda t: low_rank_adapters(base, x, a, b, batch, t)),
+        (base, lambda t: low_rank_adapters_(t, x, a, b, batch)), (x, lambda t: low_rank_adapters_(base, t, a, b, batch)),
+        (logits, lambda t: distillation_loss(t, indices, teacher)), (teacher, lambda t: distillation_loss(logits, indices, t)),
+        (logits, lambda t: distillation_loss_and_grad(t, indices, teacher)),
+        (logits, lambda t: distillation_loss_and_grad(t, indices, teacher, in_place=True)),
+    ]
+    for primal, call in calls:
+        before = primal.clone()
+        for requires_grad in (False, True):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(primal.clone().requires_grad_(requires_grad), torch.ones_like(primal))
+                with pytest.raises(RuntimeError, match="forward-mode|not differentiable|leaf"):
+                    call(dual)
+        assert torch.equal(primal, before)
