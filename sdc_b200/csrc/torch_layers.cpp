@@ -504,6 +504,7 @@ std::tuple<Tensor, Tensor> head_norm_rotary_autograd(const Tensor& q, const Tens
                                                      const Tensor& positions, OptTensor q_weight, OptTensor k_weight,
                                                      double eps, bool interleaved) {
   refuse_tangents(q, k, table, q_weight, k_weight);
+  TORCH_CHECK(!(at::GradMode::is_enabled() && table.requires_grad()), "the rotation table is not differentiable");
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || differentiates(q_weight) || differentiates(k_weight))) {
     variable_list out = HeadNormRotary::apply(q, k, table, positions, q_weight, k_weight, eps, interleaved);
@@ -632,6 +633,8 @@ Tensor distillation_loss_autograd(const Tensor& logits, const Tensor& indices, c
                                   double temperature, int64_t reduction) {
   TORCH_CHECK(reduction >= kNone && reduction <= kMean, "distillation reduction must be 0 (none), 1 (sum) or 2 (mean)");
   refuse_tangents(logits, teacher);
+  TORCH_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()),
+              "distillation is not differentiable in the teacher's logits");
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     return DistillationLoss::apply(logits, indices, teacher, temperature, reduction);
   }

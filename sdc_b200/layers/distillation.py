@@ -42,8 +42,9 @@ def distillation_loss(student_logits, teacher_indices, teacher_logits, temperatu
     student logits; an index beyond the vocabulary makes the row NaN.
 
     ``reduction``: "none" (fp32, one loss a row), "sum", or "mean" over the
-    rows that have entries. Differentiable in the student's logits; the
-    backward pass reads them again. Where the upstream gradient is known
+    rows that have entries. Differentiable in the student's logits (a teacher's
+    that require a gradient are refused: ``detach()`` them); the backward pass
+    reads them again. Where the upstream gradient is known
     beforehand, ``distillation_loss_and_grad`` reads them once."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}")

@@ -145,3 +145,20 @@ def test_forward_mode_derivatives_are_refused():
                 with pytest.raises(RuntimeError, match="forward-mode|not differentiable|leaf"):
                     call(dual)
         assert torch.equal(primal, before)
+
+
+def test_gradients_that_do_not_exist_are_refused():
+    """Of the rotation table and of the teacher's logits, unless nothing is recorded."""
+    q, table, positions, _, _, _, _, _, _, _, logits, teacher = _small()
+    indices = torch.tensor([[0, 7, 49, -1]] * 3, device=DEV)
+    with pytest.raises(RuntimeError, match="table is not differentiable"):
+        head_norm_rotary(q, q, table.clone().requires_grad_(), positions)
+    tracked = teacher.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="teacher"):
+        distillation_loss(logits, indices, tracked)
+    want = distillation_loss(logits, indices, teacher)
+    assert torch.equal(distillation_loss(logits, indices, tracked.detach()), want)
+    with torch.no_grad():
+        assert torch.equal(distillation_loss(logits, indices, tracked), want)
+        head_norm_rotary(q, q, table.clone().requires_grad_(), positions)
+    distillation_loss_and_grad(logits, indices, tracked)  # records nothing
