@@ -10,6 +10,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -514,24 +515,27 @@ std::tuple<Tensor, Tensor> head_norm_rotary_autograd(const Tensor& q, const Tens
   return head_norm_rotary(q, k, table, positions, q_weight, k_weight, eps, interleaved);
 }
 
+// In place (low_out given) base is the only output: autograd takes no other
+// beside one that may be a view.
 struct LowRankAdapters : torch::autograd::Function<LowRankAdapters> {
   static variable_list forward(AutogradContext* ctx, const Tensor& base, const Tensor& x, const Tensor& a,
                                const Tensor& b, OptTensor scale, const Tensor& rows, const Tensor& groups,
-                               const Tensor& tiles, int64_t slots, int64_t active, int64_t tile_rows, bool in_place) {
+                               const Tensor& tiles, int64_t slots, int64_t active, int64_t tile_rows, Tensor* low_out) {
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor out = base, low;
-    if (in_place) {
-      low = low_rank_adapters_(out, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+    if (low_out != nullptr) {
+      *low_out = low = low_rank_adapters_(out, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
       ctx->mark_dirty({base});
     } else {
       std::tie(out, low) = low_rank_adapters(base, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);
+      ctx->mark_non_differentiable({low});
     }
     ctx->save_for_backward({x, a, b, tensor_of(scale), low, rows, groups, tiles});
     ctx->saved_data["slots"] = slots;
     ctx->saved_data["active"] = active;
     ctx->saved_data["tile_rows"] = tile_rows;
-    ctx->mark_non_differentiable({low});
     ctx->set_materialize_grads(false);  // no zeros for `low`
+    if (low_out != nullptr) return {out};
     return {out, low};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -569,7 +573,7 @@ std::tuple<Tensor, Tensor> low_rank_adapters_autograd(const Tensor& base, const 
                                                       int64_t active, int64_t tile_rows) {
   if (adapters_differentiate(base, x, a, b, scale)) {
     variable_list out = LowRankAdapters::apply(base, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows,
-                                               false);
+                                               static_cast<Tensor*>(nullptr));
     return {out[0], out[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
@@ -580,7 +584,10 @@ Tensor low_rank_adapters_autograd_(Tensor& base, const Tensor& x, const Tensor& 
                                    const Tensor& rows, const Tensor& groups, const Tensor& tiles, int64_t slots,
                                    int64_t active, int64_t tile_rows) {
   if (adapters_differentiate(base, x, a, b, scale)) {
-    return LowRankAdapters::apply(base, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows, true)[1];
+    torch::autograd::check_inplace(base, true);  // before base is changed
+    Tensor low;
+    LowRankAdapters::apply(base, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows, &low);
+    return low;
   }
   at::AutoDispatchBelowADInplaceOrView below;
   Tensor low = low_rank_adapters_(base, x, a, b, scale, rows, groups, tiles, slots, active, tile_rows);

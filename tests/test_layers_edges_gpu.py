@@ -162,3 +162,44 @@ def test_gradients_that_do_not_exist_are_refused():
         assert torch.equal(distillation_loss(logits, indices, tracked), want)
         head_norm_rotary(q, q, table.clone().requires_grad_(), positions)
     distillation_loss_and_grad(logits, indices, tracked)  # records nothing
+
+
+def test_adapters_into_views_under_autograd():
+    """A projection's output is often a view: of other dimensions, or of a wider tensor whose rest is used as well."""
+    _, _, _, _, base, x, a, b, scale, batch, _, _ = _small()
+
+    def gradients(call, record_base):
+        leaves = [t.clone().requires_grad_() for t in (base, x, a, b)]
+        first = leaves[0] * 2 if record_base else leaves[0].detach() * 2
+        out = call(first, *leaves[1:])
+        return (out, *torch.autograd.grad(out.float().square().sum(), leaves, allow_unused=True))
+
+    def reshaped(first, *rest):
+        low_rank_adapters_(first.view(2, 4, 48).view(8, 48), *rest, batch, scale)
+        return first
+
+    def part(first, *rest):
+        side = first.detach()  # one gradient a column: autograd's own bf16 additions have no fixed order
+        wide = torch.cat((side, first, side), 1)
+        low_rank_adapters_(wide[:, 48:96], *rest, batch, scale)
+        return wide
+
+    for record_base in (True, False):
+        want = gradients(lambda first, *rest: low_rank_adapters(first, *rest, batch, scale), record_base)
+        for got, expected in zip(gradients(reshaped, record_base), want):
+            assert got is expected is None or torch.equal(got, expected)
+        want = gradients(lambda first, *rest: torch.cat((first.detach(), low_rank_adapters(first, *rest, batch, scale),
+                                                         first.detach()), 1), record_base)
+        for got, expected in zip(gradients(part, record_base), want):
+            assert got is expected is None or torch.equal(got, expected)
+
+
+def test_adapters_refuse_a_leaf_before_they_change_it():
+    _, _, _, _, base, x, a, b, scale, batch, _, _ = _small()
+    for refused in (base.clone().requires_grad_(), base.clone().requires_grad_().view(8, 48)):
+        with pytest.raises(RuntimeError, match="leaf Variable that requires grad"):
+            low_rank_adapters_(refused, x, a, b, batch, scale)
+        assert torch.equal(refused, base)
+        with torch.no_grad():
+            assert torch.equal(low_rank_adapters_(refused, x, a, b, batch, scale),
+                               low_rank_adapters(base, x, a, b, batch, scale))
