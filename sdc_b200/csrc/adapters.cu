@@ -84,9 +84,12 @@ __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot
 
 // ------------------------------------------------------------------ shrink ----
 
-// A sum's two planes: hi = round(v), lo = round(v - hi).
+// A sum's two planes: hi = round(v), lo = round(v - hi). Columns that pad the
+// rank are zeros whatever the row: an infinity times their missing weights is
+// no sum.
 template <typename T>
 __device__ __forceinline__ void store_planes(const AdapterParams& p, int64_t slot, int rank, float v) {
+  v = rank < p.rank ? v : 0.f;
   T* high = static_cast<T*>(p.low) + slot * p.rank_pad + rank;
   const T hi = from_float<T>(v);
   const float rest = v - to_float(hi);
@@ -100,8 +103,9 @@ __device__ __forceinline__ void store_planes4(const AdapterParams& p, int64_t sl
   float hi[4], lo[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    hi[i] = to_float(from_float<T>(e[i]));
-    const float rest = e[i] - hi[i];
+    const float sum = rank + i < p.rank ? e[i] : 0.f;
+    hi[i] = to_float(from_float<T>(sum));
+    const float rest = sum - hi[i];
     lo[i] = isfinite(rest) ? rest : 0.f;
   }
   T* to = static_cast<T*>(p.low) + slot * p.rank_pad + rank;  // rank and rank_pad are multiples of 4: 8-byte words

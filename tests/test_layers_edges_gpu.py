@@ -203,3 +203,29 @@ def test_adapters_refuse_a_leaf_before_they_change_it():
         with torch.no_grad():
             assert torch.equal(low_rank_adapters_(refused, x, a, b, batch, scale),
                                low_rank_adapters(base, x, a, b, batch, scale))
+
+
+# ----------------------------------------------------------- adapters' values ----
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [9, 1600])
+@pytest.mark.parametrize("rank", [1, 5, 16, 24])
+def test_adapters_of_any_rank_keep_infinities(rank, tokens, dtype):
+    """An infinite input with weights of one sign is an infinite output: the columns that pad a rank add nothing."""
+    g = rng(rank)
+    batch = AdapterBatch([tokens], [0], 1)
+    x, base = normal(g, tokens, 72, dtype=dtype), normal(g, tokens, 136, dtype=dtype)
+    x[3, 5], x[4, 6] = float("inf"), float("-inf")
+    a, b = normal(g, 1, rank, 72, dtype=dtype).abs() + 0.1, normal(g, 1, 136, rank, dtype=dtype).abs() + 0.1
+    leaf = x.clone().requires_grad_()
+    out = low_rank_adapters(base, leaf, a, b, batch)
+    assert (out[3] == float("inf")).all() and (out[4] == float("-inf")).all()
+    rest = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    rest[3:5] = False
+    assert out[rest].isfinite().all()
+    grad = torch.ones_like(out)
+    grad[7, 9] = float("inf")
+    (dx,) = torch.autograd.grad(out, leaf, grad)
+    assert (dx[7] == float("inf")).all()
+    dx[7] = 0
+    assert dx.isfinite().all()
