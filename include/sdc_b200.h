@@ -497,7 +497,8 @@ int sdc_head_norm_rotary_backward(
  * shrink: low[slot, :] = scale[adapter] * x[rows[slot], :] . weight^T, weight
  * [adapters, rank, width], or [adapters, width, rank] when weight_rank_minor.
  * low: two planes [2][slots][rank padded to 16] of the element type (the
- * value rounded, and what the rounding left), sdc_adapter_low_bytes. */
+ * value rounded, and what the rounding left), sdc_adapter_low_bytes, 16-byte
+ * aligned. fp16 rows are scaled by a power of two that they carry along. */
 size_t sdc_adapter_low_bytes(int64_t slots, int rank);
 int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride,
                        int64_t tokens, const int32_t* rows,

@@ -28,8 +28,16 @@
 //
 // `low` is kept as two 16-bit planes, hi = round(v) and lo = round(v - hi):
 // the tensor cores take 16-bit operands, and the second product then loses
-// 2^-17 of v (2^-22 in fp16) rather than 2^-9, for one more multiply on pipes
-// that wait for memory anyway.
+// 2^-17 of v (2^-21 in fp16) rather than 2^-9, for one more multiply on pipes
+// that wait for memory anyway. bf16 has the range of fp32. fp16 has not: small
+// rows (gradients of a mean loss) would lose their second plane and then their
+// first, large ones would overflow although the other weight brings them back.
+// Its rows are therefore scaled by a power of two that brings the largest finite
+// value into [2^14, 2^15), and products are scaled back: by each row's own power
+// in expand, so that no token depends on another, in outer by one for the tokens
+// that a block adds up. What is 2^-17 of the largest keeps all 21 bits, and 2^-39
+// of it is what is lost. The power travels in the row itself, as the lowest bits
+// of the first eight values of the second plane.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -84,33 +92,139 @@ __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot
 
 // ------------------------------------------------------------------ shrink ----
 
-// A sum's two planes: hi = round(v), lo = round(v - hi). Columns that pad the
-// rank are zeros whatever the row: an infinity times their missing weights is
-// no sum.
 template <typename T>
-__device__ __forceinline__ void store_planes(const AdapterParams& p, int64_t slot, int rank, float v) {
-  v = rank < p.rank ? v : 0.f;
-  T* high = static_cast<T*>(p.low) + slot * p.rank_pad + rank;
-  const T hi = from_float<T>(v);
-  const float rest = v - to_float(hi);
-  high[0] = hi;
-  high[p.slots * p.rank_pad] = from_float<T>(isfinite(rest) ? rest : 0.f);  // an infinite sum stays one
+constexpr bool kScaled = std::is_same_v<T, __half>;
+
+// N neighbouring values of a row's two planes.
+template <typename T, int N>
+struct alignas(2 * N) Planes {
+  T hi[N];
+  alignas(2 * N) T lo[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Planes<T, N> split(const float (&v)[N]) {
+  Planes<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r.hi[i] = from_float<T>(v[i]);
+    const float rest = v[i] - to_float(r.hi[i]);
+    r.lo[i] = from_float<T>(isfinite(rest) ? rest : 0.f);  // an infinite sum stays one
+  }
+  return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_planes4(const AdapterParams& p, int64_t slot, int rank, float4 v) {
-  const float e[4] = {v.x, v.y, v.z, v.w};
-  float hi[4], lo[4];
+// Scaled rows. `back` is the exponent (biased, as in fp32) of the power of two
+// that undoes a row's scale: 1 for rows of zeros, so that the bits that hold it
+// vanish from the products as well.
+__device__ __forceinline__ float power_of_two(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+template <int N>
+__device__ __forceinline__ float largest_finite(const float (&v)[N]) {
+  float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float sum = rank + i < p.rank ? e[i] : 0.f;
-    hi[i] = to_float(from_float<T>(sum));
-    const float rest = sum - hi[i];
-    lo[i] = isfinite(rest) ? rest : 0.f;
+  for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
+  return most;
+}
+template <int LANES>
+__device__ __forceinline__ float neighbours_max(float v) {
+#pragma unroll
+  for (int step = 1; step < LANES; step *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, step));
+  return v;
+}
+__device__ __forceinline__ uint32_t back_for(float largest) {
+  return static_cast<uint32_t>(max(static_cast<int>(__float_as_uint(largest) >> 23) - 14, 1));
+}
+// Values of a row from column `c` on, scaled, and the exponent's bits there.
+template <typename T, int N>
+__device__ __forceinline__ Planes<T, N> split_scaled(const float (&v)[N], uint32_t back, int c) {
+  const float scale = power_of_two(254 - back);
+  float scaled[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) scaled[i] = v[i] * scale;
+  Planes<T, N> r = split<T, N>(scaled);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t bits = __half_as_ushort(r.lo[i]);
+    if (c < 8) r.lo[i] = __ushort_as_half(static_cast<uint16_t>((bits & 0xfffeu) | (back >> (c + i) & 1u)));
   }
-  T* to = static_cast<T*>(p.low) + slot * p.rank_pad + rank;  // rank and rank_pad are multiples of 4: 8-byte words
-  *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]));
-  *reinterpret_cast<uint2*>(to + p.slots * p.rank_pad) = make_uint2(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]));
+  return r;
+}
+// The exponent from the first eight values of a row's second plane.
+__device__ __forceinline__ uint32_t back_of(const uint4& lo) {
+  const uint32_t x = (lo.x & 0x10001u) | (lo.y & 0x10001u) << 2 | (lo.z & 0x10001u) << 4 | (lo.w & 0x10001u) << 6;
+  return (x & 0x55u) | (x >> 15 & 0xaau);
+}
+__device__ __forceinline__ uint4 load_shared4(uint32_t shared) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(shared) : "memory");
+  return w;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_row_planes(const AdapterParams& p, int64_t slot, int c, const Planes<T, N>& r) {
+  using Words = std::conditional_t<N == 4, uint2, std::conditional_t<N == 2, uint32_t, uint16_t>>;
+  static_assert(sizeof(Words) == 2 * N, "one word a plane");
+  T* to = static_cast<T*>(p.low) + slot * p.rank_pad + c;  // c is a multiple of N, rank_pad of 16
+  *reinterpret_cast<Words*>(to) = *reinterpret_cast<const Words*>(r.hi);
+  *reinterpret_cast<Words*>(to + p.slots * p.rank_pad) = *reinterpret_cast<const Words*>(r.lo);
+}
+// Where a row's fp32 values from column `c` on stand in the place of its
+// planes: the first half in the first.
+template <typename T>
+__device__ __forceinline__ float* whole_row(const AdapterParams& p, int64_t slot, int c) {
+  const int half = p.rank_pad / 2;
+  T* plane = static_cast<T*>(p.low) + (slot + (c >= half ? p.slots : 0)) * p.rank_pad;
+  return reinterpret_cast<float*>(plane) + (c >= half ? c - half : c);
+}
+
+// Writes neighbouring sums of a row, c columns into the rank, `in` where there
+// is such a row. Columns that pad the rank are zeros whatever the row: an
+// infinity times their missing weights is no sum. All lanes of a warp call it;
+// LANES neighbours hold a row's part. Scaled rows in several parts wait as fp32
+// for adapter_split.
+template <typename T, int LANES, int N>
+__device__ __forceinline__ void store_low(const AdapterParams& p, bool in, int64_t slot, int c, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = c + i < p.rank ? v[i] : 0.f;
+  in = in && c < p.rank_pad;
+  if constexpr (!kScaled<T>) {
+    if (in) store_row_planes<T, N>(p, slot, c, split<T, N>(v));
+  } else if (gridDim.y > 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (in) *whole_row<T>(p, slot, c + i) = v[i];
+    }
+  } else {
+    const uint32_t back = back_for(neighbours_max<LANES>(largest_finite<N>(v)));
+    if (in) store_row_planes<T, N>(p, slot, c, split_scaled<T, N>(v, back, c));
+  }
+}
+
+// Scaled rows of more than 64 ranks, whose parts come from different blocks of
+// shrink: fp32 to planes in place, a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_split(AdapterParams p) {
+  const Tile tile = p.tiles[blockIdx.x];
+  if (tile.adapter < 0 || tile.adapter >= p.adapters) return;
+  const int lane = threadIdx.x & 31;
+  for (int row = threadIdx.x / 32; row < tile.count; row += 8) {
+    const int64_t slot = static_cast<int64_t>(tile.start) + row;
+    constexpr int kQuads = kMaxRank / 4 / 32;
+    float v[kQuads][4];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int c = (lane + 32 * i) * 4;
+      const float4 q = c < p.rank_pad ? *reinterpret_cast<const float4*>(whole_row<T>(p, slot, c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
+      most = fmaxf(most, largest_finite<4>(v[i]));
+    }
+    const uint32_t back = back_for(neighbours_max<32>(most));  // the whole row has been read
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int c = (lane + 32 * i) * 4;
+      if (c < p.rank_pad) store_row_planes<T, 4>(p, slot, c, split_scaled<T, 4>(v[i], back, c));
+    }
+  }
 }
 
 // Tiles of 16 rows (decoding): the weight is the traffic, and the tensor
@@ -249,17 +363,25 @@ __global__ void __launch_bounds__(NarrowShape<RANK, TRANS>::kThreads) adapter_sh
   }
   cluster_sync();
   const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
-  for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * RANK; e += static_cast<int>(splits) * S::kThreads) {
-    const int row = e / RANK, c = e % RANK;
-    if (rank0 + c >= p.rank_pad) continue;
-    float v = 0.f;
+  constexpr int kEach = RANK > 32 ? RANK / 32 : 1, kLanes = RANK / kEach;  // a row's lanes
+  for (int at = static_cast<int>(split) * S::kThreads + warp * 32; at < count * kLanes; at += static_cast<int>(splits) * S::kThreads) {
+    const int e = at + lane, row = e / kLanes, c = e % kLanes * kEach;
+    const bool in = row < count;
+    float v[kEach] = {};
+    if (in) {
 #pragma unroll 4
-    for (uint32_t s = 0; s < splits; ++s) {
-      const uint32_t from = mapa_shared(part, s) + e * 4;
+      for (uint32_t s = 0; s < splits; ++s) {
+        const uint32_t from = mapa_shared(part, s) + (row * RANK + c) * 4;
 #pragma unroll
-      for (int other = 0; other < 4; ++other) v += load_cluster_f32(from + other * ROWS * RANK * 4);
+        for (int other = 0; other < 4; ++other) {
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) v[i] += load_cluster_f32(from + (other * ROWS * RANK + i) * 4);
+        }
+      }
     }
-    store_planes<T>(p, tile.start + row, rank0 + c, v * scale);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) v[i] *= scale;
+    store_low<T, kLanes, kEach>(p, in, tile.start + row, rank0 + c, v);
   }
   cluster_sync();  // the others may still be reading this block's sums
 }
@@ -373,7 +495,7 @@ __device__ __forceinline__ float4 sum_cluster(const float* part, int at, uint32_
 // This thread's row of an accumulator (zeros where nothing was multiplied);
 // PLANES: 2 where RANK further columns hold the second plane's sums.
 template <int RANK, int PLANES>
-__device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any) {
+__device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any, float back = 1.f) {
   constexpr int kStep = RANK < 32 ? RANK : 32;
 #pragma unroll
   for (int c0 = 0; c0 < RANK; c0 += kStep) {
@@ -395,7 +517,7 @@ __device__ __forceinline__ void store_part(float* row, uint32_t accumulator, boo
 #pragma unroll
     for (int c = 0; c < kStep; c += 4) {
       *reinterpret_cast<float4*>(row + c0 + c) =
-          any ? make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          any ? make_float4(f[c] * back, f[c + 1] * back, f[c + 2] * back, f[c + 3] * back) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
 }
@@ -523,11 +645,12 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
   if (warp == 8) tmem_dealloc(accumulator, S::kTensorColumns);
   const float scale = p.scale != nullptr && valid ? p.scale[tile.adapter] : 1.f;
   constexpr int kQuads = RANK / 4;
-  for (int e = static_cast<int>(split) * S::kThreads + tid; e < count * kQuads; e += static_cast<int>(splits) * S::kThreads) {
-    const int row = e / kQuads, c = e % kQuads * 4;
-    if (rank0 + c >= p.rank_pad) continue;
-    const float4 v = sum_cluster(part, row * S::kPartPitch + c, splits);
-    store_planes4<T>(p, tile.start + row, rank0 + c, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
+  for (int at = static_cast<int>(split) * S::kThreads + warp * 32; at < count * kQuads; at += static_cast<int>(splits) * S::kThreads) {
+    const int e = at + lane, row = e / kQuads, c = e % kQuads * 4;
+    const bool in = e < count * kQuads;
+    const float4 sum = in ? sum_cluster(part, row * S::kPartPitch + c, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float v[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
+    store_low<T, kQuads, 4>(p, in, tile.start + row, rank0 + c, v);
   }
   cluster_sync();  // the others may still be reading this block's sums
 }
@@ -614,9 +737,11 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
   }
 
   // This thread's part of base and out: rows lane / 4 and lane / 4 + 8, 8
-  // columns of the warp's 32. The accumulators start from it.
+  // columns of the warp's 32. The accumulators start from it, or it is added to
+  // the products of scaled rows.
   const int column = column0 + warp * 32 + (lane & 3) * 8;
   float acc[4][4];
+  Raw8<T> base[2];
   T* out[2];
   int limit[2];  // columns of out; 0 where there is no row
 #pragma unroll
@@ -625,14 +750,13 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
     const int64_t token = row < tile.count ? token_of(p, tile.start + row) : -1;
     limit[h] = token >= 0 ? width - column : 0;
     out[h] = static_cast<T*>(p.out) + token * p.out_stride + column;
-    Raw8<T> base;
-    base.w[0] = make_uint4(0, 0, 0, 0);
+    base[h].w[0] = make_uint4(0, 0, 0, 0);
     const T* from = static_cast<const T*>(p.base) + token * p.base_stride + column;
     if (p.base != nullptr) {
       if constexpr (FAST) {
-        if (limit[h] > 0) base = load8(from);
+        if (limit[h] > 0) base[h] = load8(from);
       } else {
-        T* e = reinterpret_cast<T*>(&base);
+        T* e = reinterpret_cast<T*>(&base[h]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (j < limit[h]) e[j] = from[j];
@@ -640,9 +764,12 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
       }
     }
     float v[8];
-    unpack8(base, v);
+    unpack8(base[h], v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j][2 * h] = v[2 * j], acc[j][2 * h + 1] = v[2 * j + 1];
+    for (int j = 0; j < 4; ++j) {
+      acc[j][2 * h] = kScaled<T> ? 0.f : v[2 * j];
+      acc[j][2 * h + 1] = kScaled<T> ? 0.f : v[2 * j + 1];
+    }
   }
 
   griddep_wait();  // `low` from here on
@@ -686,8 +813,20 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float v[8];
+    if (kScaled<T> && adapted) {
+      const float back = power_of_two(back_of(load_shared4(low_shared + (kNarrow + (lane >> 2) + 8 * h) * pitch)));
+      unpack8(base[h], v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[2 * j] = acc[j][2 * h], v[2 * j + 1] = acc[j][2 * h + 1];
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = fmaf(acc[j][2 * h], back, v[2 * j]);
+        v[2 * j + 1] = fmaf(acc[j][2 * h + 1], back, v[2 * j + 1]);
+      }
+    } else if constexpr (kScaled<T>) {
+      unpack8(base[h], v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[2 * j] = acc[j][2 * h], v[2 * j + 1] = acc[j][2 * h + 1];
+    }
     if constexpr (FAST) {
       if (limit[h] > 0) store8(out[h], pack8<T>(v));
     } else {
@@ -920,17 +1059,26 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       // one were (it has completed), a new weight where the one before this
       // was; with room for one only it waits for this product.
       weight_shared = newest;
+      // Scaled rows: their powers are read with the products they belong to.
+      if (kScaled<T> && product > 0 && !wait(&drained, product - 1)) break;
       const bool early = !mine || next.adapter == adapter || p.weights == 2;
       if (early) load(next, next_product);
       look(next, next_token);
       if (mine && warp == 0) multiply(product);
       if (mine && !wait(&ready, product)) break;
+      if (kScaled<T> && mine && !wait(&loaded[product & 1], product >> 1)) break;  // long there: for the rows' powers
       products = next_product;
       if (!early) load(next, next_product);
       check(next_token);
       tc_fence_after();
 #pragma unroll
       for (int half = 0; half < S::kHalves; ++half) {
+        float back[2] = {1.f, 1.f};
+        if (kScaled<T> && mine) {
+          const uint32_t at = low_shared + (product & 1) * S::low_bytes(pad) + pieces * S::kLowStep;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) back[h] = power_of_two(back_of(load_shared4(at + (row0 + 16 * half + 8 * h) * 16)));
+        }
 #pragma unroll
         for (int g = 0; g < S::kGroups; ++g) {
           uint32_t d[16];
@@ -946,8 +1094,8 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
             if (mine) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                v[2 * j] += __uint_as_float(d[4 * j + 2 * h]);
-                v[2 * j + 1] += __uint_as_float(d[4 * j + 2 * h + 1]);
+                v[2 * j] = fmaf(__uint_as_float(d[4 * j + 2 * h]), back[h], v[2 * j]);
+                v[2 * j + 1] = fmaf(__uint_as_float(d[4 * j + 2 * h + 1]), back[h], v[2 * j + 1]);
               }
             }
             const int32_t row = token[2 * half + h];
@@ -996,7 +1144,9 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
 // 40 in a backward pass, where earlier writes are still leaving L2; each
 // further 16384 rows take 24 (4.9 TB/s). Register accumulators took 68. A block takes 256 columns and RANK ranks; the blocks of a
 // cluster share the adapter's tokens.
-template <int RANK>
+// Scaled rows: the pieces of a row are read and written again by neighbouring
+// lanes, so the panels stand 128 bytes / panels further apart, on other banks.
+template <int RANK, bool SCALED>
 struct OuterShape {
   static constexpr int kThreads = kTensorThreads;
   static constexpr int kColumns = 256;
@@ -1004,8 +1154,9 @@ struct OuterShape {
   static constexpr int kStages = 4;
   static constexpr int kSubBytes = kTokens * 128;  // 64 columns
   static constexpr int kRowBytes = kColumns / 64 * kSubBytes;
-  static constexpr int kPlaneBytes = kTokens * RANK * 2;
-  static constexpr int kStageBytes = kRowBytes + 2 * kPlaneBytes;
+  static constexpr int kPanelBytes = kTokens * 16 + (SCALED ? 128 / (RANK / 8) : 0);
+  static constexpr int kPlaneBytes = RANK / 8 * kPanelBytes;
+  static constexpr int kStageBytes = (kRowBytes + 2 * kPlaneBytes + 1023) / 1024 * 1024;  // the swizzle goes by address bits
   static constexpr int kTensorColumns = 4 * RANK;
   static constexpr int kPartPitch = RANK + 4;
   static constexpr int kPartBytes = kColumns * kPartPitch * 4 * 3 / 2;  // and a cluster's share, at most half
@@ -1013,8 +1164,8 @@ struct OuterShape {
 };
 
 template <typename T, int RANK, bool FAST>
-__global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(AdapterParams p) {
-  using S = OuterShape<RANK>;
+__global__ void __launch_bounds__(kTensorThreads, 2) adapter_outer(AdapterParams p) {
+  using S = OuterShape<RANK, kScaled<T>>;
   extern __shared__ uint8_t shared_raw[];
   __shared__ TensorRing<S::kStages> ring;
   uint8_t* shared = shared_raw + (-smem_u32(shared_raw) & 1023u);  // the swizzle goes by address bits
@@ -1037,6 +1188,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   tc_fence_after();
   const uint32_t accumulator = ring.tensor_memory;
 
+  uint32_t back = 127;  // scaled rows: the block's, the same for all filling threads
   if (warp < 8) {
     constexpr int kRowCopies = S::kTokens / 8;  // a warp copies rows warp, warp + 8, ...: whole lines
     static_assert(S::kColumns == 32 * 8, "a lane copies one piece of a row");
@@ -1049,6 +1201,8 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
     const bool low_in = rank0 + low_piece * 8 < p.rank_pad;
     const T* low = static_cast<const T*>(p.low) + (low_in ? rank0 + low_piece * 8 : 0);
     const uint32_t low_to = stages + S::kRowBytes;
+    const int row_of_low = low_row % S::kTokens;  // of all of a thread's pieces of a tile
+    static_assert(kLowStep % S::kTokens == 0, "a thread's pieces are of one row");
 
     // Tokens of the warp's rows of 8 tiles, one a lane, read 8 tiles ahead.
     auto look = [&](int tile) {
@@ -1059,13 +1213,11 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
     };
     constexpr int kBatch = 32 / kRowCopies;
     int32_t tokens = look(first), next_tokens = look(first + kBatch);
-    for (int tile = first; tile < last; ++tile) {
-      const int fill = tile - first;
-      if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+    auto copy_rows = [&](int fill) {
       const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
       if (fill > 0 && fill % kBatch == 0) {
         tokens = next_tokens;
-        next_tokens = look(tile + kBatch);
+        next_tokens = look(first + fill + kBatch);
       }
 #pragma unroll
       for (int i = 0; i < kRowCopies; ++i) {
@@ -1073,16 +1225,104 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
         copy8<T, FAST>(row_to + stage + i * 8 * 128, x + static_cast<int64_t>(max(token, 0)) * p.row_stride,
                        token >= 0 ? columns_left : 0);
       }
-      const int slot0 = begin + tile * S::kTokens;
+    };
+    auto copy_low = [&](int fill) {
+      const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
+      const int slot = begin + (first + fill) * S::kTokens + row_of_low;
+      const bool in = low_in && slot < end;
 #pragma unroll
       for (int i = 0; i < kLowCopies; ++i) {
-        const int at = low_row + i * kLowStep, plane = at / S::kTokens, row = at % S::kTokens;
-        if (2 * S::kTokens % kLowStep != 0 && at >= 2 * S::kTokens) continue;
-        const bool in = low_in && slot0 + row < end;
-        cp_async16(low_to + stage + plane * S::kPlaneBytes + paneled(row, low_piece, S::kTokens * 16),
-                   low + (in ? (plane * p.slots + slot0 + row) * p.rank_pad : 0), in);
+        const int plane = (low_row + i * kLowStep) / S::kTokens;
+        if (plane >= 2) continue;
+        cp_async16(low_to + stage + plane * S::kPlaneBytes + paneled(row_of_low, low_piece, S::kPanelBytes),
+                   low + (in ? (plane * p.slots + slot) * p.rank_pad : 0), in);
       }
-      ring.filled<FAST>(fill);
+    };
+    const int fills = last - first;
+    if constexpr (!kScaled<T>) {
+      for (int fill = 0; fill < fills; ++fill) {
+        if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+        copy_rows(fill);
+        copy_low(fill);
+        ring.filled<FAST>(fill);
+      }
+    } else {
+      // Scaled rows: their planes arrive as they are and each thread brings its
+      // own pieces to the block's power, that of its largest row, two fillings
+      // later. (Pieces loaded into registers took twice the time: an arrival at a
+      // barrier waits for the thread's loads, whichever they are for.)
+      constexpr int kAhead = 2;
+      for (int fill = 0; fill < kAhead; ++fill) {
+        if (fill < fills) copy_rows(fill), copy_low(fill);
+        cp_async_commit();
+      }
+      const T* second = static_cast<const T*>(p.low) + p.slots * p.rank_pad;
+      auto power = [&](int slot) {
+        return slot < end ? *reinterpret_cast<const uint4*>(second + static_cast<int64_t>(slot) * p.rank_pad) : make_uint4(0, 0, 0, 0);
+      };
+      // Powers of the rows that the warp's pieces are of, for 8 tiles, one or more
+      // a lane, read 8 tiles ahead.
+      constexpr int kWarpRows = 32 / kLowPieces, kPowers = 8 / kLowPieces;
+      auto powers_of = [&](int fill, uint4 (&to)[kPowers]) {
+#pragma unroll
+        for (int i = 0; i < kPowers; ++i) {
+          const int tile = first + fill + i * kLowPieces + lane / kWarpRows;
+          const int row = (warp * kWarpRows + lane % kWarpRows) % S::kTokens;
+          to[i] = tile < last ? power(begin + tile * S::kTokens + row) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      uint4 next_powers[kPowers];
+      uint32_t powers[kPowers];
+      powers_of(0, next_powers);
+      __shared__ uint32_t warps[kFillThreads / 32];
+      uint32_t most = 1;
+#pragma unroll 4
+      for (int slot = begin + first * S::kTokens + tid; slot < begin + last * S::kTokens; slot += kFillThreads) {
+        most = max(most, back_of(power(slot)));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) warps[warp] = most;
+      named_barrier(1, kFillThreads);
+      back = __reduce_max_sync(0xffffffffu, warps[lane % (kFillThreads / 32)]);
+
+      for (int fill = 0; fill < fills; ++fill) {
+        const int ahead = fill + kAhead;
+        if (ahead < fills) {
+          if (ahead >= S::kStages && !ring.wait(ring.used, ahead - S::kStages, p.watchdog)) break;
+          copy_rows(ahead);
+          copy_low(ahead);
+        }
+        cp_async_commit();
+        if (fill % 8 == 0) {
+#pragma unroll
+          for (int i = 0; i < kPowers; ++i) powers[i] = back_of(next_powers[i]);
+          powers_of(fill + 8, next_powers);
+        }
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPowers; ++i) {
+          const uint32_t other = __shfl_sync(0xffffffffu, powers[i], fill % kLowPieces * kWarpRows + lane / kLowPieces);
+          if (fill % 8 / kLowPieces == i) mine = other;
+        }
+        const float scale = power_of_two(static_cast<uint32_t>(max(127 + static_cast<int>(mine) - static_cast<int>(back), 0)));
+        const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
+        cp_async_wait<kAhead>();
+#pragma unroll
+        for (int i = 0; i < kLowCopies; ++i) {
+          const int plane = (low_row + i * kLowStep) / S::kTokens;
+          if (plane >= 2) continue;
+          const uint32_t at = low_to + stage + plane * S::kPlaneBytes + paneled(row_of_low, low_piece, S::kPanelBytes);
+          Raw8<T> raw;
+          raw.w[0] = load_shared4(at);
+          float v[8];
+          unpack8(raw, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= scale;
+          const uint4 w = pack8<T>(v).w[0];
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+        }
+        mbar_arrive(&ring.full[fill % S::kStages]);
+      }
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -1090,7 +1330,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
     constexpr uint32_t kInstruction = idesc_f16<T>(128, 2 * RANK, true, true);
     // Groups of 8 slots are 1024 bytes apart, runs of 64 columns kSubBytes.
     const uint64_t a = smem_desc(stages, S::kSubBytes, 1024, 2);
-    const uint64_t b = smem_desc(stages + S::kRowBytes, 128, S::kTokens * 16, 0);
+    const uint64_t b = smem_desc(stages + S::kRowBytes, 128, S::kPanelBytes, 0);
     ring.multiply(last - first, p.watchdog, [&](int fill) {
       // Addresses advance in the descriptors' units of 16 bytes.
       const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
@@ -1111,7 +1351,7 @@ __global__ void __launch_bounds__(OuterShape<RANK>::kThreads, 2) adapter_outer(A
   if (warp < 8) {
     const int half = warp / 4, c = half * 128 + warp % 4 * 32 + lane;
     store_part<RANK, 2>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * 2 * RANK,
-                        first < last);
+                        first < last, power_of_two(back));
   }
   tc_fence_before();
   cluster_sync();
@@ -1220,11 +1460,18 @@ int launch_shrink(AdapterParams p, int64_t tiles, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(tiles * split), rank_blocks);
   const bool fast = p.vector_rows && p.vector_weight && p.width % 8 == 0 && (!TRANS || p.rank % 8 == 0);
   auto launch = [&](auto kernel) { return launch_clustered(kernel, p, grid, S::kThreads, split, S::kBytes, false, stream); };
+  int rc;
   if constexpr (ROWS == kWide) {
-    return fast ? launch(adapter_shrink_wide<T, RANK, TRANS, true>) : launch(adapter_shrink_wide<T, RANK, TRANS, false>);
+    rc = fast ? launch(adapter_shrink_wide<T, RANK, TRANS, true>) : launch(adapter_shrink_wide<T, RANK, TRANS, false>);
   } else {
-    return fast ? launch(adapter_shrink<T, RANK, TRANS, true>) : launch(adapter_shrink<T, RANK, TRANS, false>);
+    rc = fast ? launch(adapter_shrink<T, RANK, TRANS, true>) : launch(adapter_shrink<T, RANK, TRANS, false>);
   }
+  if constexpr (kScaled<T>) {
+    if (rc != SDC_OK || rank_blocks == 1) return rc;
+    adapter_split<T><<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p);
+    SDC_CUDA_CHECK(cudaGetLastError());
+  }
+  return rc;
 }
 
 template <typename T, int ROWS, bool TRANS>
@@ -1292,7 +1539,7 @@ int expand_typed(const AdapterParams& p, int tile_rows, bool trans, int64_t tile
 
 template <typename T, int RANK>
 int launch_outer(const AdapterParams& p, cudaStream_t stream) {
-  using S = OuterShape<RANK>;
+  using S = OuterShape<RANK, kScaled<T>>;
   const int64_t columns = ceil_div(p.width, S::kColumns);
   const unsigned rank_blocks = static_cast<unsigned>(ceil_div(p.rank, RANK));
   const int64_t tiles = ceil_div(ceil_div(p.slots, p.adapters), S::kTokens);

@@ -96,8 +96,11 @@ def low_rank_adapters(base, x, a, b, batch, scale=None):
     ``AdapterBatch`` of the same tokens and count. Tokens without an adapter
     keep ``base``. Returns a new tensor; differentiable in ``base``, ``x``,
     ``a`` and ``b``. Adapters without tokens get zero gradients. The low-rank
-    rows are kept in 32 bits up to the second product, which takes them as two
-    16-bit terms; in fp16 they overflow beyond 65504 like the type does."""
+    rows (and their gradients) are sums in 32 bits; the second product takes
+    them as two 16-bit terms, which lose 2^-17 of a value in bf16. In fp16 they
+    are scaled by a power of two first, so that the range is that of fp32, and
+    lose 2^-21 of a value and 2^-39 of the largest: of the token's own row, or
+    in the weights' gradients of the tokens added up."""
     _check(x, batch)
     return _OP(base, x, a, b, scale, *batch.arguments(a.shape[1]))[0]
 

@@ -229,3 +229,92 @@ def test_adapters_of_any_rank_keep_infinities(rank, tokens, dtype):
     assert (dx[7] == float("inf")).all()
     dx[7] = 0
     assert dx.isfinite().all()
+
+
+def close(got, exact, magnitude, arithmetic):
+    """One rounding of ``exact`` to fp16 and ``arithmetic`` times ``magnitude``."""
+    tolerance = 2.0 ** -11 * exact.abs() * (1 + 2.0 ** -10) + 2.0 ** -25 + arithmetic * magnitude
+    off = (got.double() - exact).abs()
+    bad = ~(off <= tolerance)
+    assert not bad.any(), (off[bad].max().item(), tolerance[bad].min().item(), int(bad.sum()))
+
+
+# Two terms of the low-rank rows lose 2^-21, and the floor of their scaling (2^-39 of the largest) less than that among
+# normal rows; fp32 sums of n products lose at most n 2^-23 of their magnitude.
+def fp16_arithmetic(*lengths):
+    return 2.0 ** -20 + sum(lengths) * 2.0 ** -23
+
+
+def adapters64(x, base, a, b, grad):
+    """One adapter's outputs and gradients, each with the magnitude of what enters its elements."""
+    def run(x, base, a, b, grad):
+        low, down = x @ a.T, grad @ b
+        return base + low @ b.T, down @ a, down.T @ x, grad.T @ low
+    x, base, a, b, grad = (t.double() for t in (x, base, a, b, grad))
+    return list(zip(run(x, base, a, b, grad), run(x.abs(), base.abs(), a.abs(), b.abs(), grad.abs())))
+
+
+# Scales of x, a, b and the gradient. The gradients of a mean loss beside a weight that starts near zero: low-rank rows
+# of 1e-7 (fp16 ends at 6e-8). Large inputs: rows beyond 65504 that the second weight brings back.
+FP16_RANGES = {"small": (1.0, 0.05, 1e-3, 1e-5), "smaller": (1e-2, 1e-3, 10.0, 1e-6), "large": (100.0, 10.0, 1e-4, 1e-4)}
+
+
+@pytest.mark.parametrize("ranges", list(FP16_RANGES))
+@pytest.mark.parametrize("tokens,rank,k,n", [(1, 16, 200, 136), (60, 5, 104, 520), (300, 256, 264, 136), (1600, 24, 200, 136),
+                                             (1600, 64, 37, 53), (2100, 100, 200, 136), (1600, 256, 264, 136)])
+def test_fp16_adapters_over_the_range_of_their_low_rows(tokens, rank, k, n, ranges):
+    g = rng(tokens + rank)
+    sx, sa, sb, sg = FP16_RANGES[ranges]
+    dtype = torch.float16
+    x, base, grad = (normal(g, tokens, k, dtype=dtype, scale=sx), normal(g, tokens, n, dtype=dtype),
+                     normal(g, tokens, n, dtype=dtype, scale=sg))
+    a, b = normal(g, 1, rank, k, dtype=dtype, scale=sa), normal(g, 1, n, rank, dtype=dtype, scale=sb)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    out = low_rank_adapters(base, *leaves, AdapterBatch([tokens], [0], 1))
+    dx, da, db = torch.autograd.grad(out, leaves, grad)
+    exact = adapters64(x, base, a[0], b[0], grad)
+    for got, (value, size), lengths in zip((out.detach(), dx, da[0], db[0]), exact,
+                                           ((k, rank), (n, rank), (n, tokens), (k, tokens))):
+        close(got, value, size, fp16_arithmetic(*lengths))
+
+
+@pytest.mark.parametrize("tokens", [40, 1700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapters_of_a_token_do_not_depend_on_the_other_tokens_values(tokens, dtype):
+    g = rng(tokens)
+    x, base = normal(g, tokens, 128, dtype=dtype), normal(g, tokens, 264, dtype=dtype)
+    a, b = normal(g, 1, 24, 128, dtype=dtype, scale=0.1), normal(g, 1, 264, 24, dtype=dtype, scale=0.1)
+    grad, batch = normal(g, tokens, 264, dtype=dtype), AdapterBatch([tokens], [0], 1)
+
+    def results(x, grad):
+        leaf = x.clone().requires_grad_()
+        out = low_rank_adapters(base, leaf, a, b, batch)
+        return out, torch.autograd.grad(out, leaf, grad)[0]
+
+    want = results(x, grad)
+    changed = torch.arange(0, tokens, 3, device=DEV)
+    factors = torch.tensor([2.0 ** -14, 1e3, 0.0, float("inf")], device=DEV)[torch.arange(len(changed), device=DEV) % 4, None]
+    x2, grad2 = x.clone(), grad.clone()
+    x2[changed] = (x2[changed].float() * factors).to(dtype)
+    grad2[changed] = (grad2[changed].float() * factors).to(dtype)
+    rest = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    rest[changed] = False
+    for got, expected in zip(results(x2, grad2), want):
+        assert torch.equal(got[rest], expected[rest])
+
+
+def test_fp16_adapters_add_tokens_of_unlike_sizes():
+    """The weights' gradients of tokens between 2^-14 and 2^7 of one another, in long and short runs."""
+    dtype = torch.float16
+    for tokens in (50, 1600, 5000):
+        g = rng(tokens)
+        size = 2.0 ** torch.randint(-14, 8, (tokens, 1), device=DEV, generator=g)
+        x, grad = (normal(g, tokens, 136) * size).to(dtype), (normal(g, tokens, 264) * size.flip(0) * 2.0 ** -8).to(dtype)
+        base = normal(g, tokens, 264, dtype=dtype)
+        a, b = normal(g, 1, 40, 136, dtype=dtype, scale=0.1), normal(g, 1, 264, 40, dtype=dtype, scale=0.1)
+        leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+        out = low_rank_adapters(base, *leaves, AdapterBatch([tokens], [0], 1))
+        dx, da, db = torch.autograd.grad(out, leaves, grad)
+        for got, (value, magnitude), lengths in zip((out.detach(), dx, da[0], db[0]), adapters64(x, base, a[0], b[0], grad),
+                                                    ((136, 40), (264, 40), (264, tokens), (136, tokens))):
+            close(got, value, magnitude, fp16_arithmetic(*lengths))
