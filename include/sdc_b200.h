@@ -79,14 +79,16 @@ const char* sdc_last_error(void);
 int sdc_device_check(int device);
 /* Reads and clears the device watchdog word of the current device: 0 when no
  * kernel gave up a bounded wait since the last call, otherwise the code of the
- * first wait that expired. Synchronises `stream`. */
+ * first wait that expired (1 to 8: the GEMMs, 9: low-rank adapters, 10:
+ * distillation loss with gradient). Synchronises `stream`. */
 int sdc_read_device_error(sdc_stream_t stream, int32_t* code);
 /* Test hook (no counterpart in the reference): wait_limit_ns != 0 replaces the
- * 2 s limit of every bounded wait in later GEMM launches; pace_extra > 0 is
+ * 2 s limit of every bounded wait in later launches; pace_extra > 0 is
  * added to the prediction warps' pacing targets, which makes their wait
- * unreachable so that it expires. (0, 0) restores normal operation. Lets a
- * test check that an expired wait is reported in-band (hit bit 1, detected)
- * without hanging or faulting the GPU. */
+ * unreachable so that it expires, and gives the layer operators a wait of that
+ * kind. (0, 0) restores normal operation. Lets a test check that an expired wait
+ * is reported in-band (GEMMs: hit bit 1, detected; layer operators: NaN) without
+ * hanging or faulting the GPU. */
 int sdc_test_set_watchdog(uint64_t wait_limit_ns, int32_t pace_extra);
 /* Test hook (no counterpart in the reference): how later K-slice launches
  * compute their prediction. 0 (default) chooses by shape; 1 forces the
@@ -450,7 +452,9 @@ int sdc_abft_correct_fp8_block(const uint8_t* a, const uint8_t* b_rows,
 
 /* ---- layer operators beside the protected GEMMs (extension) --------------
  * None of these has a counterpart in the reference. Element types: 0 fp32,
- * 1 bf16, 2 fp16; arithmetic is fp32 with one rounding at the store.
+ * 1 bf16, 2 fp16; arithmetic is fp32 with one rounding at the store. Where a
+ * kernel gives up a bounded wait, all that its block (its cluster, in the loss
+ * with gradient) was to write is NaN, and sdc_read_device_error tells.
  *
  * Norm of each query and key head and rotation by position, one pass.
  * q [batch, sequence, heads_q, dim], k [batch, sequence, heads_k, dim] with

@@ -80,6 +80,8 @@ struct AdapterParams {
   int64_t out_rank_stride;   // outer
   int chunks_per_split;
   int32_t* watchdog;
+  uint64_t wait_limit_ns;
+  bool expire;               // test hook: a wait that nothing ends
   int tile_count, tiles_per_block;  // expand
   int weights;               // expand of wide tiles: buffers of weights, 1 or 2
   int piece_bits;            // expand: 2^piece_bits >= rank_pad / 8 threads copy a row
@@ -412,12 +414,13 @@ __device__ __forceinline__ uint32_t paneled(int k, int panel, int stride) { retu
 // filling is full when every filling thread's copies have arrived, and its
 // stage is free again when the products that read it have completed. Waits
 // are bounded: one that runs out is recorded in the watchdog word, the warps
-// leave their loops one after the other and meet at the block's next barrier.
+// leave their loops one after the other and meet at the block's next barrier,
+// where the block's sums become NaN, so that nothing made of them looks whole.
 constexpr int kFillThreads = 256, kTensorThreads = kFillThreads + 32;
 
 template <int STAGES>
 struct TensorRing {
-  uint64_t full[STAGES], used[STAGES];
+  uint64_t full[STAGES], used[STAGES], never;
   uint32_t tensor_memory;
   int32_t abort;
 
@@ -428,6 +431,7 @@ struct TensorRing {
         mbar_init(&full[i], kFillThreads);
         mbar_init(&used[i], 1);
       }
+      mbar_init(&never, 1);
       fence_barrier_init();
       abort = 0;
     }
@@ -437,9 +441,11 @@ struct TensorRing {
   }
   // Until the index-th filling is full, or its products have completed. The
   // same for a whole warp.
-  __device__ __forceinline__ bool wait(uint64_t* bars, int index, int32_t* watchdog) {
-    const uint32_t parity = static_cast<uint32_t>(index / STAGES) & 1;
-    return __all_sync(0xffffffffu, mbar_wait(&bars[index % STAGES], parity, kWaitAccum, &abort, watchdog)) != 0;
+  __device__ __forceinline__ bool wait(uint64_t* bars, int index, const AdapterParams& p) {
+    return wait_bar(&bars[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1, p);
+  }
+  __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const AdapterParams& p) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, kWaitAdapters, &abort, p.watchdog, p.wait_limit_ns)) != 0;
   }
   // A filling thread's copies of a filling have been issued (FAST: the
   // barrier counts it when they arrive) or made.
@@ -454,15 +460,19 @@ struct TensorRing {
       mbar_arrive(&full[index % STAGES]);
     }
   }
+  // After the block's barrier behind the loops.
+  __device__ __forceinline__ bool gave_up() const { return abort != 0; }
+  __device__ __forceinline__ float instead() const { return gave_up() ? __int_as_float(0x7fffffff) : 0.f; }
   __device__ __forceinline__ void drain(int index) {
     mbar_drain(&used[index % STAGES], static_cast<uint32_t>(index / STAGES) & 1);
   }
   // The ninth warp: products of `count` fillings, issued by one lane.
   template <typename Products>
-  __device__ __forceinline__ void multiply(int count, int32_t* watchdog, const Products& products) {
+  __device__ __forceinline__ void multiply(int count, const AdapterParams& p, const Products& products) {
     int done = 0;
+    if (p.expire && count > 0 && !wait_bar(&never, 0, p)) return;
     for (; done < count; ++done) {
-      if (!wait(full, done, watchdog)) break;
+      if (!wait(full, done, p)) break;
       fence_proxy_async_smem();  // the copies were made by ordinary writes
       tc_fence_after();
       if ((threadIdx.x & 31) == 0) {
@@ -492,10 +502,10 @@ __device__ __forceinline__ float4 sum_cluster(const float* part, int at, uint32_
   }
   return sum;
 }
-// This thread's row of an accumulator (zeros where nothing was multiplied);
+// This thread's row of an accumulator, or `instead` where nothing was multiplied;
 // PLANES: 2 where RANK further columns hold the second plane's sums.
 template <int RANK, int PLANES>
-__device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any, float back = 1.f) {
+__device__ __forceinline__ void store_part(float* row, uint32_t accumulator, bool any, float instead, float back = 1.f) {
   constexpr int kStep = RANK < 32 ? RANK : 32;
 #pragma unroll
   for (int c0 = 0; c0 < RANK; c0 += kStep) {
@@ -517,7 +527,8 @@ __device__ __forceinline__ void store_part(float* row, uint32_t accumulator, boo
 #pragma unroll
     for (int c = 0; c < kStep; c += 4) {
       *reinterpret_cast<float4*>(row + c0 + c) =
-          any ? make_float4(f[c] * back, f[c + 1] * back, f[c + 2] * back, f[c + 3] * back) : make_float4(0.f, 0.f, 0.f, 0.f);
+          any ? make_float4(f[c] * back, f[c + 1] * back, f[c + 2] * back, f[c + 3] * back)
+              : make_float4(instead, instead, instead, instead);
     }
   }
 }
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
                                (TRANS ? paneled(weight_row, weight_piece, S::kChunk * 16) : swizzled(weight_row, weight_piece));
     constexpr int kWeightStride = kWeightStep * (TRANS ? 16 : 128);
     for (int fill = 0; fill < last - first; ++fill) {
-      if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+      if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p)) break;
       const uint32_t stage = static_cast<uint32_t>(fill % S::kStages) * S::kStageBytes;
 #pragma unroll
       for (int i = 0; i < kRowCopies; ++i) {
@@ -623,7 +634,7 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
     constexpr uint32_t kInstruction = idesc_f16<T>(kWide, RANK, false, TRANS);
     const uint64_t a = sw128_desc(stages);
     const uint64_t b = TRANS ? smem_desc(stages + S::kRowBytes, 128, S::kChunk * 16, 0) : sw128_desc(stages + S::kRowBytes);
-    ring.multiply(last - first, p.watchdog, [&](int fill) {
+    ring.multiply(last - first, p, [&](int fill) {
       // Addresses advance in the descriptors' units of 16 bytes.
       const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
 #pragma unroll
@@ -633,11 +644,12 @@ __global__ void __launch_bounds__(WideShape<RANK, TRANS>::kThreads, 2) adapter_s
     });
   }
   float* part = reinterpret_cast<float*>(shared);
-  if (first < last) ring.wait(ring.used, last - 1 - first, p.watchdog);
+  if (first < last) ring.wait(ring.used, last - 1 - first, p);
   tc_fence_after();
   __syncthreads();
   if (warp < 4) {
-    store_part<RANK, 1>(part + (warp * 32 + lane) * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp) << 21), first < last);
+    store_part<RANK, 1>(part + (warp * 32 + lane) * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp) << 21),
+                        first < last && !ring.gave_up(), ring.instead());
   }
   tc_fence_before();
   cluster_sync();
@@ -881,7 +893,7 @@ template <typename T, bool TRANS, bool FAST>
 __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(AdapterParams p) {
   using S = ExpandWide;
   extern __shared__ __align__(128) uint8_t shared[];
-  __shared__ uint64_t loaded[2], ready, drained;
+  __shared__ uint64_t loaded[2], ready, drained, never;
   __shared__ uint32_t tensor_memory;
   __shared__ int32_t abort;
   const int width = static_cast<int>(p.width), pad = p.rank_pad, pieces = pad / 8;
@@ -898,6 +910,7 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       mbar_init(&loaded[1], kFillThreads);
       mbar_init(&ready, 1);
       mbar_init(&drained, S::kWarps);
+      mbar_init(&never, 1);
       fence_barrier_init();
       abort = 0;
     }
@@ -912,14 +925,17 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
   // False for the whole warp once a wait of the block has run out: the warps
   // then leave their loops one after the other and meet at the last barrier.
   auto wait = [&](uint64_t* bar, int index) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, static_cast<uint32_t>(index) & 1, kWaitAccum, &abort, p.watchdog)) != 0;
+    const uint32_t parity = static_cast<uint32_t>(index) & 1;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, kWaitAdapters, &abort, p.watchdog, p.wait_limit_ns)) != 0;
   };
   auto adapted = [&](const Tile& tile) { return tile.adapter >= 0 && tile.adapter < p.adapters; };
   constexpr Tile kNone{0, 0, -1};
 
   // Warp 0, one lane: a tile's product, once its operands are there and the
   // last one has been read.
+  int issued = 0;
   auto multiply = [&](int product) {
+    if (p.expire && product == 0 && !wait(&never, 0)) return;
     if (!wait(&loaded[product & 1], product >> 1) || (product > 0 && !wait(&drained, product - 1))) return;
     fence_proxy_async_smem();  // the copies were made by ordinary writes
     tc_fence_after();
@@ -937,9 +953,9 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       }
       tc_commit(&ready);
     }
+    issued = product + 1;
     __syncwarp();
   };
-  int products = 0;
   {
     // Copies by these 256 threads; each arrives once for every product.
     auto load_low = [&](const Tile& tile, int product) {
@@ -1067,7 +1083,6 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
       if (mine && warp == 0) multiply(product);
       if (mine && !wait(&ready, product)) break;
       if (kScaled<T> && mine && !wait(&loaded[product & 1], product >> 1)) break;  // long there: for the rows' powers
-      products = next_product;
       if (!early) load(next, next_product);
       check(next_token);
       tc_fence_after();
@@ -1124,12 +1139,22 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
     cp_async_commit();
     cp_async_wait<0>();
   }
-  if (abort != 0 && tid == 0 && products > 0) mbar_drain(&ready, static_cast<uint32_t>(products - 1) & 1);
+  if (abort != 0 && tid == 0 && issued > 0) mbar_drain(&ready, static_cast<uint32_t>(issued - 1) & 1);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 0) tmem_dealloc(accumulator, S::kColumns);
+  if (abort == 0) return;
+  const int columns = min(S::kColumns, width - column0);
+  for (int t = first; t < last; ++t) {
+    const Tile tile = p.tiles[t];
+    for (int i = tid; i < tile.count * columns; i += S::kThreads) {
+      const int64_t token = token_of(p, tile.start + i / columns);
+      T* row = static_cast<T*>(p.out) + token * p.out_stride + column0;
+      if (token >= 0) row[i % columns] = from_float<T>(__int_as_float(0x7fffffff));
+    }
+  }
 }
 
 // ------------------------------------------------------------------- outer ----
@@ -1241,7 +1266,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2) adapter_outer(AdapterParams
     const int fills = last - first;
     if constexpr (!kScaled<T>) {
       for (int fill = 0; fill < fills; ++fill) {
-        if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p.watchdog)) break;
+        if (fill >= S::kStages && !ring.wait(ring.used, fill - S::kStages, p)) break;
         copy_rows(fill);
         copy_low(fill);
         ring.filled<FAST>(fill);
@@ -1288,7 +1313,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2) adapter_outer(AdapterParams
       for (int fill = 0; fill < fills; ++fill) {
         const int ahead = fill + kAhead;
         if (ahead < fills) {
-          if (ahead >= S::kStages && !ring.wait(ring.used, ahead - S::kStages, p.watchdog)) break;
+          if (ahead >= S::kStages && !ring.wait(ring.used, ahead - S::kStages, p)) break;
           copy_rows(ahead);
           copy_low(ahead);
         }
@@ -1331,7 +1356,7 @@ __global__ void __launch_bounds__(kTensorThreads, 2) adapter_outer(AdapterParams
     // Groups of 8 slots are 1024 bytes apart, runs of 64 columns kSubBytes.
     const uint64_t a = smem_desc(stages, S::kSubBytes, 1024, 2);
     const uint64_t b = smem_desc(stages + S::kRowBytes, 128, S::kPanelBytes, 0);
-    ring.multiply(last - first, p.watchdog, [&](int fill) {
+    ring.multiply(last - first, p, [&](int fill) {
       // Addresses advance in the descriptors' units of 16 bytes.
       const uint64_t stage = static_cast<uint64_t>(fill % S::kStages) * (S::kStageBytes / 16);
 #pragma unroll
@@ -1345,13 +1370,13 @@ __global__ void __launch_bounds__(kTensorThreads, 2) adapter_outer(AdapterParams
     });
   }
   float* part = reinterpret_cast<float*>(shared);
-  if (first < last) ring.wait(ring.used, last - 1 - first, p.watchdog);
+  if (first < last) ring.wait(ring.used, last - 1 - first, p);
   tc_fence_after();
   __syncthreads();
   if (warp < 8) {
     const int half = warp / 4, c = half * 128 + warp % 4 * 32 + lane;
     store_part<RANK, 2>(part + c * S::kPartPitch, accumulator + (static_cast<uint32_t>(warp % 4) << 21) + half * 2 * RANK,
-                        first < last, power_of_two(back));
+                        first < last && !ring.gave_up(), ring.instead(), power_of_two(back));
   }
   tc_fence_before();
   cluster_sync();
@@ -1421,6 +1446,15 @@ int check_adapters(int dtype, int64_t tokens, int64_t width, int rank, int adapt
   SDC_REQUIRE(width > 0 && width < INT_MAX - 512, "low-rank adapter widths must be positive and fit padded int32 extents");
   SDC_REQUIRE(rank >= 1 && rank <= kMaxRank, "low-rank adapters take ranks of 1 to 256");
   SDC_REQUIRE(adapters >= 1 && adapters <= 65535, "low-rank adapters take 1 to 65535 adapters");
+  return SDC_OK;
+}
+
+int set_watchdog(AdapterParams& p) {
+  p.watchdog = watchdog_ptr();
+  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
+  const WatchdogSettings watch = watchdog_settings();
+  p.wait_limit_ns = watch.wait_limit_ns;
+  p.expire = watch.pace_extra > 0;
   return SDC_OK;
 }
 
@@ -1585,8 +1619,8 @@ int sdc_adapter_shrink(int dtype, const void* x, int64_t x_stride, int64_t token
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
-  p.watchdog = watchdog_ptr();
-  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
+  rc = set_watchdog(p);
+  if (rc != SDC_OK) return rc;
   p.rows_in = x;
   p.row_stride = x_stride;
   p.tokens = tokens;
@@ -1623,8 +1657,8 @@ int sdc_adapter_expand(int dtype, const void* base, int64_t base_stride, int64_t
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
-  p.watchdog = watchdog_ptr();
-  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
+  rc = set_watchdog(p);
+  if (rc != SDC_OK) return rc;
   p.tokens = tokens;
   p.rows = rows;
   p.tiles = reinterpret_cast<const Tile*>(tiles);
@@ -1660,8 +1694,8 @@ int sdc_adapter_outer(int dtype, const void* x, int64_t x_stride, int64_t tokens
   rc = check_current_device();
   if (rc != SDC_OK) return rc;
   AdapterParams p{};
-  p.watchdog = watchdog_ptr();
-  if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "low-rank adapters have no watchdog word on this device");
+  rc = set_watchdog(p);
+  if (rc != SDC_OK) return rc;
   p.rows_in = x;
   p.row_stride = x_stride;
   p.tokens = tokens;

@@ -67,6 +67,8 @@ enum WatchdogCode : int32_t {
   kWaitProjection = 6, // K-slice projection waiting for its A rows
   kWaitGrid = 7,       // prediction warps waiting at the grid-wide barrier
   kWaitPace = 8,       // prediction warps waiting for the epilogue's progress
+  kWaitAdapters = 9,   // low-rank adapters
+  kWaitDistill = 10,   // distillation loss with gradient
 };
 
 // 2 seconds of globaltimer nanoseconds; a healthy wait ends in microseconds.
@@ -74,7 +76,8 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 // Per-launch watchdog parameters: the wait limit, and a pacing offset that
 // only the test hook sdc_test_set_watchdog changes (it makes the prediction
-// warps' pacing wait unreachable, so a test can watch a bounded wait expire).
+// warps' pacing wait unreachable, so a test can watch a bounded wait expire;
+// the layer operators wait for a barrier that nothing arrives at instead).
 struct WatchdogSettings {
   uint64_t wait_limit_ns;
   int32_t pace_extra;

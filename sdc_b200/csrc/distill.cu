@@ -70,6 +70,8 @@ struct DistillParams {
   int slice;                // 16-byte words of a row per block
   int chunks;               // backward: blocks per row
   int32_t* watchdog;
+  uint64_t wait_limit_ns;
+  bool expire;              // test hook: a wait that nothing ends
   int64_t rows;             // loss with gradient: rows and log2 of the hash table's size
   int hash_bits;
 };
@@ -500,6 +502,7 @@ struct GradBarriers {
   uint64_t empty[kChunks];  // every streaming warp has read the chunk for the last time
   uint64_t joined;          // every streaming warp's pair is there, and the list has been read
   uint64_t exchanged[2];    // the pairs of all blocks, of alternate rows
+  uint64_t never;
 };
 
 enum RowState : int { kEmptyList = 1, kStrayIndex = 2 };
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
   __shared__ GradBarriers bars;
   __shared__ int states[2];
   __shared__ float upstream[2];
-  __shared__ int32_t abort;
+  __shared__ int32_t abort, cluster_abort;
   __shared__ float2 warp_parts[kRowThreads / 32];
   __shared__ float2 parts[2][kMaxCluster];
   constexpr int kPer = 16 / sizeof(T);
@@ -578,16 +581,18 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
       mbar_init(&bars.exchanged[i], 1);
       mbar_arrive_expect_tx(&bars.exchanged[i], exchange_bytes);
     }
+    mbar_init(&bars.never, 1);
     fence_barrier_init();
-    abort = 0;
+    abort = cluster_abort = 0;
   }
   cluster_sync();
 
   // False for the whole warp once a wait of the block has run out. Every wait
   // is of this kind, so the warps then leave their loops one after the other
-  // and meet at the cluster's last barrier.
+  // and meet at the cluster's last barrier, behind which all of the cluster's
+  // rows become NaN.
   auto wait = [&](uint64_t* bar, uint32_t phase) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, phase, kWaitOther, &abort, p.watchdog)) != 0;
+    return __all_sync(0xffffffffu, mbar_wait(bar, phase, kWaitDistill, &abort, p.watchdog, p.wait_limit_ns)) != 0;
   };
   auto words_of = [&](int64_t row) {
     return RowWords<T>(static_cast<const T*>(p.logits) + row * p.row_stride, static_cast<int>(p.vocab),
@@ -646,6 +651,7 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
     }
     uint32_t turn = 0;
     for (int64_t row = first_row; row < p.rows; row += clusters, ++turn) {
+      if (p.expire && !wait(&bars.never, 0)) break;
       const Entry* list = lists_of[turn & 1];
       const bool some = !teacher.empty;
       const RowWords<T> in = words_of(row);
@@ -782,7 +788,25 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
     }
   }
   __syncwarp();
+  if (abort != 0 && lane < static_cast<int>(ranks)) {
+    const uint32_t to = mapa_shared(&cluster_abort, static_cast<uint32_t>(lane));
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(1) : "memory");
+  }
   cluster_sync();  // the other blocks may still be sending their pairs
+  if (cluster_abort == 0) return;
+  const float nan = __int_as_float(0x7fffffff);
+  float nans[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) nans[i] = nan;
+  for (int64_t row = first_row; row < p.rows; row += clusters) {
+    const RowWords<T> in = words_of(row);
+    T* grad = static_cast<T*>(p.grad) + row * p.grad_stride;
+    for (int w = tid; w < in.count; w += kRowBlock) in.store(grad, false, w, pack_word<T>(nans));
+    if (rank == 0 && tid == 0) {
+      p.loss[row] = nan;
+      p.stats[row] = make_float4(nan, nan, nan, nan);
+    }
+  }
 }
 
 // The gradient from the row statistics: one read, one write, blocks of a row
@@ -1018,6 +1042,9 @@ int run_rows(DistillParams p, int dtype, int64_t rows, int cluster, cudaStream_t
   p.hash_bits = hash_bits(p.top);
   p.watchdog = watchdog_ptr();
   if (p.watchdog == nullptr) return fail(SDC_ERR_CUDA, "distillation has no watchdog word on this device");
+  const WatchdogSettings watch = watchdog_settings();
+  p.wait_limit_ns = watch.wait_limit_ns;
+  p.expire = watch.pace_extra > 0;
   const size_t shared = shared_bytes(p.vocab, dtype, p.top, cluster, GRAD);
   if (dtype == kF32) return launch_rows<float, GRAD>(p, rows, cluster, shared, stream);
   if (dtype == kBF16) return launch_rows<__nv_bfloat16, GRAD>(p, rows, cluster, shared, stream);

@@ -6,12 +6,14 @@ that run out, and walks of many rows, tiles and tokens by one block.
 Tolerances as in the operators' other tests: one rounding to the output's type
 plus a power of two times the sum of the magnitudes that enter an element.
 """
+import ctypes
 import threading
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from sdc_b200 import capi
 from sdc_b200.layers import (AdapterBatch, distillation_loss, distillation_loss_and_grad, head_norm_rotary,
                              low_rank_adapters, low_rank_adapters_, rotary_table)
 
@@ -318,3 +320,97 @@ def test_fp16_adapters_add_tokens_of_unlike_sizes():
         for got, (value, magnitude), lengths in zip((out.detach(), dx, da[0], db[0]), adapters64(x, base, a[0], b[0], grad),
                                                     ((136, 40), (264, 40), (264, tokens), (136, tokens))):
             close(got, value, magnitude, fp16_arithmetic(*lengths))
+
+
+# ------------------------------------------------------------- expired waits ----
+
+WAIT_ADAPTERS, WAIT_DISTILL = 9, 10  # codes of the device watchdog
+
+
+def _watchdog():
+    code = ctypes.c_int32(-1)
+    capi.check(capi.lib().sdc_read_device_error(torch.cuda.current_stream().cuda_stream, ctypes.byref(code)))
+    return code.value
+
+
+def _expired(call):
+    """The call's result where a wait runs out after a millisecond (one for a barrier that nothing arrives at)."""
+    try:
+        capi.check(capi.lib().sdc_test_set_watchdog(1_000_000, 1))
+        result = call()
+        torch.cuda.synchronize()
+    finally:
+        capi.check(capi.lib().sdc_test_set_watchdog(0, 0))
+    return result
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapters_report_an_expired_wait_in_their_results(dtype):
+    g = rng(9)
+    lengths, adapters = [1300, 40, 700], [0, -1, 1]
+    tokens, batch = sum(lengths), AdapterBatch(lengths, adapters, 3)
+    x, base, grad = (normal(g, tokens, w, dtype=dtype) for w in (264, 520, 520))
+    a, b = normal(g, 3, 24, 264, dtype=dtype), normal(g, 3, 520, 24, dtype=dtype)
+    adapted = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    adapted[1300:1340] = False
+
+    def call():
+        leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+        out = low_rank_adapters(base, *leaves, batch)
+        return (out, *torch.autograd.grad(out, leaves, grad))
+
+    assert _watchdog() == 0
+    want = call()
+    out, dx, da, db = _expired(call)
+    assert out[adapted].isnan().all() and dx[adapted].isnan().all()
+    assert da[:2].isnan().all() and db[:2].isnan().all() and not da[2].any() and not db[2].any()
+    assert _watchdog() == WAIT_ADAPTERS
+    assert low_rank_adapters_(base.clone(), x, a, b, batch).isfinite().all()
+    in_place = _expired(lambda: low_rank_adapters_(base.clone(), x, a, b, batch))
+    assert in_place[adapted].isnan().all()
+    assert torch.equal(in_place[~adapted], base[~adapted])
+    assert _watchdog() == WAIT_ADAPTERS
+
+    # Each kernel by itself, on whole operands.
+    rows, groups, tiles, slots, active, tile_rows = batch.arguments(24)
+    assert tile_rows == 128
+    low = torch.ops.sdc_cutlass.low_rank_adapters(base, x, a, b, None, *batch.arguments(24))[1]
+    code, stream = {torch.bfloat16: 1, torch.float16: 2}[dtype], torch.cuda.current_stream().cuda_stream
+    expanded, outer = torch.zeros_like(base), torch.zeros_like(b)
+
+    def expand():
+        capi.check(capi.lib().sdc_adapter_expand(code, base.data_ptr(), 520, tokens, rows.data_ptr(), tiles.data_ptr(), active,
+                                                 128, b.data_ptr(), 3, 24, 520, 1, low.data_ptr(), slots, 0,
+                                                 expanded.data_ptr(), 520, stream))
+        return expanded
+
+    def products():
+        capi.check(capi.lib().sdc_adapter_outer(code, grad.data_ptr(), 520, tokens, rows.data_ptr(), groups.data_ptr(), 3,
+                                                low.data_ptr(), slots, 24, 520, 1, outer.data_ptr(), stream))
+        return outer
+
+    assert _expired(expand)[adapted].isnan().all() and not expanded[~adapted].any()
+    assert _expired(products)[:2].isnan().all() and not outer[2].any()
+    assert _watchdog() == WAIT_ADAPTERS
+    assert torch.equal(expand()[adapted], want[0][adapted]) and torch.equal(products(), want[3])
+    for got, expected in zip(call(), want):
+        assert torch.equal(got, expected)
+    assert _watchdog() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_reports_an_expired_wait_in_its_results(dtype):
+    g = rng(10)
+    for rows, vocab in ((5, 3001), (700, 513)):  # clusters of several blocks, and several rows a cluster
+        logits, teacher = normal(g, rows, vocab, dtype=dtype), normal(g, rows, 8)
+        indices = torch.randint(0, vocab, (rows, 8), device=DEV, generator=g)
+        indices[1] = -1
+        want = distillation_loss_and_grad(logits, indices, teacher)
+        assert _watchdog() == 0
+        for in_place in (False, True):
+            loss, grad = _expired(lambda: distillation_loss_and_grad(logits.clone(), indices, teacher, in_place=in_place))
+            assert loss.isnan().all() and grad.isnan().all()
+            assert _watchdog() == WAIT_DISTILL
+        for got, expected in zip(distillation_loss_and_grad(logits, indices, teacher), want):
+            assert torch.equal(got, expected)
+        assert _watchdog() == 0
