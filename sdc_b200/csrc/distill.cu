@@ -632,6 +632,9 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
       }
       if (read && from < to) {
         const uint32_t bytes = static_cast<uint32_t>(to - from) * 16;
+        // The chunk's last row was read, and words at its ends written, by
+        // ordinary accesses; rows start elsewhere in their words.
+        fence_proxy_async_smem();
         mbar_arrive_expect_tx(&bars.full[i], bytes);
         asm volatile(
             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(

@@ -414,3 +414,57 @@ def test_distillation_reports_an_expired_wait_in_its_results(dtype):
         for got, expected in zip(distillation_loss_and_grad(logits, indices, teacher), want):
             assert torch.equal(got, expected)
         assert _watchdog() == 0
+
+
+# -------------------------------------------------------------------- walks ----
+# Blocks that stay for the whole launch walk over tokens, tiles or rows. Here each of them has several.
+
+def _sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("rows,vocab,top,dtype", [(2000, 513, 16, torch.bfloat16), (1999, 514, 16, torch.float32),
+                                                  (700, 50021, 33, torch.float32), (300, 151937, 64, torch.bfloat16),
+                                                  (2100, 4099, 200, torch.float16)])
+def test_distillation_walks_many_rows(rows, vocab, top, dtype):
+    """Odd vocabularies (rows start elsewhere in their words), rows without entries and with stray ones between others."""
+    g = rng(rows)
+    logits, teacher = normal(g, rows, vocab, dtype=dtype, scale=3.0), normal(g, rows, top, scale=3.0)
+    indices = torch.randint(0, vocab, (rows, top), device=DEV, generator=g)
+    indices[torch.rand(rows, top, device=DEV, generator=g) < 0.2] = -1
+    kind = torch.rand(rows, device=DEV, generator=g)
+    empty, stray = kind < 0.2, kind > 0.95
+    indices[empty] = -1
+    logits[empty] = float("nan")  # of which nothing is looked at
+    indices[stray, 0] = vocab
+    # At most three blocks stay on an SM; a row's words fill as many blocks of 74 KB as it takes.
+    assert rows > 3 * _sms() / max(1, vocab * logits.element_size() // (74 * 1024)) * 2
+    upstream = normal(g, rows)
+    loss, grad = distillation_loss_and_grad(logits, indices, teacher, 1.5, upstream)
+    replaced = logits.clone()
+    again = distillation_loss_and_grad(replaced, indices, teacher, 1.5, upstream, in_place=True)
+    good = ~stray
+    for first, second in ((loss, again[0]), (grad, replaced)):
+        assert torch.equal(first[good], second[good])
+        assert first[stray].isnan().all() and second[stray].isnan().all()
+        assert not first[empty].any()
+    kept = indices >= 0
+    for start in range(0, rows, 200):
+        part = slice(start, start + 200)
+        some = good[part] & ~empty[part]
+        s, t, at = logits[part][some].double() / 1.5, teacher[part][some].double() / 1.5, indices[part][some]
+        log_q = torch.log_softmax(s, 1)
+        log_p = torch.log_softmax(t.masked_fill(at < 0, -float("inf")), 1)
+        p = log_p.exp()
+        chosen = log_q.gather(1, at.clamp_min(0))
+        exact = torch.where(at >= 0, p * (log_p - chosen), 0.0).sum(1) * 2.25
+        size = torch.where(at >= 0, p * (log_p.abs() + chosen.abs() + 1), 0.0).sum(1) * 2.25
+        assert ((loss[part][some].double() - exact).abs() <= 2.0 ** -24 * exact.abs() + 2.0 ** -17 * size).all()
+        spread = torch.zeros_like(s).scatter_add_(1, at.clamp_min(0), torch.where(at >= 0, p, 0.0))
+        row = upstream[part][some].double()[:, None] * 1.5
+        q = log_q.exp()
+        exact, size = (q - spread) * row, (q + spread) * row.abs()
+        unit = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}[dtype]
+        tolerance = unit * exact.abs() * (1 + 2.0 ** -10) + (2.0 ** -25 if dtype == torch.float16 else 1e-38) + 2.0 ** -17 * size
+        assert ((grad[part][some].double() - exact).abs() <= tolerance).all()
+    assert kept[good & ~empty].any(1).all()
