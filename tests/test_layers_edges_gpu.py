@@ -13,6 +13,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import test_layers_gpu as layers
 from sdc_b200 import capi
 from sdc_b200.layers import (AdapterBatch, distillation_loss, distillation_loss_and_grad, head_norm_rotary,
                              low_rank_adapters, low_rank_adapters_, rotary_table)
@@ -468,3 +469,74 @@ def test_distillation_walks_many_rows(rows, vocab, top, dtype):
         tolerance = unit * exact.abs() * (1 + 2.0 ** -10) + (2.0 ** -25 if dtype == torch.float16 else 1e-38) + 2.0 ** -17 * size
         assert ((grad[part][some].double() - exact).abs() <= tolerance).all()
     assert kept[good & ~empty].any(1).all()
+
+
+@pytest.mark.parametrize("lengths,ids,count,rank,k,n", [
+    ([700, 300, 37, 900, 128, 1100], [0, 1, -1, 2, 0, 1], 4, 16, 136, 18944),   # two weights
+    ([700, 300, 37, 900, 128, 1100], [0, 1, -1, 2, 0, 1], 4, 48, 18944, 136),
+    ([2000, 30, 1500], [0, -1, 2], 3, 64, 136, 18944),                          # one
+    ([130, 140, 1900, 150, 800], [3, 0, 1, 2, -1], 4, 128, 18941, 37),          # no vector form
+    ([130, 140, 1900, 150, 800], [3, 0, 1, 2, -1], 4, 24, 37, 18941),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapters_walk_many_tiles(lengths, ids, count, rank, k, n, dtype):
+    g = rng(rank)
+    tokens, batch = sum(lengths), AdapterBatch(lengths, ids, count)
+    x, base, grad = (normal(g, tokens, w, dtype=dtype) for w in (k, n, n))
+    a, b = normal(g, count, rank, k, dtype=dtype, scale=k ** -0.5), normal(g, count, n, rank, dtype=dtype, scale=rank ** -0.5)
+    scale = torch.rand(count, device=DEV, generator=g) + 0.5
+    tiles, tile_rows = batch.arguments(rank)[2], batch.arguments(rank)[5]
+    # Blocks of 256 columns, at most two on an SM.
+    assert tile_rows == 128 and len(tiles) > 2 * (2 * _sms() // -(-max(k, n) // 256))
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    out = low_rank_adapters(base, *leaves, batch, scale)
+    dx, da, db = torch.autograd.grad(out, leaves, grad)
+    in_place = low_rank_adapters_(base.clone(), x, a, b, batch, scale)
+    assert torch.equal(in_place, out)
+    exact, size, parts = layers.adapters64(lengths, ids, x, base, a, b, scale, grad)
+    layers.close(out.detach(), exact, size, layers.adapter_arithmetic(k, rank))
+    layers.close(dx, parts[0], parts[1], layers.adapter_arithmetic(n, rank))
+    layers.close(da, parts[2], parts[3], layers.adapter_arithmetic(n, tokens))
+    layers.close(db, parts[4], parts[5], layers.adapter_arithmetic(k, tokens))
+
+
+# batch, sequence, heads, kv heads, dim, rotary, interleaved, norm, fp32 weights: groups of lanes walk several tokens in
+# whole runs (a few pieces or many of a token on their way), and without the vector form.
+@pytest.mark.parametrize("case,dtype", [
+    ((2, 8192, 14, 2, 64, 64, False, True, False), torch.bfloat16), ((1, 16385, 28, 4, 64, 32, False, True, True), torch.float16),
+    ((1, 9001, 14, 2, 80, 40, True, True, False), torch.float32), ((1, 16000, 14, 3, 34, 10, False, True, True), torch.bfloat16),
+    ((3, 3001, 28, 4, 128, 128, True, True, False), torch.bfloat16), ((1, 9001, 14, 2, 128, 128, False, False, False), torch.float32)])
+def test_head_norm_rotary_walks_many_tokens(case, dtype):
+    batch, sequence, heads, kv, dim = case[:5]
+    lanes = 1
+    while 16 * lanes < dim:
+        lanes *= 2
+    # Two blocks of 256 threads on an SM; a group takes four heads at most.
+    assert batch * sequence * (-(-heads // 4) + -(-kv // 4)) > 2 * (2 * _sms() * 256 // lanes)
+    q, k, table, positions, weights, interleaved = layers._rotary_inputs(case, dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, *weights) if t is not None]
+    q_weight, k_weight = leaves[2:] or (None, None)
+    out = head_norm_rotary(leaves[0], leaves[1], table, positions, q_weight, k_weight, 1e-6, interleaved)
+    g = rng(1)
+    upstream = [normal(g, *o.shape, dtype=dtype) for o in out]
+    grads = torch.autograd.grad(out, leaves, upstream)
+    angles = table.double()[positions][:, :, None]
+    half = table.shape[1] // 2
+    for i in range(2):
+        exact = [t.detach().double().requires_grad_() for t in ([leaves[i]] + ([leaves[2 + i]] if len(leaves) > 2 else []))]
+        weight = exact[1] if len(exact) > 1 else None
+        reference, magnitude = layers.rotary64(exact[0], table, positions, weight, 1e-6, interleaved)
+        layers.close(out[i].detach(), reference.detach(), magnitude.detach(), 2.0 ** -19)
+        expected = torch.autograd.grad(reference, exact, upstream[i].double())
+        size = upstream[i].double().abs()
+        turned = layers.rotate64(size, angles[..., :half].abs(), -angles[..., half:].abs(), table.shape[1], interleaved).abs() + size
+        if weight is None:
+            layers.close(grads[i], expected[0], turned, 2.0 ** -19)
+            continue
+        x = exact[0].detach()
+        r = torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+        gw, u = turned * weight.detach().abs(), (x * r).abs()
+        layers.close(grads[i], expected[0], r * (gw + u * (gw * u).mean(-1, keepdim=True)), 2.0 ** -18)
+        # A weight's gradient is a sum of fp32 chains: a thread's tokens and heads, a block's groups, a strand's blocks, 32
+        # strands: less than 256 additions deep.
+        layers.close(grads[2 + i], expected[1], (turned * u).sum((0, 1, 2)), 2.0 ** -16)
