@@ -1463,10 +1463,51 @@ int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
 bool vector_rows(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
-// Clusters of 1, 2, ... 16 blocks that run at once when an SM holds two blocks
-// (the driver's occupancy figures on a B200 of 148 SMs; another layout of the
-// SMs costs time, not results).
-constexpr int kClusterRoom[kMaxSplit + 1] = {0, 296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14};
+// Stands in for the kernels of clusters where the runtime is asked how many run
+// at once: of kernels that allocate tensor memory it assumes one block an SM. It
+// is never launched.
+__global__ void __launch_bounds__(kTensorThreads, 2) cluster_probe(AdapterParams) {}
+
+int ask_clusters(int size, int shared) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(size));
+  config.blockDim = dim3(kTensorThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(shared);
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attribute[0].val.clusterDim.y = 1;
+  attribute[0].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if (allow_shared(reinterpret_cast<const void*>(cluster_probe), shared) != SDC_OK ||
+      (size > kPortableSplit &&
+       cudaFuncSetAttribute(cluster_probe, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+      cudaOccupancyMaxActiveClusters(&clusters, cluster_probe, &config) != cudaSuccess) {
+    cudaGetLastError();  // no cluster of that size here, and no error of the call's
+    return 0;
+  }
+  return clusters;
+}
+
+// Clusters of `size` blocks that run at once when an SM holds two blocks (100 KB
+// of shared memory), 0 where the device has none. Those beyond the portable size
+// must also fit with one block an SM. Asked of the runtime once for each device
+// and size. B200 with 148 SMs: 296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21,
+// 17, 14, 14 and 14 of 1 to 16 blocks.
+int cluster_room(int size) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][kMaxSplit + 1] = {};  // 0: not asked yet, else 1 more
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) return 0;
+  int room = known[device][size].load(std::memory_order_relaxed) - 1;
+  if (room < 0) {
+    room = size <= kPortableSplit || ask_clusters(size, 150 * 1024) > 0 ? ask_clusters(size, 100 * 1024) : 0;
+    known[device][size].store(room + 1, std::memory_order_relaxed);
+  }
+  return room;
+}
 
 // Blocks that share a tile's sum: as many as fill the SMs' `resident` blocks
 // each once, as long as each keeps two chunks (four of more than eight blocks),
@@ -1480,7 +1521,7 @@ int split_count(int64_t clusters, int64_t chunks, int resident, int most) {
   const int64_t wanted = std::min<int64_t>(static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(clusters, 1), chunks / 2);
   int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, most)));
   if (split > kPortableSplit && chunks / split < 4) split = kPortableSplit;
-  while (split > 1 && clusters > kClusterRoom[split] * resident / 2) --split;
+  while (split > 1 && clusters > static_cast<int64_t>(cluster_room(split)) * resident / 2) --split;
   return split;
 }
 
