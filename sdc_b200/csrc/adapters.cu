@@ -1442,7 +1442,8 @@ int launch_clustered(Kernel kernel, const AdapterParams& p, dim3 grid, int threa
 
 int check_adapters(int dtype, int64_t tokens, int64_t width, int rank, int adapters) {
   SDC_REQUIRE(dtype == kBF16 || dtype == kF16, "low-rank adapters compute BF16 (1) or FP16 (2)");
-  SDC_REQUIRE(tokens >= 0 && tokens < INT_MAX - 128, "low-rank adapters take fewer than 2^31 - 128 tokens");
+  // Slots are looked up ahead in 32 bits, up to 576 of them.
+  SDC_REQUIRE(tokens >= 0 && tokens <= INT_MAX - 1024, "low-rank adapters take fewer than 2^31 - 1024 tokens");
   SDC_REQUIRE(width > 0 && width < INT_MAX - 512, "low-rank adapter widths must be positive and fit padded int32 extents");
   SDC_REQUIRE(rank >= 1 && rank <= kMaxRank, "low-rank adapters take ranks of 1 to 256");
   SDC_REQUIRE(adapters >= 1 && adapters <= 65535, "low-rank adapters take 1 to 65535 adapters");

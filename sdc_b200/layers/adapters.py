@@ -54,8 +54,8 @@ class AdapterBatch:
         if lengths.size and (lengths.min() < 0 or adapters.min() < -1 or adapters.max() >= count):
             raise ValueError("AdapterBatch lengths must not be negative and adapters must be -1 or below count")
         tokens = int(lengths.sum())
-        if tokens >= 2 ** 31 - 128:
-            raise ValueError("AdapterBatch takes fewer than 2^31 - 128 tokens")
+        if tokens >= 2 ** 31 - 1024:
+            raise ValueError("AdapterBatch takes fewer than 2^31 - 1024 tokens")
         of_token = np.repeat(np.where(adapters < 0, count, adapters), lengths)
         offsets = np.concatenate(([0], np.cumsum(np.bincount(of_token, minlength=count + 1))))[:count + 1]
         slots = int(offsets[-1])
