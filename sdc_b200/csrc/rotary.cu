@@ -161,16 +161,18 @@ struct HeadIO {
       }
     }
   }
-  __device__ __forceinline__ void store(T* head, const float* v) const {
+  // Pairs that pass together come from `passed`.
+  __device__ __forceinline__ void store(T* head, const float* v, const float* passed) const {
     if constexpr (VECTOR) {
       float a[8], b[8];
+      const float* r = kTogether ? passed : v;  // runs
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool runs = !split;
-        a[2 * i] = runs ? v[i] : v[2 * i];
-        a[2 * i + 1] = runs ? v[8 + i] : v[2 * i + 1];
-        b[2 * i] = runs ? v[4 + i] : v[8 + 2 * i];
-        b[2 * i + 1] = runs ? v[12 + i] : v[8 + 2 * i + 1];
+        a[2 * i] = runs ? r[i] : v[2 * i];
+        a[2 * i + 1] = runs ? r[8 + i] : v[2 * i + 1];
+        b[2 * i] = runs ? r[4 + i] : v[8 + 2 * i];
+        b[2 * i + 1] = runs ? r[12 + i] : v[8 + 2 * i + 1];
       }
       store8(head + low_run, pack8<T>(a));
       store8(head + high_run, pack8<T>(b));
@@ -245,17 +247,17 @@ __device__ __forceinline__ void load_angles(const RotaryParams& p, int64_t posit
 
 // Turns the lane's pairs by their angles, or (BACK) by their opposites. Pairs
 // that pass are kept apart: a product with a sine of 0 would carry an infinity
-// or a NaN of one element over to the other.
+// or a NaN of one element over to the other. Where a lane's pairs pass together
+// the caller keeps v instead.
 template <bool BACK, typename IO>
-__device__ __forceinline__ void turn(const IO& io, const Angles& a, float* v) {
-  if (IO::kTogether && !io.split) return;
+__device__ __forceinline__ void turn(const IO& io, const Angles& a, const float* v, float* out) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool passes = !IO::kTogether && __float_as_uint(a.sine[i]) == kPasses;
     const float sine = BACK ? -a.sine[i] : a.sine[i];
     const float x = v[i], y = v[8 + i];
-    v[i] = x * a.cosine[i] - (passes ? 0.f : y) * sine;
-    v[8 + i] = y * a.cosine[i] + (passes ? 0.f : x) * sine;
+    out[i] = x * a.cosine[i] - (passes ? 0.f : y) * sine;
+    out[8 + i] = y * a.cosine[i] + (passes ? 0.f : x) * sine;
   }
 }
 
@@ -368,8 +370,9 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
         for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
       }
       if (!mine) continue;
-      turn<false>(walk.io, angles, v);
-      walk.io.store(y + h * p.dim, v);
+      float out[16];
+      turn<false>(walk.io, angles, v, out);
+      walk.io.store(y + h * p.dim, out, v);
     }
   }
 }
@@ -420,7 +423,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
       float v[16], g[16];
       if (mine) {
         walk.io.unpack(walk.head(round, 1, p.dy[role], p.dys[role], h), g);
-        turn<true>(walk.io, angles, g);
+        if (!W::IO::kTogether || walk.io.split) turn<true>(walk.io, angles, g, g);
       }
       if (norm) {
         float squares = 0.f, products = 0.f;
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward
           }
         }
       }
-      if (mine) walk.io.store(dx + h * p.dim, g);
+      if (mine) walk.io.store(dx + h * p.dim, g, g);
     }
   }
   if (p.partials == nullptr) return;
