@@ -863,7 +863,7 @@ __global__ void __launch_bounds__(NarrowExpand::kThreads, 4) adapter_expand(Adap
 // used, its low rows (and weight, if another) while the current tile is worked
 // on. Bound by base and out: 16384 x 3584 bf16, rank 32, 49 us (4.8 TB/s; each
 // further 16384 rows take 40, 5.8 TB/s), rank 64 63 us (register accumulators
-// and mma.sync: 80); 8191 x 18944 fp16 of 23 ragged adapters 123 us (5.0 TB/s).
+// and mma.sync: 80); 8191 x 18944 fp16 of 23 ragged adapters 122 us (5.0 TB/s).
 // Blocks of 128 columns, two or three to an SM, took 58 and 66 us for the
 // first; runs half as long, in two waves, 57, though 4 % less where ragged
 // adapters leave the runs uneven.
@@ -1165,10 +1165,11 @@ __global__ void __launch_bounds__(ExpandWide::kThreads, 2) adapter_expand_wide(A
 // side by side are B (in panels), so that A, whose reading takes longer than
 // the product, is read once; the planes' sums are added at the end. Each block
 // takes about 0.43 us for a stage of 16 KB, with one or two blocks on the SM
-// and 4 or 5 stages. 16384 x 3584 bf16, rank 32, 4 adapters: 34 us (3.5 TB/s),
-// 40 in a backward pass, where earlier writes are still leaving L2; each
-// further 16384 rows take 24 (4.9 TB/s). Register accumulators took 68. A block takes 256 columns and RANK ranks; the blocks of a
-// cluster share the adapter's tokens.
+// and 4 or 5 stages. 16384 x 3584 bf16, rank 32, 4 adapters: 36 us (3.3 TB/s),
+// 41 to 47 behind the product that writes dx, whose rows are still leaving L2;
+// fp16 38 and up to 51. Each further 16384 rows of bf16 take 24 (4.9 TB/s).
+// Register accumulators took 68. A block takes 256 columns and RANK ranks; the
+// blocks of a cluster share the adapter's tokens.
 // Scaled rows: the pieces of a row are read and written again by neighbouring
 // lanes, so the panels stand 128 bytes / panels further apart, on other banks.
 template <int RANK, bool SCALED>

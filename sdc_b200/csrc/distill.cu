@@ -79,6 +79,8 @@ struct DistillParams {
 // 1 / sum of a row without teacher entries.
 constexpr float kEmptyRow = -1.f;
 
+// A relative error of about 2^-22, as much as the rounding of the exponent adds;
+// tests hold a loss to 2^-17 of its terms.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -419,8 +421,8 @@ __device__ __forceinline__ void write_empty(const DistillParams& p, int64_t row)
 
 // The losses alone: a cluster of blocks per row streams it through registers.
 // Bound by memory: 4096 rows of 151936 bf16 take 191 us (1245 MB, 6.5 TB/s),
-// 509 rows 33.7 us (4.6 TB/s: the start and the last, partly filled wave cost
-// more of so few rows); one row 6.1 us.
+// 509 rows 33.8 us (4.6 TB/s: the start and the last, partly filled wave cost
+// more of so few rows); one row 6.0 us.
 template <typename T>
 __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams p) {
   extern __shared__ uint4 shared[];
@@ -493,10 +495,10 @@ __global__ void __launch_bounds__(kRowBlock, 4) distill_loss_rows(DistillParams 
 // the next row's at once. The list warp looks ahead for rows without entries
 // (which are not read at all), issues the copies, and after the streaming
 // warps writes the list's columns again with the teacher's part. 4096 rows of
-// 151936 bf16 take 504 us (2489 MB, 4.9 TB/s): two exponentials an element
+// 151936 bf16 take 507 us (2489 MB, 4.9 TB/s): two exponentials an element
 // keep their unit 56 % busy, and a row's exchange costs about a microsecond in
 // which its block reads but does not write. Loss and backward pass one after
-// the other take 566 us.
+// the other take 568 us.
 struct GradBarriers {
   uint64_t full[kChunks];   // the chunk's copy has arrived
   uint64_t empty[kChunks];  // every streaming warp has read the chunk for the last time
@@ -816,7 +818,7 @@ __global__ void __launch_bounds__(kRowBlock, kGradBlocks) distill_grad_rows(Dist
 // independent of each other. A warp of its own collects the block's entries of
 // the list meanwhile (their logits before they are overwritten: the gradient
 // may replace them) and writes their columns last. Bound by memory: 4096 rows
-// of 151936 bf16 take 375 us (2489 MB, 6.6 TB/s).
+// of 151936 bf16 take 377 us (2489 MB, 6.6 TB/s).
 struct BackEntry {
   float s, p;
   int at;

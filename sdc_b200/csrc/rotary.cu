@@ -320,9 +320,11 @@ struct Walk {
   }
 };
 
-// Bound by memory: 16384 tokens of 28 + 4 heads of 128 bf16 take 43.5 us
-// (268 MB, 6.2 TB/s); of 14 + 2 heads of 64 15.9 us (67 MB, half of it still in
-// L2 when the launch ends). One token takes 3.9 us, a launch.
+// Bound by memory: 16384 tokens of 28 + 4 heads of 128 bf16 take 44 us (268 MB,
+// 6.1 TB/s), without the norm 40; of 14 + 2 heads of 64 16.2 us (67 MB, half of
+// it still in L2 when the launch ends); 8192 of 28 + 4 of 128 fp32 60 us (268 MB,
+// 4.5 TB/s: groups of two heads have half the copies under way). One token takes
+// 3.7 us, a launch.
 template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int kHeads>
 __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(RotaryParams p) {
   extern __shared__ uint4 copies[];
@@ -380,10 +382,10 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_forward(
 // As the forward pass, over x and dy; a thread's 16 weight gradients stay in
 // registers for the whole launch, the block adds its groups' sums in a fixed
 // order and writes one partial per role. 16384 tokens of 28 + 4 heads of 128
-// bf16 take 95 us (403 MB, 4.2 TB/s), of 14 + 2 heads of 64 26.6 us (101 MB,
-// 3.8 TB/s): half the issue slots and half the memory's rate at two blocks an
-// SM, whose 128 registers a thread (x, dy, weights and their gradients) leave
-// no room for a third.
+// bf16 take 87 us (403 MB, 4.6 TB/s), of 14 + 2 heads of 64 26.6 us (101 MB,
+// 3.8 TB/s), 8192 of 28 + 4 of 128 fp32 108 us (3.7 TB/s): half the issue slots
+// at two blocks an SM, whose 128 registers a thread (x, dy, weights and their
+// gradients) leave no room for a third. Without the norm 49 us (268 MB, 5.5 TB/s).
 template <typename T, int LANES, bool INTERLEAVED, bool VECTOR, int kHeads>
 __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) rotary_backward(RotaryParams p) {
   extern __shared__ uint4 copies[];
