@@ -95,7 +95,7 @@ __device__ __forceinline__ int64_t token_of(const AdapterParams& p, int64_t slot
 // ------------------------------------------------------------------ shrink ----
 
 template <typename T>
-constexpr bool kScaled = std::is_same_v<T, __half>;
+constexpr bool kScaled = std::is_same_v<T, __half>;  // the rows of `low` are
 
 // N neighbouring values of a row's two planes.
 template <typename T, int N>
